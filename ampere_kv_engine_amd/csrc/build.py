@@ -28,6 +28,11 @@ PARTS_SOURCES = ("tokenwise_f32.hip", "latent_attention.hip", "selective_scan.hi
                  "recurrent_mixers.hip", "delta_rule.hip", "linear_states.hip")
 PARTS_HEADERS = ("common.h", "api_parts.h", "state_walk.h")
 PARTS_LIBRARY = "libakv_parts.so"
+# a third one: a step's layout and the drafted tokens' verification
+ROUNDS_SOURCES = ("place_tokens.hip", "verify_drafts.hip")
+ROUNDS_HEADERS = ("common.h", "api_rounds.h")
+ROUNDS_LIBRARY = "libakv_rounds.so"
+SHARED_PREFIX_SOURCE = "shared_prefix.hip"     # compiled once per head size as well
 ATTENTION_SOURCE = "attention_mfma.hip"        # compiled once per head size, into its own small library
 DEFAULT_HEAD_DIMS = (16, 32, 48, 64, 80, 96, 128, 192, 256)
 ARCH = "gfx950"
@@ -228,11 +233,76 @@ def ensure_attention(head_dim: int, verbose: bool = True) -> str:
     return attention_library_path(head_dim) or build_attention(head_dim, verbose)
 
 
+# ---- rounds of drafted tokens -----------------------------------------------------------------------------------------
+
+def _found(lib_name: str, mark_name: str, stamp: str) -> str | None:
+    for folder in (os.path.join(HERE, "_build"),
+                   os.path.join(tempfile.gettempdir(), f"akv_build_{os.getuid()}_{source_stamp()[:12]}")):
+        lib, mark = os.path.join(folder, lib_name), os.path.join(folder, mark_name)
+        if os.path.exists(lib) and os.path.exists(mark):
+            with open(mark) as handle:
+                if handle.read().strip() == stamp:
+                    return lib
+    return None
+
+
+def _build_small(sources, defines, lib_name: str, mark_name: str, stamp: str, verbose: bool) -> str:
+    """A small library from a few sources, compiled and linked by one command."""
+    hipcc = _hipcc()
+    out_dir = _build_dir()
+    started = time.time()
+    lib = os.path.join(out_dir, lib_name)
+    partial = lib + f".{os.getpid()}.tmp"
+    if verbose:
+        _log(f"compiling {', '.join(sources)} into {lib_name}")
+    cmd = [hipcc, *FLAGS, *defines, "-shared", *(os.path.join(HERE, name) for name in sources), "-o", partial]
+    result = subprocess.run(cmd, capture_output=True, text=True)
+    if result.returncode != 0:
+        raise RuntimeError(f"hipcc failed on {lib_name}:\n{result.stderr}")
+    os.replace(partial, lib)
+    with open(os.path.join(out_dir, mark_name), "w") as handle:
+        handle.write(stamp)
+    if verbose:
+        _log(f"built {lib} ({time.time() - started:.0f} s)")
+    return lib
+
+
+def rounds_library_path() -> str | None:
+    return _found(ROUNDS_LIBRARY, "stamp_rounds", source_stamp(ROUNDS_SOURCES, ROUNDS_HEADERS))
+
+
+def build_rounds(verbose: bool = True) -> str:
+    return _build_small(ROUNDS_SOURCES, (), ROUNDS_LIBRARY, "stamp_rounds", source_stamp(ROUNDS_SOURCES, ROUNDS_HEADERS), verbose)
+
+
+def ensure_rounds(verbose: bool = True) -> str:
+    return rounds_library_path() or build_rounds(verbose)
+
+
+def _shared_prefix_names(head_dim: int) -> tuple[str, str, str]:
+    return (f"libakv_shared_prefix_d{head_dim}.so", f"stamp_shared_prefix_d{head_dim}", source_stamp((SHARED_PREFIX_SOURCE,), ("common.h",)))
+
+
+def shared_prefix_library_path(head_dim: int) -> str | None:
+    return _found(*_shared_prefix_names(head_dim))
+
+
+def build_shared_prefix(head_dim: int, verbose: bool = True) -> str:
+    if head_dim % 16 or not 16 <= head_dim <= 256:
+        raise ValueError(f"attention over a shared prompt takes head sizes that are multiples of 16 up to 256, not {head_dim}")
+    return _build_small((SHARED_PREFIX_SOURCE,), (f"-DAKV_HEAD_DIM={head_dim}",), *_shared_prefix_names(head_dim), verbose)
+
+
+def ensure_shared_prefix(head_dim: int, verbose: bool = True) -> str:
+    return shared_prefix_library_path(head_dim) or build_shared_prefix(head_dim, verbose)
+
+
 def build_all(head_dims=DEFAULT_HEAD_DIMS, verbose: bool = True) -> list[str]:
-    """The kernel library and the attention libraries of the usual head sizes."""
-    paths = [build(verbose), build_parts(verbose)]
+    """The kernel libraries and the attention libraries of the usual head sizes."""
+    paths = [build(verbose), build_parts(verbose), build_rounds(verbose)]
     with ThreadPoolExecutor(max_workers=4) as pool:
         paths += list(pool.map(lambda d: build_attention(d, verbose), head_dims))
+        paths += list(pool.map(lambda d: build_shared_prefix(d, verbose), head_dims))
     return paths
 
 

@@ -1,0 +1,475 @@
+// Attention of a batch whose requests share a long prefix, over the paged cache.  Compiled once per head size:
+// -DAKV_HEAD_DIM=<multiple of 16, at most 256>.
+//
+// The first `shared` tokens of every request lie in the same pages.  A query's softmax runs over them and over its own request's
+// tokens behind them, and sums of exponentials join:  with m the larger of two maxima, l = l1 2^(m1-m) + l2 2^(m2-m), and the same for
+// the weighted sums of values.  So the prefix is walked once for the queries of ALL requests - they are the columns of one product,
+// and a key is read once for all of them instead of once per request -, a request's own keys for its own queries, both cut into
+// segments, each of which leaves (maximum, sum, weighted values); a second launch joins a row's segments.
+//
+// The columns of a kv head are its (token, query head of the group) pairs, token by token.  Both products are computed transposed:
+//     S^T[key][col] = K[key][:] . Q[col][:]       A = 32 keys x 16 dims of a key page    (keys lie [page_size, dim])
+//     O^T[dim][col] = V^T[dim][:] . P^T[:][col]   A = 32 dims x 16 keys of a value page  (values lie [dim, page_size])
+// on 32 x 32 matrix instructions.  Which of the 32 keys of a step stands in which row of A is free: with row 8a + 4h + b holding key
+// 16 (a / 2) + 8h + 4 (a % 2) + b, the scores that a lane gets are those of the keys whose values it multiplies next, in order, so
+// that nothing is exchanged between the products.  float32 goes the same way on the float32 instruction (2 dims or keys a turn).
+
+#include "common.h"
+
+#ifndef AKV_HEAD_DIM
+#error "compile with -DAKV_HEAD_DIM=<head size>"
+#endif
+
+using namespace akv;
+
+namespace {
+
+constexpr int D = AKV_HEAD_DIM;
+static_assert(D % 16 == 0 && D >= 16 && D <= 256, "head sizes are multiples of 16 up to 256");
+constexpr int KC = D / 16;             // steps of 16 dims of the score product
+constexpr int DT = (D + 31) / 32;      // tiles of 32 dims of the output (the last may be half empty)
+constexpr int kThreads = 256, kWaves = 4;
+constexpr int kRow = D + 4;            // floats a column takes in LDS: rows then lie 4 banks apart
+constexpr float kLog2e = 1.4426950408889634f;
+
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(4))) float floatx4;
+typedef __attribute__((ext_vector_type(16))) float floatx16;
+typedef __attribute__((ext_vector_type(4))) unsigned int uintx4;
+
+struct Args {
+  const void* q;              // [tokens, q_heads * D]
+  const void* k_pages;        // [pages, kv_heads, page_size, D]
+  const void* v_pages;        // [pages, kv_heads, D, page_size]
+  void* out;                  // [tokens, q_heads * D]
+  float* sums;                // [kv_heads][segments][rows][D] weighted values of a segment, below its maximum
+  float* stats;               // [kv_heads][rows][segments][2] a segment's maximum (base 2, scaled) and its sum of weights
+  const int* q_start;         // [requests + 1]
+  const int* seq_lens;        // [requests] tokens held, the new ones among them
+  const int* block_table;     // [.., table_width]
+  const int* table_rows;      // null, or [requests]: a request's row of the table
+  int table_width, requests;
+  long tokens, rows;          // rows = tokens * group: columns of a kv head
+  int q_heads, kv_heads, page_shift, shared, max_own, max_new;
+  long num_pages;
+  float scale_log2;
+  Divider group;
+  int prefix_segments, prefix_keys;    // segments of the prefix and keys of one
+  int own_segments, own_keys;          // the same of a request's own keys
+  int prefix_tiles, own_tiles;         // tiles of columns: of all rows, of the most rows a request brings
+  long prefix_blocks;
+};
+
+// Eight neighbouring elements of an operand: what a lane holds of 16 dims (or keys).
+template <typename T> struct Piece;
+template <> struct Piece<bf16_t> { uintx4 v; };
+template <> struct Piece<float> { floatx4 low, high; };
+
+template <typename T> __device__ __forceinline__ Piece<T> load_piece(const T* at);
+template <> __device__ __forceinline__ Piece<bf16_t> load_piece<bf16_t>(const bf16_t* at) { return {*reinterpret_cast<const uintx4*>(at)}; }
+template <> __device__ __forceinline__ Piece<float> load_piece<float>(const float* at) {
+  return {*reinterpret_cast<const floatx4*>(at), *reinterpret_cast<const floatx4*>(at + 4)};
+}
+__device__ __forceinline__ Piece<bf16_t> empty_piece(bf16_t) { return {uintx4{0u, 0u, 0u, 0u}}; }
+__device__ __forceinline__ Piece<float> empty_piece(float) { return {floatx4{0.f, 0.f, 0.f, 0.f}, floatx4{0.f, 0.f, 0.f, 0.f}}; }
+
+// What stays of a piece whose first `count` elements are there.
+__device__ __forceinline__ void keep_first(Piece<bf16_t>& p, int count) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (2 * i >= count) p.v[i] = 0u;
+    else if (2 * i + 1 >= count) p.v[i] &= 0xffffu;
+  }
+}
+__device__ __forceinline__ void keep_first(Piece<float>& p, int count) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (i >= count) p.low[i] = 0.f;
+    if (i + 4 >= count) p.high[i] = 0.f;
+  }
+}
+__device__ __forceinline__ bool all_finite(const Piece<bf16_t>& p) {
+  bool fine = true;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) fine = fine && (p.v[i] & 0x7f80u) != 0x7f80u && (p.v[i] & 0x7f800000u) != 0x7f800000u;
+  return fine;
+}
+__device__ __forceinline__ bool all_finite(const Piece<float>& p) {
+  bool fine = true;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) fine = fine && fabsf(p.low[i]) < INFINITY && fabsf(p.high[i]) < INFINITY;
+  return fine;
+}
+
+__device__ __forceinline__ void keep_finite(Piece<bf16_t>& p) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if ((p.v[i] & 0x7f80u) == 0x7f80u) p.v[i] &= 0xffff0000u;
+    if ((p.v[i] & 0x7f800000u) == 0x7f800000u) p.v[i] &= 0xffffu;
+  }
+}
+__device__ __forceinline__ void keep_finite(Piece<float>& p) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (!(fabsf(p.low[i]) < INFINITY)) p.low[i] = 0.f;
+    if (!(fabsf(p.high[i]) < INFINITY)) p.high[i] = 0.f;
+  }
+}
+
+__device__ __forceinline__ floatx16 multiply(const Piece<bf16_t>& a, const Piece<bf16_t>& b, floatx16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a.v), __builtin_bit_cast(bf16x8, b.v), c, 0, 0, 0);
+}
+__device__ __forceinline__ floatx16 multiply(const Piece<float>& a, const Piece<float>& b, floatx16 c) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.low[i], b.low[i], c, 0, 0, 0);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.high[i], b.high[i], c, 0, 0, 0);
+  return c;
+}
+
+// O += V^T P for 16 keys, `p` a lane's eight weights.  In bfloat16 the weights go in two parts, the rounded one and what the
+// rounding left: the sum is then as exact as the 32-bit weights, and here, where reads are what counts, costs nothing.
+__device__ __forceinline__ floatx16 weigh(const Piece<bf16_t>& v, const float* p, floatx16 c) {
+  Piece<bf16_t> high, low;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    high.v[i] = bf16_pair(p[2 * i], p[2 * i + 1]);
+    low.v[i] = bf16_pair(p[2 * i] - __uint_as_float(high.v[i] << 16), p[2 * i + 1] - __uint_as_float(high.v[i] & 0xffff0000u));
+  }
+  return multiply(v, low, multiply(v, high, c));
+}
+__device__ __forceinline__ floatx16 weigh(const Piece<float>& v, const float* p, floatx16 c) {
+  const Piece<float> w{floatx4{p[0], p[1], p[2], p[3]}, floatx4{p[4], p[5], p[6], p[7]}};
+  return multiply(v, w, c);
+}
+
+// The same value of the other half's lane joined in: lanes l and l + 32 hold the same column.
+__device__ __forceinline__ float max_over_halves(float v) {
+  const uint32_t bits = __float_as_uint(v);
+  const auto swapped = __builtin_amdgcn_permlane32_swap(bits, bits, false, false);
+  return fmaxf(__uint_as_float(swapped[0]), __uint_as_float(swapped[1]));
+}
+__device__ __forceinline__ float sum_over_halves(float v) {
+  const uint32_t bits = __float_as_uint(v);
+  const auto swapped = __builtin_amdgcn_permlane32_swap(bits, bits, false, false);
+  return __uint_as_float(swapped[0]) + __uint_as_float(swapped[1]);
+}
+
+// One tile of 32 columns over the keys first_key .. end_key - 1, by the block's four waves in turn, 32 keys a step.
+// `row0`: the tile's first row of the kv head's, `columns` how many of the 32 are there.  A column sees the keys below `visible`
+// (its lane's), `all_see` the least of them over the tile.
+template <typename T>
+__device__ __forceinline__ void walk(const Args& a, const int* table, int head, long row0, int columns, int first_key, int end_key,
+                                     int visible, int all_see, int segment, float* lds) {
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const int r = lane & 31, half = lane >> 5;
+  const int group = static_cast<int>(a.group.by), segments = a.prefix_segments + a.own_segments;
+  const int page_mask = (1 << a.page_shift) - 1;
+  Piece<T> qf[KC];
+  {
+    const long row = row0 + min(r, columns - 1);
+    const long token = group == 1 ? row : row / group;
+    const T* q = static_cast<const T*>(a.q) + (token * a.q_heads + static_cast<long>(head) * group + (row - token * group)) * D + 8 * half;
+#pragma unroll
+    for (int c = 0; c < KC; ++c) qf[c] = load_piece<T>(q + 16 * c);
+  }
+  floatx16 o[DT];
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[t][i] = 0.f;
+  float m = -INFINITY, l = 0.f;       // (m is the column's, l what this lane's keys add to its sum)
+  bool bad = false;
+  // the key of the step that this lane's row of A holds
+  const int key_at = 16 * (r >> 4) + 8 * ((r >> 2) & 1) + 4 * ((r >> 3) & 1) + (r & 3);
+  auto page_of = [&](int key) {
+    const int page = table[key >> a.page_shift];
+    const bool outside = page < 0 || page >= a.num_pages;
+    bad |= outside;
+    return static_cast<size_t>(outside ? 0 : page) * a.kv_heads + head;
+  };
+  float* mine = lds + wave * 32 * kRow;       // the wave's results, a row a column
+  bool odd = false;                           // whether values that are not finite stand there already
+  for (int base = first_key + 32 * wave; base < end_key; base += 32 * kWaves) {
+    const int key = min(base + key_at, end_key - 1);
+    const T* k = static_cast<const T*>(a.k_pages) + ((page_of(key) << a.page_shift) + (key & page_mask)) * D + 8 * half;
+    Piece<T> kf[KC];
+#pragma unroll
+    for (int c = 0; c < KC; ++c) kf[c] = load_piece<T>(k + 16 * c);
+    Piece<T> vf[2][DT];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int octet = base + 16 * c + 8 * half;
+      const int there = min(octet, (end_key - 1) & ~7);
+      const T* v = static_cast<const T*>(a.v_pages) + ((page_of(there) * D + r) << a.page_shift) + (there & page_mask);
+#pragma unroll
+      for (int t = 0; t < DT; ++t) {
+        if (D % 32 == 0 || t + 1 < DT || r < 16) vf[c][t] = load_piece<T>(v + (static_cast<size_t>(32 * t) << a.page_shift));
+        else vf[c][t] = empty_piece(T{});
+      }
+    }
+    floatx16 s;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = 0.f;
+#pragma unroll
+    for (int c = 0; c < KC; ++c) s = multiply(kf[c], qf[c], s);
+    const bool ends = base + 32 > end_key, masked = all_see < end_key && base + 32 > all_see;
+    if (ends || masked) {
+      const int limit = min(visible, end_key) - base - 8 * half;
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (16 * (i >> 3) + (i & 7) >= limit) s[i] = -INFINITY;
+    }
+    if (ends) {     // what lies behind the last key is not multiplied: it may be anything
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int t = 0; t < DT; ++t) keep_first(vf[c][t], end_key - (base + 16 * c + 8 * half));
+    }
+    float top = s[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+    const float m_new = fmaxf(m, max_over_halves(top) * a.scale_log2);
+    const float reference = m_new == -INFINITY ? 0.f : m_new;
+    if (__any(m_new > m)) {
+      const float by = __builtin_amdgcn_exp2f(m - reference);
+      l *= by;
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[t][i] *= by;
+    }
+    m = m_new;
+    float p[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.scale_log2, -reference));
+      l += p[i];
+    }
+    bool fine = true;
+    if (masked) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int t = 0; t < DT; ++t) fine = fine && all_finite(vf[c][t]);
+    }
+    if (!__all(fine)) {
+      // A key that some column does not see has a value that is not finite, and 0 times it would reach that column: such values are
+      // left out of the product and added, as they are, to the dims of the columns that see their key (any weight times them is
+      // the same), in LDS until the waves' results are joined.
+      if (!odd)
+        for (int i = lane; i < 32 * kRow; i += kWave) mine[i] = 0.f;
+      odd = true;
+      __builtin_amdgcn_wave_barrier();
+      for (int dim = half; dim < D; dim += 2) {
+        float sum = 0.f;
+        for (int j = base; j < min(base + 32, min(end_key, visible)); ++j) {
+          const float v = to_float(static_cast<const T*>(a.v_pages)[((page_of(j) * D + dim) << a.page_shift) + (j & page_mask)]);
+          if (!(fabsf(v) < INFINITY)) sum += v;
+        }
+        mine[r * kRow + dim] += sum;
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int t = 0; t < DT; ++t) keep_finite(vf[c][t]);
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int t = 0; t < DT; ++t) o[t] = weigh(vf[c][t], p + 8 * c, o[t]);
+  }
+  l = sum_over_halves(l);
+  if (__any(bad)) m = l = NAN;
+  // the four waves' results, joined through LDS
+  float* shares = lds + kWaves * 32 * kRow;     // [waves][32][2]
+  __syncthreads();
+  if (half == 0) { shares[(wave * 32 + r) * 2] = m; shares[(wave * 32 + r) * 2 + 1] = l; }
+  __syncthreads();
+  float top = -INFINITY, whole = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) top = fmaxf(top, shares[(w * 32 + r) * 2]);
+  const float reference = top == -INFINITY ? 0.f : top;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) whole += shares[(w * 32 + r) * 2 + 1] * __builtin_amdgcn_exp2f(shares[(w * 32 + r) * 2] - reference);
+  const float by = __builtin_amdgcn_exp2f(m - reference);
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int dim = 32 * t + 8 * q + 4 * half;
+      if (D % 32 == 0 || dim < D) {
+        floatx4 four = {o[t][4 * q] * by, o[t][4 * q + 1] * by, o[t][4 * q + 2] * by, o[t][4 * q + 3] * by};
+        floatx4* at = reinterpret_cast<floatx4*>(mine + r * kRow + dim);
+        if (odd) four += *at;
+        *at = four;
+      }
+    }
+  __syncthreads();
+  if (wave == 0 && half == 0 && r < columns) {
+    float* at = a.stats + ((static_cast<size_t>(head) * a.rows + row0 + r) * segments + segment) * 2;
+    at[0] = top;
+    at[1] = whole;
+  }
+  float* sums = a.sums + ((static_cast<size_t>(head) * segments + segment) * a.rows + row0) * D;
+  for (int i = threadIdx.x; i < columns * (D / 4); i += kThreads) {
+    const int column = i / (D / 4), at = i % (D / 4) * 4;
+    floatx4 sum = *reinterpret_cast<const floatx4*>(lds + column * kRow + at);
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) sum += *reinterpret_cast<const floatx4*>(lds + (w * 32 + column) * kRow + at);
+    *reinterpret_cast<floatx4*>(sums + static_cast<size_t>(column) * D + at) = sum;
+  }
+}
+
+// Blocks 0 .. prefix_blocks - 1 take (segment and head, tile) of the prefix, the others (request, head, tile, segment) of the requests'
+// own keys.
+template <typename T>
+__global__ __launch_bounds__(kThreads, (sizeof(T) == 4 || D > 128 ? 1 : 2)) void shared_prefix_kernel(Args a) {
+  extern __shared__ float lds[];
+  long block = blockIdx.x;
+  const int lane = threadIdx.x & (kWave - 1), r = lane & 31;
+  int head, segment, request = 0, columns, first, end, visible, all_see;
+  long row0;
+  if (block < a.prefix_blocks) {
+    const int tile = static_cast<int>(block % a.prefix_tiles), item = static_cast<int>(block / a.prefix_tiles);
+    head = item % a.kv_heads;
+    segment = item / a.kv_heads;
+    row0 = 32L * tile;
+    columns = static_cast<int>(min(32L, a.rows - row0));
+    first = segment * a.prefix_keys;
+    visible = all_see = end = min(a.shared, first + a.prefix_keys);
+  } else {
+    block -= a.prefix_blocks;
+    segment = static_cast<int>(block % a.own_segments);
+    block /= a.own_segments;
+    const int tile = static_cast<int>(block % a.own_tiles);
+    block /= a.own_tiles;
+    head = static_cast<int>(block % a.kv_heads);
+    request = static_cast<int>(block / a.kv_heads);
+    const int begin = a.q_start[request], count = a.q_start[request + 1] - begin, length = a.seq_lens[request], before = length - count;
+    // (what the host could not see: numbers outside its bounds are left alone here and answered with NaN by the join)
+    if (count <= 0 || count > a.max_new || begin < 0 || begin + count > a.tokens || length - a.shared > a.max_own || before < a.shared) return;
+    const int group = static_cast<int>(a.group.by);
+    columns = min(32, count * group - 32 * tile);
+    if (columns <= 0) return;
+    first = a.shared + segment * a.own_keys;
+    end = min(before + a.group.quotient(32 * tile + columns - 1) + 1, first + a.own_keys);     // (what the tile's last token sees)
+    if (first >= end) return;
+    visible = before + a.group.quotient(32 * tile + min(r, columns - 1)) + 1;
+    all_see = before + a.group.quotient(32 * tile) + 1;
+    row0 = static_cast<long>(begin) * group + 32 * tile;
+    segment += a.prefix_segments;
+  }
+  const int row = a.table_rows != nullptr ? a.table_rows[request] : request;
+  walk<T>(a, a.block_table + static_cast<size_t>(row) * a.table_width, head, row0, columns, first, end, visible, all_see, segment, lds);
+}
+
+// One block a (token, query head): the row's segments joined.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void join_kernel(Args a) {
+  constexpr int kLanes = D / 4, kParts = kThreads / kLanes;     // threads a row of values, and how many segments at a time
+  __shared__ float weights[512];
+  __shared__ floatx4 shares[kParts][kLanes];
+  const int token = blockIdx.x, q_head = blockIdx.y, tid = threadIdx.x;
+  const int group = static_cast<int>(a.group.by), head = a.group.quotient(q_head);
+  int before = 0;                                               // requests whose first row is this token's or lies before it
+  for (int i0 = 0; i0 < a.requests; i0 += kThreads)
+    before += __syncthreads_count(i0 + tid < a.requests && a.q_start[min(i0 + tid, a.requests - 1)] <= token);
+  if (before == 0 || token >= a.q_start[a.requests]) return;    // rows behind the last request's are left as they are
+  const int request = before - 1;                               // (the last of those: the ones that bring nothing come before it)
+  const int begin = a.q_start[request], count = a.q_start[request + 1] - begin, length = a.seq_lens[request];
+  const int seen = length - count + token - begin + 1;          // keys of the token
+  T* out = static_cast<T*>(a.out) + (static_cast<size_t>(token) * a.q_heads + q_head) * D;
+  if (count > a.max_new || length - a.shared > a.max_own || length - count < a.shared) {
+    if (tid < D) out[tid] = from_float<T>(NAN);
+    return;
+  }
+  const int segments = a.prefix_segments + a.own_segments;
+  const int used = a.prefix_segments + (seen - a.shared + a.own_keys - 1) / a.own_keys;
+  const size_t row = static_cast<size_t>(token) * group + (q_head - head * group);
+  const float* stats = a.stats + (static_cast<size_t>(head) * a.rows + row) * segments * 2;
+  const int lane = tid & (kWave - 1);
+  float top = -INFINITY;
+  bool nan = false;
+  for (int i = lane; i < used; i += kWave) {
+    nan |= stats[2 * i] != stats[2 * i];
+    top = fmaxf(top, stats[2 * i]);
+  }
+  top = wave_max(top);
+  const float reference = top == -INFINITY ? 0.f : top;
+  float total = 0.f;
+  for (int i = lane; i < used; i += kWave) {
+    const float by = __builtin_amdgcn_exp2f(stats[2 * i] - reference);
+    total += by * stats[2 * i + 1];
+    if (tid < kWave) weights[i] = by;
+  }
+  total = wave_sum(total);
+  if (__any(nan)) total = NAN;
+  __syncthreads();
+  const int part = tid / kLanes, at = tid % kLanes;
+  if (part < kParts) {
+    const float* sums = a.sums + (static_cast<size_t>(head) * segments * a.rows + row) * D + 4 * at;
+    floatx4 sum = {0.f, 0.f, 0.f, 0.f};
+    for (int i = part; i < used; i += kParts) sum += *reinterpret_cast<const floatx4*>(sums + static_cast<size_t>(i) * a.rows * D) * weights[i];
+    shares[part][at] = sum;
+  }
+  __syncthreads();
+  if (tid < kLanes) {
+    floatx4 sum = shares[0][tid];
+#pragma unroll
+    for (int i = 1; i < kParts; ++i) sum += shares[i][tid];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) out[4 * tid + j] = from_float<T>(sum[j] / total);
+  }
+}
+
+template <typename T> int run(const Args& a, hipStream_t stream) {
+  constexpr size_t lds = (kWaves * 32 * kRow + kWaves * 32 * 2) * sizeof(float);
+  static_assert(lds <= 160 * 1024, "LDS of a compute unit");
+  const long blocks = a.prefix_blocks + static_cast<long>(a.requests) * a.kv_heads * a.own_tiles * a.own_segments;
+  if (blocks > 0x7fffffffL || a.q_heads > 65535) return -2;
+  if (hipFuncSetAttribute(reinterpret_cast<const void*>(shared_prefix_kernel<T>), hipFuncAttributeMaxDynamicSharedMemorySize,
+                          static_cast<int>(lds)) != hipSuccess)
+    return static_cast<int>(hipGetLastError());
+  shared_prefix_kernel<T><<<static_cast<unsigned>(blocks), kThreads, lds, stream>>>(a);
+  const int status = AKV_LAUNCH_STATUS();
+  if (status != 0) return status;
+  join_kernel<T><<<dim3(static_cast<unsigned>(a.tokens), a.q_heads), kThreads, 0, stream>>>(a);
+  return AKV_LAUNCH_STATUS();
+}
+
+}  // namespace
+
+#define AKV_NAME_(dim) akv_attention_shared_prefix_d##dim
+#define AKV_NAME(dim) AKV_NAME_(dim)
+
+// `sums` and `stats` hold kv_heads * (prefix_segments + own_segments) * tokens * (q_heads / kv_heads) rows of head size and of two
+// floats; segments: prefix_segments of prefix_keys (multiples of 32) cover `shared`, own_segments of own_keys `max_own` keys of a
+// request behind it, at most 512 together.  Operands lie on 16-byte boundaries.
+extern "C" int AKV_NAME(AKV_HEAD_DIM)(const void* q, const void* k_pages, const void* v_pages, void* out, int dtype, float* sums, float* stats,
+                                      const int* q_start, const int* seq_lens, const int* block_table, const int* table_rows, int table_width,
+                                      int requests, long tokens, int q_heads, int kv_heads, int page_size, long num_pages, float scale,
+                                      int shared, int max_own, int max_new, int prefix_segments, int prefix_keys, int own_segments,
+                                      int own_keys, hipStream_t stream) {
+  if (requests <= 0 || tokens <= 0) return 0;
+  if (kv_heads <= 0 || q_heads % kv_heads != 0 || page_size < 8 || (page_size & (page_size - 1)) != 0 || shared % page_size != 0 ||
+      max_own <= 0 || max_new <= 0 || own_segments < 1 || prefix_segments + own_segments > 512 || prefix_keys % 32 != 0 || own_keys % 32 != 0 ||
+      static_cast<long>(prefix_segments) * prefix_keys < shared || static_cast<long>(own_segments) * own_keys < max_own ||
+      (static_cast<long>(shared) + max_own + page_size - 1) / page_size > table_width)
+    return -2;
+  Args a{};
+  const int group = q_heads / kv_heads;
+  a.q = q; a.k_pages = k_pages; a.v_pages = v_pages; a.out = out; a.sums = sums; a.stats = stats;
+  a.q_start = q_start; a.seq_lens = seq_lens; a.block_table = block_table; a.table_rows = table_rows;
+  a.table_width = table_width; a.requests = requests; a.tokens = tokens; a.rows = tokens * group;
+  a.q_heads = q_heads; a.kv_heads = kv_heads; a.shared = shared; a.max_own = max_own; a.max_new = max_new;
+  a.num_pages = num_pages; a.scale_log2 = scale * kLog2e; a.group = Divider::of(group);
+  while ((1 << a.page_shift) < page_size) ++a.page_shift;
+  a.prefix_segments = prefix_segments; a.prefix_keys = prefix_keys; a.own_segments = own_segments; a.own_keys = own_keys;
+  a.prefix_tiles = static_cast<int>((a.rows + 31) / 32);
+  a.own_tiles = static_cast<int>((static_cast<long>(max_new) * group + 31) / 32);
+  a.prefix_blocks = static_cast<long>(prefix_segments) * kv_heads * a.prefix_tiles;
+  if (dtype == kF32) return run<float>(a, stream);
+  if (dtype == kBF16) return run<bf16_t>(a, stream);
+  return -1;
+}

@@ -16,6 +16,7 @@ from ..csrc.build import ensure_attention, ensure_built
 from ..parts.base import KernelSet
 from . import partial_sums
 from .hip_parts import PartsKernels
+from .hip_rounds import RoundKernels
 
 _DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1}
 MAX_HEAD_DIM = 256
@@ -106,7 +107,7 @@ class StackedGate:
         self.stacked = stacked
 
 
-class HipKernels(PartsKernels, KernelSet):
+class HipKernels(PartsKernels, RoundKernels, KernelSet):
     name = "hip-gfx950"
     OWN_SKINNY_ROWS = 64            # the most rows the engine's own decode product takes
 

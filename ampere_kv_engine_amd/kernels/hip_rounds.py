@@ -1,0 +1,234 @@
+"""Wrappers over the kernels of a round of drafted tokens: attention of requests that share a prompt (`csrc/shared_prefix.hip`, a
+library per head size), the drafts' verification and the step's layout (`csrc/api_rounds.h`).  `HipKernels` inherits them.
+
+They take the requests' lengths as they lie on the device and read nothing back, so that a round can follow the one before -
+whose number of kept tokens no host has seen - or be recorded.  The host gives bounds (`max_seq_len`, `max_new_tokens`, the sizes of
+the outputs); what a kernel finds outside them it answers, as said at each call, and never follows out of its operands."""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from ..csrc.build import ensure_rounds, ensure_shared_prefix
+
+_DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1}
+
+
+def _ptr(t):
+    return ctypes.c_void_p(t.data_ptr()) if t is not None else ctypes.c_void_p(0)
+
+
+def cut_prefix(rows: int, kv_heads: int, shared: int, units: int) -> tuple[int, int]:
+    """(segments, keys of one) of a shared prompt: two blocks a unit, segments of 128 keys - a step for each wave - at least."""
+    if shared == 0:
+        return 0, 32
+    blocks = kv_heads * ((rows + 31) // 32)
+    segments = max(1, min(2 * units // blocks, (shared + 127) // 128, 128))
+    keys = ((shared + segments - 1) // segments + 127) // 128 * 128
+    return (shared + keys - 1) // keys, keys
+
+
+def cut_own(requests: int, rows: int, kv_heads: int, most: int, units: int) -> tuple[int, int]:
+    """The same of up to `most` keys that a request of up to `rows` rows a kv head holds behind the prompt."""
+    blocks = requests * kv_heads * ((rows + 31) // 32)
+    segments = max(1, min(4 * units // blocks, (most + 127) // 128, 128))
+    keys = ((most + segments - 1) // segments + 127) // 128 * 128
+    return (most + keys - 1) // keys, keys
+
+
+class RoundKernels:
+    """Mixed into `HipKernels` (which provides `_dense`, `_check`, `_pages`, `_stream`, `device`)."""
+
+    _rounds_lib = None
+
+    def _rounds(self):
+        if self._rounds_lib is None:
+            self._rounds_lib = self._load(ensure_rounds())
+            for name in ("akv_place_tokens", "akv_place_most_requests", "akv_verify_drafts"):
+                getattr(self._rounds_lib, name).restype = ctypes.c_int
+            self._rounds_lib.akv_verify_workspace.restype = ctypes.c_long
+        return self._rounds_lib
+
+    def _load(self, path: str):
+        try:
+            return ctypes.CDLL(path)
+        except OSError as error:
+            raise self._error(f"the kernel library {path} could not be loaded: {error}") from error
+
+    @staticmethod
+    def _error(message: str):
+        from .hip import KernelError
+        return KernelError(message)
+
+    def _shared_prefix_entry(self, head_dim: int):
+        entries = self.__dict__.setdefault("_shared_prefix_entries", {})
+        if head_dim not in entries:
+            entry = getattr(self._load(ensure_shared_prefix(head_dim)), f"akv_attention_shared_prefix_d{head_dim}")
+            entry.restype = ctypes.c_int
+            entries[head_dim] = entry
+        return entries[head_dim]
+
+    def _placed(self, t, name: str) -> None:
+        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.get_device() != self.device.index:
+            raise self._error(f"{name} must be a tensor on {self.device}, got {getattr(t, 'device', type(t))}")
+
+    def _apart(self, outputs: dict, inputs: dict) -> None:
+        """Refuses outputs that lie in each other or in an input (kernels of several blocks read while others write)."""
+        spans = [(name, t, t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), out)
+                 for out, named in ((True, outputs), (False, inputs)) for name, t in named.items() if t is not None and t.numel()]
+        spans.sort(key=lambda span: span[2])
+        end, of, of_out = 0, None, False
+        for name, _, low, high, out in spans:
+            if low < end and (out or of_out):
+                raise self._error(f"{name} and {of} share memory")
+            if high > end or out:
+                end, of, of_out = max(high, end), name, out
+
+    # ---- attention -----------------------------------------------------------------------------------------------------
+    def attention_shared_prefix(self, q, k_pages, v_pages, block_table, q_start, seq_lens, shared, q_heads, kv_heads, head_dim, scale, out,
+                                max_seq_len, max_new_tokens, rows=None):
+        """Attention of requests whose first `shared` tokens (a multiple of the page size; 0: none) lie in the same pages: those
+        are read once for all of them, so that many requests cost little more than one.  q, out [tokens, q_heads * head_dim]:
+        encoded queries, request by request, whose keys and values are in the pages already.  q_start [requests + 1]: a request's
+        first row; seq_lens [requests]: the tokens it holds, its new ones among them; both int32 on the device.  block_table: row r,
+        or rows[r] where `rows` is given, holds request r's pages; the first request's row is read for the prompt.  No request holds
+        more than `max_seq_len` tokens or brings more than `max_new_tokens` (0 is fine, and any number from there on; prompts of
+        thousands of tokens are `attention`'s).
+        float32 or bfloat16; head sizes as `check_attention_sizes` has them; pages of 8 tokens or more, a power of two.
+        A token gets NaN where its request's table names a page outside the pool, where its request exceeds the bounds, or where it
+        stands within the prompt.  Rows of `out` behind the last request's are left as they are."""
+        tokens, requests = q.shape[0], seq_lens.shape[0]
+        self.check_attention_sizes(q_heads, kv_heads, head_dim, 1)
+        if q.dtype not in _DTYPE_CODE:
+            raise self._error(f"kernels take float32 or bfloat16 tensors, got {q.dtype}")
+        self._dense(q, "q", None, (tokens, q_heads * head_dim))
+        self._dense(out, "out", q.dtype, (tokens, q_heads * head_dim))
+        num_pages, page_size = self._pages(k_pages, v_pages, kv_heads, head_dim, q.dtype)
+        if page_size < 8 or page_size & (page_size - 1):
+            raise self._error(f"pages of {page_size} tokens: attention over a shared prompt takes 8 or more, a power of two")
+        self._dense(q_start, "q_start", torch.int32, (requests + 1,))
+        self._dense(seq_lens, "seq_lens", torch.int32, (requests,))
+        self._dense(block_table, "block_table", torch.int32)
+        if block_table.dim() != 2 or (rows is None and block_table.shape[0] != requests):
+            raise self._error(f"block_table must be [{requests if rows is None else 'rows'}, pages], got {tuple(block_table.shape)}")
+        if rows is not None:
+            self._dense(rows, "table rows", torch.int32, (requests,))
+        shared, max_seq_len, max_new_tokens = int(shared), int(max_seq_len), int(max_new_tokens)
+        if shared < 0 or shared % page_size:
+            raise self._error(f"a shared prompt of {shared} tokens is not whole pages of {page_size}")
+        if max_new_tokens < 1 or max_seq_len <= shared:
+            raise self._error(f"a request of up to {max_seq_len} tokens, up to {max_new_tokens} of them new, has none behind a prompt of {shared}")
+        if max_seq_len > block_table.shape[1] * page_size:
+            raise self._error(f"a request of {max_seq_len} tokens does not fit a block table of {block_table.shape[1]} pages")
+        if not (scale > 0.0 and math.isfinite(scale)):
+            raise self._error(f"the scores' scale must be positive and finite, not {scale}")
+        if (q.data_ptr() | k_pages.data_ptr() | v_pages.data_ptr() | out.data_ptr()) % 16:
+            raise self._error("queries, pages and the output must lie on 16-byte boundaries")
+        self._apart({"out": out}, {"q": q, "k_pages": k_pages, "v_pages": v_pages, "block_table": block_table, "q_start": q_start,
+                                   "seq_lens": seq_lens, "table rows": rows})
+        if tokens == 0 or requests == 0:
+            return
+        if num_pages == 0:
+            raise self._error("there are no pages")
+        group = q_heads // kv_heads
+        max_new_tokens = min(max_new_tokens, tokens)
+        prefix_segments, prefix_keys = cut_prefix(tokens * group, kv_heads, shared, self.compute_units)
+        own_segments, own_keys = cut_own(requests, max_new_tokens * group, kv_heads, max_seq_len - shared, self.compute_units)
+        segments = prefix_segments + own_segments
+        # (from torch's pool: a recorded call then has room of its own, and calls on other streams do not meet in one)
+        room = torch.empty(segments * tokens * q_heads * (head_dim + 2), dtype=torch.float32, device=self.device)
+        sums, stats = room, room[segments * tokens * q_heads * head_dim:]
+        self._check(self._shared_prefix_entry(head_dim)(
+            _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(out), _DTYPE_CODE[q.dtype], _ptr(sums), _ptr(stats), _ptr(q_start), _ptr(seq_lens),
+            _ptr(block_table), _ptr(rows), block_table.shape[1], requests, ctypes.c_long(tokens), q_heads, kv_heads, page_size,
+            ctypes.c_long(num_pages), ctypes.c_float(scale), shared, max_seq_len - shared, max_new_tokens, prefix_segments, prefix_keys,
+            own_segments, own_keys, self._stream()), "attention_shared_prefix")
+
+    # ---- drafted tokens ------------------------------------------------------------------------------------------------
+    def verify_drafts(self, logits, tokens, q_start, temperature, uniforms, kept, chosen, draft_logits=None):
+        """How many of every request's drafted tokens the target keeps, and the token that follows them; the result is distributed as
+        the target's own draws.  logits [rows, vocab] float32: the target's, for the rows q_start[r] .. q_start[r + 1] - 1 (int32) of
+        request r; tokens [rows] int32: what was fed there, the request's last token and its drafts behind it.  uniforms [requests,
+        places] float32 in [0, 1), places - 1 the most drafts of a request: number i for draft i, the last for the token that follows.
+        temperature [requests] float32; 0 (or less) keeps a draft where it is the largest logit (ties: the lowest id).
+        draft_logits [requests, places - 1, vocab] float32: what the drafts were drawn from, at the same temperature - any strides, rows
+        contiguous; None: drafts that were not drawn (looked up in a text), kept with the target's probability of them.
+        kept [requests], chosen [requests, places] int32: the kept drafts, the token that follows, -1 behind it.
+        A request without rows gets 0 and -1.  A row that has no next token - a NaN, nothing above minus infinity, or (where it is
+        drawn from) plus infinity, in the target's or the draft's - ends the walk with -1 as the token.  A draft that is no id of the
+        vocabulary is not kept."""
+        if logits.dim() != 2 or uniforms.dim() != 2:
+            raise self._error("logits and uniforms must be matrices")
+        (count, vocab), (requests, places) = logits.shape, uniforms.shape
+        self._dense(logits, "logits", torch.float32)
+        self._dense(tokens, "tokens", torch.int32, (count,))
+        self._dense(q_start, "q_start", torch.int32, (requests + 1,))
+        self._dense(temperature, "temperature", torch.float32, (requests,))
+        self._dense(uniforms, "uniforms", torch.float32)
+        self._dense(kept, "kept", torch.int32, (requests,))
+        self._dense(chosen, "chosen", torch.int32, (requests, places))
+        strides = (0, 0)
+        if draft_logits is not None and places > 1:
+            self._placed(draft_logits, "draft_logits")
+            if draft_logits.dtype != torch.float32 or draft_logits.shape != (requests, places - 1, vocab):
+                raise self._error(f"draft_logits must be float32 [{requests}, {places - 1}, {vocab}], got {draft_logits.dtype} {tuple(draft_logits.shape)}")
+            if vocab > 1 and draft_logits.stride(2) != 1:
+                raise self._error("draft_logits must have contiguous rows")
+            strides = draft_logits.stride()[:2]
+        elif draft_logits is not None:
+            draft_logits = None
+        self._apart({"kept": kept, "chosen": chosen}, {"logits": logits, "tokens": tokens, "q_start": q_start, "temperature": temperature,
+                                                       "uniforms": uniforms})
+        if requests == 0:
+            return
+        lib = self._rounds()
+        room = lib.akv_verify_workspace(requests, places, vocab)
+        if room < 0:
+            raise self._error(f"verify_drafts: {requests} requests of up to {places} rows of {vocab} logits: at most 65,535, 64 and 524,288 are taken")
+        workspace = torch.empty(room, dtype=torch.uint8, device=self.device)
+        self._check(lib.akv_verify_drafts(
+            _ptr(logits), count, vocab, _ptr(tokens), _ptr(q_start), _ptr(temperature), _ptr(uniforms), requests, places, _ptr(draft_logits),
+            ctypes.c_long(strides[0]), ctypes.c_long(strides[1]), _ptr(kept), _ptr(chosen), _ptr(workspace), self._stream()), "verify_drafts")
+
+    # ---- a step's layout -----------------------------------------------------------------------------------------------
+    def place_tokens(self, lengths, counts, held, free_pages, cursor, table, page_size, q_start, seq_lens, held_after, cursor_after, positions,
+                     seq_of_token, slot_map, status, rows=None, prefix_pages=None):
+        """A step's layout from lengths on the device (all int32).  lengths, counts, held [requests]: the tokens a request holds, those it
+        brings, and its pages.  It takes the pages it lacks from free_pages[cursor ...], in the requests' order; they are entered into its
+        row of `table` (row r, or rows[r]), and held_after [requests] and cursor_after [1] say what is held and taken then.  A request
+        that holds no page starts on `prefix_pages`, if they are given: they are entered too, and `lengths` counts their tokens.
+        q_start [requests + 1], seq_lens [requests] (the tokens held after the step); positions, seq_of_token and slot_map [tokens]: of
+        every token, request by request; tokens are all that the requests bring, or more: entries behind the last are left as they are.
+        status [1]: the pages taken, or, with nothing else written, -1 too few free pages, -2 a row that the table does not have, that is too
+        narrow or that two requests name, -3 more tokens than the maps have room for, -4 a negative number, or fewer pages than a length fills."""
+        requests, tokens = lengths.shape[0], positions.shape[0]
+        lib = self._rounds()
+        named = dict(lengths=lengths, counts=counts, held=held, q_start=q_start, seq_lens=seq_lens, held_after=held_after, cursor=cursor,
+                     cursor_after=cursor_after, positions=positions, seq_of_token=seq_of_token, slot_map=slot_map, status=status)
+        sizes = dict(q_start=requests + 1, cursor=1, cursor_after=1, status=1, positions=tokens, seq_of_token=tokens, slot_map=tokens)
+        for name, t in named.items():
+            self._dense(t, name, torch.int32, (sizes.get(name, requests),))
+        self._dense(free_pages, "free_pages", torch.int32, (free_pages.shape[0],))
+        self._dense(table, "table", torch.int32)
+        if table.dim() != 2 or (rows is None and table.shape[0] < requests):
+            raise self._error(f"table must be a matrix with a row for each of {requests} requests, got {tuple(table.shape)}")
+        if rows is not None:
+            self._dense(rows, "table rows", torch.int32, (requests,))
+        if prefix_pages is not None:
+            self._dense(prefix_pages, "prefix_pages", torch.int32, (prefix_pages.shape[0],))
+        if int(page_size) < 1:
+            raise self._error(f"page_size {page_size} must be positive")
+        if requests > lib.akv_place_most_requests():
+            raise self._error(f"{requests} requests in one step; at most {lib.akv_place_most_requests()} are taken")
+        written = ("q_start", "seq_lens", "held_after", "cursor_after", "positions", "seq_of_token", "slot_map", "status")
+        self._apart({**{name: named[name] for name in written}, "table": table},
+                    {"lengths": lengths, "counts": counts, "held": held, "cursor": cursor, "free_pages": free_pages, "table rows": rows,
+                     "prefix_pages": prefix_pages})
+        self._check(lib.akv_place_tokens(
+            _ptr(lengths), _ptr(counts), _ptr(held), _ptr(free_pages), ctypes.c_long(free_pages.shape[0]), _ptr(cursor), _ptr(table), _ptr(rows),
+            table.shape[0], table.shape[1], int(page_size), _ptr(prefix_pages), prefix_pages.shape[0] if prefix_pages is not None else 0, requests,
+            tokens, _ptr(q_start), _ptr(seq_lens), _ptr(held_after), _ptr(cursor_after), _ptr(positions), _ptr(seq_of_token), _ptr(slot_map),
+            _ptr(status), self._stream()), "place_tokens")
