@@ -14,6 +14,8 @@
 // 16 (a / 2) + 8h + 4 (a % 2) + b, the scores that a lane gets are those of the keys whose values it multiplies next, in order, so
 // that nothing is exchanged between the products.  float32 goes the same way on the float32 instruction (2 dims or keys a turn).
 
+#include <type_traits>
+
 #include "common.h"
 
 #ifndef AKV_HEAD_DIM
@@ -155,10 +157,10 @@ __device__ __forceinline__ float sum_over_halves(float v) {
   return __uint_as_float(swapped[0]) + __uint_as_float(swapped[1]);
 }
 
-// One tile of 32 columns over the keys first_key .. end_key - 1, by the block's four waves in turn, 32 keys a step.
+// One tile of 32 columns over the keys first_key .. end_key - 1, by the block's waves in turn, 32 keys a step.
 // `row0`: the tile's first row of the kv head's, `columns` how many of the 32 are there.  A column sees the keys below `visible`
 // (its lane's), `all_see` the least of them over the tile.
-template <typename T>
+template <typename T, int WAVES>
 __device__ __forceinline__ void walk(const Args& a, const int* table, int head, long row0, int columns, int first_key, int end_key,
                                      int visible, int all_see, int segment, float* lds) {
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
@@ -188,31 +190,42 @@ __device__ __forceinline__ void walk(const Args& a, const int* table, int head, 
     bad |= outside;
     return static_cast<size_t>(outside ? 0 : page) * a.kv_heads + head;
   };
-  float* mine = lds + wave * 32 * kRow;       // the wave's results, a row a column
-  bool odd = false;                           // whether values that are not finite stand there already
-  for (int base = first_key + 32 * wave; base < end_key; base += 32 * kWaves) {
+  // A step's loads are asked for while the step before is worked on: its keys when those before have been multiplied, its values when
+  // those before have.
+  Piece<T> kf[KC], vf[2][DT];
+  auto fetch_keys = [&](int base) {
     const int key = min(base + key_at, end_key - 1);
     const T* k = static_cast<const T*>(a.k_pages) + ((page_of(key) << a.page_shift) + (key & page_mask)) * D + 8 * half;
-    Piece<T> kf[KC];
 #pragma unroll
     for (int c = 0; c < KC; ++c) kf[c] = load_piece<T>(k + 16 * c);
-    Piece<T> vf[2][DT];
+  };
+  auto fetch_values = [&](int base) {
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      const int octet = base + 16 * c + 8 * half;
-      const int there = min(octet, (end_key - 1) & ~7);
-      const T* v = static_cast<const T*>(a.v_pages) + ((page_of(there) * D + r) << a.page_shift) + (there & page_mask);
+      const int octet = min(base + 16 * c + 8 * half, (end_key - 1) & ~7);
+      const T* v = static_cast<const T*>(a.v_pages) + ((page_of(octet) * D + r) << a.page_shift) + (octet & page_mask);
 #pragma unroll
       for (int t = 0; t < DT; ++t) {
         if (D % 32 == 0 || t + 1 < DT || r < 16) vf[c][t] = load_piece<T>(v + (static_cast<size_t>(32 * t) << a.page_shift));
         else vf[c][t] = empty_piece(T{});
       }
     }
+  };
+  float* mine = lds + wave * 32 * kRow;       // the wave's results, a row a column
+  bool odd = false;                           // whether values that are not finite stand there already
+  const int first_base = first_key + 32 * wave;
+  if (first_base < end_key) {
+    fetch_keys(first_base);
+    fetch_values(first_base);
+  }
+  for (int base = first_base; base < end_key; base += 32 * WAVES) {
     floatx16 s;
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] = 0.f;
 #pragma unroll
     for (int c = 0; c < KC; ++c) s = multiply(kf[c], qf[c], s);
+    const bool more = base + 32 * WAVES < end_key;
+    if (more) fetch_keys(base + 32 * WAVES);
     const bool ends = base + 32 > end_key, masked = all_see < end_key && base + 32 > all_see;
     if (ends || masked) {
       const int limit = min(visible, end_key) - base - 8 * half;
@@ -278,20 +291,21 @@ __device__ __forceinline__ void walk(const Args& a, const int* table, int head, 
     for (int c = 0; c < 2; ++c)
 #pragma unroll
       for (int t = 0; t < DT; ++t) o[t] = weigh(vf[c][t], p + 8 * c, o[t]);
+    if (more) fetch_values(base + 32 * WAVES);
   }
   l = sum_over_halves(l);
   if (__any(bad)) m = l = NAN;
-  // the four waves' results, joined through LDS
-  float* shares = lds + kWaves * 32 * kRow;     // [waves][32][2]
+  // the waves' results, joined through LDS
+  float* shares = lds + WAVES * 32 * kRow;     // [waves][32][2]
   __syncthreads();
   if (half == 0) { shares[(wave * 32 + r) * 2] = m; shares[(wave * 32 + r) * 2 + 1] = l; }
   __syncthreads();
   float top = -INFINITY, whole = 0.f;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) top = fmaxf(top, shares[(w * 32 + r) * 2]);
+  for (int w = 0; w < WAVES; ++w) top = fmaxf(top, shares[(w * 32 + r) * 2]);
   const float reference = top == -INFINITY ? 0.f : top;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) whole += shares[(w * 32 + r) * 2 + 1] * __builtin_amdgcn_exp2f(shares[(w * 32 + r) * 2] - reference);
+  for (int w = 0; w < WAVES; ++w) whole += shares[(w * 32 + r) * 2 + 1] * __builtin_amdgcn_exp2f(shares[(w * 32 + r) * 2] - reference);
   const float by = __builtin_amdgcn_exp2f(m - reference);
 #pragma unroll
   for (int t = 0; t < DT; ++t)
@@ -312,28 +326,254 @@ __device__ __forceinline__ void walk(const Args& a, const int* table, int head, 
     at[1] = whole;
   }
   float* sums = a.sums + ((static_cast<size_t>(head) * segments + segment) * a.rows + row0) * D;
-  for (int i = threadIdx.x; i < columns * (D / 4); i += kThreads) {
+  for (int i = threadIdx.x; i < columns * (D / 4); i += (WAVES * kWave)) {
     const int column = i / (D / 4), at = i % (D / 4) * 4;
     floatx4 sum = *reinterpret_cast<const floatx4*>(lds + column * kRow + at);
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) sum += *reinterpret_cast<const floatx4*>(lds + (w * 32 + column) * kRow + at);
+    for (int w = 1; w < WAVES; ++w) sum += *reinterpret_cast<const floatx4*>(lds + (w * 32 + column) * kRow + at);
     *reinterpret_cast<floatx4*>(sums + static_cast<size_t>(column) * D + at) = sum;
   }
 }
 
+// ---- a prompt's keys for many columns ---------------------------------------------------------------------------------------
+// bfloat16 heads of 64 and 128 on pages of 16 tokens and more.  A block's four waves take 32 columns each and share every step of 32
+// keys through LDS, which loads write directly (16 bytes a lane in the lanes' order), in rings of four steps.  In LDS a key's row
+// stands where the matrix instruction wants it, its pieces of 16 bytes exchanged by the row's number, and values lie [16 keys][32
+// dims] an instruction's operand after the other: every read of an operand is a run of 1 KB or goes over all banks.
+// A turn multiplies the scores of step j + 1, turns those of step j into weights and adds the values of step j - 1: the three do not
+// wait for each other, so the matrix cores and the vector unit, which has as much to do, work beside each other.
+// The weights are rounded to bfloat16, once: where the products bound the time a second part would cost half as much again, and the sum
+// that they are divided by is the sum of the rounded ones, so that what is left is the error of an average over the keys.
+constexpr bool kWideFits = D == 64 || D == 128;
+constexpr int kWideWaves = 4, kWideColumns = 32 * kWideWaves;
+constexpr int kStepBytes = 32 * D * 2;              // of a step's keys, and of its values
+constexpr int kWideLoads = kStepBytes / 1024 / kWideWaves;      // instructions a wave for either
+constexpr int kWideLds = 8 * kStepBytes;
+constexpr float kSlack = 8.f;      // weights grow to 2^8 before the reference point follows a column's maximum
+
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+
+// Waits until all but the wave's last `COUNT` loads and all its reads of LDS have arrived, then for the block's other waves.
+template <int COUNT> __device__ __forceinline__ void arrived() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(COUNT) : "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// 16 bytes a lane into LDS at `to` (and on, in the lanes' order).  As text: the compiler would wait for every load before the next
+// read of LDS; the turns' counted waits order them.  No register is written.
+__device__ __forceinline__ void load_to_lds(const char* from, uint32_t offset, uint32_t to) {
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(from) : "m0", "memory");
+#pragma clang diagnostic pop
+}
+
+__device__ __forceinline__ void walk_wide(const Args& a, const int* table, int head, long row0, int first_key, int end_key, int segment,
+                                          float* lds) {
+  typedef const __attribute__((address_space(3))) char* lds_chars;
+  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int r = lane & 31, half = lane >> 5;
+  const int group = static_cast<int>(a.group.by);
+  const long my_row = row0 + 32 * wave + r;
+  const uint32_t keys_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_chars)(reinterpret_cast<char*>(lds))));
+  const uint32_t values_at = keys_at + 4 * kStepBytes;
+  // what this wave fetches of a step: rows or operands of one half of its keys, 1 KB an instruction
+  const int chunk = wave >> 1;
+  uint32_t key_from[kWideLoads], value_from[kWideLoads];
+#pragma unroll
+  for (int i = 0; i < kWideLoads; ++i) {
+    const int n = wave * kWideLoads + i;
+    constexpr int kPieces = D / 8, kRows = 64 / kPieces;         // pieces of a row, rows of an instruction
+    const int row = n * kRows + lane / kPieces, slot = lane % kPieces;
+    const int piece = slot ^ (D == 128 ? row & 15 : (row >> 1) & 7);
+    const int key = 8 * ((row >> 2) & 1) + 4 * ((row >> 3) & 1) + (row & 3);      // (within the half)
+    key_from[i] = static_cast<uint32_t>(key * D * 2 + piece * 16);
+    const int dim = n % DT * 32 + r;
+    value_from[i] = (static_cast<uint32_t>(dim) << (a.page_shift + 1)) + half * 16u;
+  }
+  const int steps = (end_key - first_key + 31) / 32;
+  const int last_page = (end_key - 1) >> a.page_shift, page_mask = (1 << a.page_shift) - 1;
+  const uint32_t page_count = static_cast<uint32_t>(min(a.num_pages, 0x7fffffffL));
+  const size_t page_bytes = static_cast<size_t>(D * 2) << a.page_shift;
+  bool bad = false;
+  // (a last half behind the prompt's end reads the prompt's last page: such scores are masked, such values left out)
+  // (the table is not written while the kernel runs: read as constant memory, by the scalar unit, or each lookup would be a wait for
+  // every load on its way)
+  typedef const __attribute__((address_space(4))) int* constant_ints;
+  const constant_ints pages = (constant_ints)reinterpret_cast<uintptr_t>(table);
+  auto lookup = [&](int step) { return pages[min((first_key + min(step, steps - 1) * 32 + 16 * chunk) >> a.page_shift, last_page)]; };
+  auto page_at = [&](int page) {
+    const bool outside = static_cast<uint32_t>(page) >= page_count;
+    bad |= outside;
+    return (static_cast<size_t>(outside ? 0 : page) * a.kv_heads + head) * page_bytes;
+  };
+  const char* k_bytes = static_cast<const char*>(a.k_pages);
+  const char* v_bytes = static_cast<const char*>(a.v_pages);
+  auto fetch_keys = [&](int step, size_t page) {
+    const int inside = (first_key + min(step, steps - 1) * 32 + 16 * chunk) & page_mask;
+    const char* from = k_bytes + page + static_cast<uint32_t>(inside) * (D * 2u);
+#pragma unroll
+    for (int i = 0; i < kWideLoads; ++i) load_to_lds(from, key_from[i], keys_at + (step & 3) * kStepBytes + (wave * kWideLoads + i) * 1024u);
+  };
+  auto fetch_values = [&](int step, size_t page) {
+    const int inside = (first_key + min(max(step, 0), steps - 1) * 32 + 16 * chunk) & page_mask;
+    const char* from = v_bytes + page + static_cast<uint32_t>(inside) * 2u;
+#pragma unroll
+    for (int i = 0; i < kWideLoads; ++i)
+      load_to_lds(from, value_from[i], values_at + (step & 3) * kStepBytes + (wave * kWideLoads + i) * 1024u);
+  };
+  Piece<bf16_t> qf[KC];
+  {
+    const long row = min(my_row, a.rows - 1), token = group == 1 ? row : row / group;
+    const bf16_t* q = static_cast<const bf16_t*>(a.q) + (token * a.q_heads + static_cast<long>(head) * group + (row - token * group)) * D + 8 * half;
+#pragma unroll
+    for (int c = 0; c < KC; ++c) qf[c] = load_piece<bf16_t>(q + 16 * c);
+  }
+  floatx16 o[DT], s, next;
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[t][i] = 0.f;
+  float reference = -INFINITY, l = 0.f;
+  Piece<bf16_t> weights[2];
+  const int swizzle = D == 128 ? r & 15 : (r >> 1) & 7;
+  const char* keys = reinterpret_cast<const char*>(lds);
+  auto scores = [&](int step) {
+    const char* row = keys + (step & 3) * kStepBytes + r * D * 2;
+    floatx16 sum;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum[i] = 0.f;
+#pragma unroll
+    for (int c = 0; c < KC; ++c) sum = multiply(Piece<bf16_t>{*reinterpret_cast<const uintx4*>(row + (((2 * c + half) ^ swizzle) << 4))}, qf[c], sum);
+    return sum;
+  };
+  auto add_values = [&](int step, int chunks) {
+    const char* from = keys + 4 * kStepBytes + (step & 3) * kStepBytes + lane * 16;
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+      if (c < chunks)
+#pragma unroll
+        for (int t = 0; t < DT; ++t) o[t] = multiply(Piece<bf16_t>{*reinterpret_cast<const uintx4*>(from + (c * DT + t) * 1024)}, weights[c], o[t]);
+  };
+  // the weights of the scores in `s`, and what the sums so far have to be multiplied by: a column's reference point follows its
+  // maximum where weights would pass 2^kSlack
+  float by = 1.f;
+  auto weigh_scores = [&](Piece<bf16_t> (&made)[2]) {
+    float top = s[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+    top = max_over_halves(top) * a.scale_log2;
+    const float moved = top > reference + kSlack ? top : reference;
+    const float below = moved == -INFINITY ? 0.f : moved;
+    by = __builtin_amdgcn_exp2f(reference - below);
+    l *= by;
+    reference = moved;
+    const bf16x2 ones = {static_cast<__bf16>(1.f), static_cast<__bf16>(1.f)};
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t pair = bf16_pair(__builtin_amdgcn_exp2f(fmaf(s[8 * c + 2 * i], a.scale_log2, -below)),
+                                        __builtin_amdgcn_exp2f(fmaf(s[8 * c + 2 * i + 1], a.scale_log2, -below)));
+        made[c].v[i] = pair;
+        l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pair), ones, l, false);
+      }
+  };
+  auto rescale = [&]() {
+    if (!__any(by != 1.f)) return;
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[t][i] *= by;
+  };
+  // Turn j asks for the keys of step j + 4 and the values of step j + 2; it needs the keys of step j + 1 and the values of step j - 1,
+  // which turn j - 3 asked for.  (Steps behind the last are asked for as the last again, into slots that nobody reads any more.)
+  constexpr int kOnTheirWay = 4 * kWideLoads;       // of the two turns before
+  size_t at0, at1, at2;                             // pages of steps j + 2, j + 3 and j + 4
+  at0 = page_at(lookup(0));
+  at1 = page_at(lookup(1));
+  at2 = page_at(lookup(2));
+  const size_t at3 = page_at(lookup(3));
+  int pending = lookup(4);
+  fetch_keys(0, at0); fetch_values(0, at0);
+  fetch_keys(1, at1); fetch_values(0, at0);         // (twice: every turn asks for as much)
+  fetch_keys(2, at2); fetch_values(0, at0);
+  arrived<kOnTheirWay>();
+  fetch_keys(3, at3); fetch_values(1, at1);
+  s = scores(0);
+  at0 = at2;
+  at1 = at3;
+  for (int j = 0; j + 1 < steps; ++j) {
+    at2 = page_at(pending);
+    pending = lookup(j + 5);
+    arrived<kOnTheirWay>();
+    fetch_keys(j + 4, at2);
+    fetch_values(j + 2, at0);
+    at0 = at1;
+    at1 = at2;
+    next = scores(j + 1);
+    Piece<bf16_t> made[2];
+    weigh_scores(made);
+    if (j > 0) add_values(j - 1, 2);
+    asm volatile("" : "+v"(made[0].v), "+v"(made[1].v), "+v"(l));     // (made here, beside the products, and not behind the branch)
+    rescale();
+    weights[0] = made[0];
+    weights[1] = made[1];
+    s = next;
+  }
+  arrived<0>();
+  if (steps > 1) add_values(steps - 2, 2);
+  const int there = end_key - first_key - (steps - 1) * 32;       // keys of the last step: 16 or 32
+  if (there < 32) {
+#pragma unroll
+    for (int i = 8; i < 16; ++i) s[i] = -INFINITY;
+  }
+  Piece<bf16_t> made[2];
+  weigh_scores(made);
+  rescale();
+  weights[0] = made[0];
+  weights[1] = made[1];
+  if (there < 32) add_values(steps - 1, 1);
+  else add_values(steps - 1, 2);
+  l = sum_over_halves(l);
+  const bool spoilt = __syncthreads_or(bad);
+  if (my_row >= a.rows) return;
+  const int segments = a.prefix_segments + a.own_segments;
+  if (half == 0) {
+    float* at = a.stats + ((static_cast<size_t>(head) * a.rows + my_row) * segments + segment) * 2;
+    at[0] = reference;
+    at[1] = spoilt ? NAN : l;
+  }
+  float* sums = a.sums + ((static_cast<size_t>(head) * segments + segment) * a.rows + my_row) * D + 4 * half;
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<floatx4*>(sums + 32 * t + 8 * i) = floatx4{o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]};
+}
+
 // Blocks 0 .. prefix_blocks - 1 take (segment and head, tile) of the prefix, the others (request, head, tile, segment) of the requests'
 // own keys.
-template <typename T>
-__global__ __launch_bounds__(kThreads, (sizeof(T) == 4 || D > 128 ? 1 : 2)) void shared_prefix_kernel(Args a) {
+template <typename T, bool WIDE>
+__global__ __launch_bounds__(WIDE ? kWideWaves * kWave : kThreads, (sizeof(T) == 4 || D > 128 ? 1 : 2)) void shared_prefix_kernel(Args a) {
   extern __shared__ float lds[];
   long block = blockIdx.x;
   const int lane = threadIdx.x & (kWave - 1), r = lane & 31;
   int head, segment, request = 0, columns, first, end, visible, all_see;
   long row0;
   if (block < a.prefix_blocks) {
-    const int tile = static_cast<int>(block % a.prefix_tiles), item = static_cast<int>(block / a.prefix_tiles);
+    // Blocks go to the XCDs in turn: the tiles of one segment and head, which read the same pages, stand eight apart, on one XCD.
+    const int items = a.prefix_segments * a.kv_heads, run = static_cast<int>(block / (kXcds * a.prefix_tiles)) * kXcds;
+    const int in_run = static_cast<int>(block - static_cast<long>(run) * a.prefix_tiles), wide = min(kXcds, items - run);
+    const int tile = in_run / wide, item = run + in_run % wide;
     head = item % a.kv_heads;
     segment = item / a.kv_heads;
+    if constexpr (WIDE) {
+      const int from = segment * a.prefix_keys;
+      const int* table = a.block_table + (a.table_rows != nullptr ? static_cast<size_t>(a.table_rows[0]) * a.table_width : 0);
+      walk_wide(a, table, head, static_cast<long>(kWideColumns) * tile, from, min(a.shared, from + a.prefix_keys), segment, lds);
+      return;
+    }
     row0 = 32L * tile;
     columns = static_cast<int>(min(32L, a.rows - row0));
     first = segment * a.prefix_keys;
@@ -361,80 +601,91 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 || D > 128 ? 1 : 2)) void
     segment += a.prefix_segments;
   }
   const int row = a.table_rows != nullptr ? a.table_rows[request] : request;
-  walk<T>(a, a.block_table + static_cast<size_t>(row) * a.table_width, head, row0, columns, first, end, visible, all_see, segment, lds);
+  walk<T, WIDE ? kWideWaves : kWaves>(a, a.block_table + static_cast<size_t>(row) * a.table_width, head, row0, columns, first, end, visible, all_see, segment, lds);
 }
 
-// One block a (token, query head): the row's segments joined.
+// A wave a (token, query head), four of a token a block: the row's segments joined.  What a row waits for is a chain of reads - whose
+// the token is, the segments' maxima and sums, their values -, so many short waves run beside each other: no wave waits for another.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void join_kernel(Args a) {
-  constexpr int kLanes = D / 4, kParts = kThreads / kLanes;     // threads a row of values, and how many segments at a time
-  __shared__ float weights[512];
-  __shared__ floatx4 shares[kParts][kLanes];
-  const int token = blockIdx.x, q_head = blockIdx.y, tid = threadIdx.x;
+  constexpr int kEach = (D + kWave - 1) / kWave;                // dims of a lane, kEach in a row (the last lanes may have none)
+  const int token = blockIdx.x, q_head = blockIdx.y * kWaves + threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
+  if (q_head >= a.q_heads) return;
   const int group = static_cast<int>(a.group.by), head = a.group.quotient(q_head);
   int before = 0;                                               // requests whose first row is this token's or lies before it
-  for (int i0 = 0; i0 < a.requests; i0 += kThreads)
-    before += __syncthreads_count(i0 + tid < a.requests && a.q_start[min(i0 + tid, a.requests - 1)] <= token);
+  for (int i0 = 0; i0 < a.requests; i0 += kWave)
+    before += __popcll(__ballot(i0 + lane < a.requests && a.q_start[min(i0 + lane, a.requests - 1)] <= token));
   if (before == 0 || token >= a.q_start[a.requests]) return;    // rows behind the last request's are left as they are
   const int request = before - 1;                               // (the last of those: the ones that bring nothing come before it)
   const int begin = a.q_start[request], count = a.q_start[request + 1] - begin, length = a.seq_lens[request];
   const int seen = length - count + token - begin + 1;          // keys of the token
-  T* out = static_cast<T*>(a.out) + (static_cast<size_t>(token) * a.q_heads + q_head) * D;
-  if (count > a.max_new || length - a.shared > a.max_own || length - count < a.shared) {
-    if (tid < D) out[tid] = from_float<T>(NAN);
-    return;
-  }
+  T* out = static_cast<T*>(a.out) + (static_cast<size_t>(token) * a.q_heads + q_head) * D + kEach * lane;
+  const bool here = kEach * lane < D;
   const int segments = a.prefix_segments + a.own_segments;
-  const int used = a.prefix_segments + (seen - a.shared + a.own_keys - 1) / a.own_keys;
-  const size_t row = static_cast<size_t>(token) * group + (q_head - head * group);
-  const float* stats = a.stats + (static_cast<size_t>(head) * a.rows + row) * segments * 2;
-  const int lane = tid & (kWave - 1);
-  float top = -INFINITY;
-  bool nan = false;
-  for (int i = lane; i < used; i += kWave) {
-    nan |= stats[2 * i] != stats[2 * i];
-    top = fmaxf(top, stats[2 * i]);
-  }
-  top = wave_max(top);
-  const float reference = top == -INFINITY ? 0.f : top;
-  float total = 0.f;
-  for (int i = lane; i < used; i += kWave) {
-    const float by = __builtin_amdgcn_exp2f(stats[2 * i] - reference);
-    total += by * stats[2 * i + 1];
-    if (tid < kWave) weights[i] = by;
-  }
-  total = wave_sum(total);
-  if (__any(nan)) total = NAN;
-  __syncthreads();
-  const int part = tid / kLanes, at = tid % kLanes;
-  if (part < kParts) {
-    const float* sums = a.sums + (static_cast<size_t>(head) * segments * a.rows + row) * D + 4 * at;
-    floatx4 sum = {0.f, 0.f, 0.f, 0.f};
-    for (int i = part; i < used; i += kParts) sum += *reinterpret_cast<const floatx4*>(sums + static_cast<size_t>(i) * a.rows * D) * weights[i];
-    shares[part][at] = sum;
-  }
-  __syncthreads();
-  if (tid < kLanes) {
-    floatx4 sum = shares[0][tid];
+  float sum[kEach], total = 0.f;
 #pragma unroll
-    for (int i = 1; i < kParts; ++i) sum += shares[i][tid];
+  for (int e = 0; e < kEach; ++e) sum[e] = 0.f;
+  if (count > a.max_new || length - a.shared > a.max_own || length - count < a.shared) {
+    total = NAN;
+  } else {
+    const int used = a.prefix_segments + (seen - a.shared + a.own_keys - 1) / a.own_keys;
+    const size_t row = static_cast<size_t>(token) * group + (q_head - head * group);
+    const float2* stats = reinterpret_cast<const float2*>(a.stats) + (static_cast<size_t>(head) * a.rows + row) * segments;
+    const float* sums = a.sums + (static_cast<size_t>(head) * segments * a.rows + row) * D + (here ? kEach * lane : 0);
+    float top = -INFINITY;
+    for (int i0 = 0; i0 < used; i0 += kWave) {
+      const float2 one = i0 + lane < used ? stats[i0 + lane] : float2{-INFINITY, 0.f};
+      const float m = fmaxf(top, wave_max(one.x)), reference = m == -INFINITY ? 0.f : m;
+      if (i0 != 0) {                                            // (more segments than lanes: what is there already goes along)
+        const float by = __builtin_amdgcn_exp2f(top - reference);
+        total *= by;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) out[4 * tid + j] = from_float<T>(sum[j] / total);
+        for (int e = 0; e < kEach; ++e) sum[e] *= by;
+      }
+      top = m;
+      const float weight = __builtin_amdgcn_exp2f(one.x - reference);
+      total += wave_sum(weight * one.y);
+      const int run = min(kWave, used - i0);
+      constexpr int kAhead = 8;                                 // segments whose values are on their way together
+      for (int i = 0; i < run; i += kAhead) {
+        float fetched[kAhead][kEach];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          const float* at = sums + static_cast<size_t>(i0 + min(i + u, run - 1)) * a.rows * D;
+#pragma unroll
+          for (int e = 0; e < kEach; ++e) fetched[u][e] = at[e];
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          const float by = __shfl(weight, min(i + u, run - 1), kWave);
+          if (i + u < run) {
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) sum[e] = fmaf(by, fetched[u][e], sum[e]);
+          }
+        }
+      }
+    }
+  }
+  if (here) {
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) out[e] = from_float<T>(sum[e] / total);
   }
 }
 
-template <typename T> int run(const Args& a, hipStream_t stream) {
-  constexpr size_t lds = (kWaves * 32 * kRow + kWaves * 32 * 2) * sizeof(float);
+template <typename T, bool WIDE> int run(const Args& a, hipStream_t stream) {
+  constexpr int waves = WIDE ? kWideWaves : kWaves;
+  constexpr size_t narrow = (waves * 32 * kRow + waves * 32 * 2) * sizeof(float);
+  constexpr size_t lds = WIDE && kWideLds > narrow ? kWideLds : narrow;
   static_assert(lds <= 160 * 1024, "LDS of a compute unit");
   const long blocks = a.prefix_blocks + static_cast<long>(a.requests) * a.kv_heads * a.own_tiles * a.own_segments;
   if (blocks > 0x7fffffffL || a.q_heads > 65535) return -2;
-  if (hipFuncSetAttribute(reinterpret_cast<const void*>(shared_prefix_kernel<T>), hipFuncAttributeMaxDynamicSharedMemorySize,
+  if (hipFuncSetAttribute(reinterpret_cast<const void*>(shared_prefix_kernel<T, WIDE>), hipFuncAttributeMaxDynamicSharedMemorySize,
                           static_cast<int>(lds)) != hipSuccess)
     return static_cast<int>(hipGetLastError());
-  shared_prefix_kernel<T><<<static_cast<unsigned>(blocks), kThreads, lds, stream>>>(a);
+  shared_prefix_kernel<T, WIDE><<<static_cast<unsigned>(blocks), waves * kWave, lds, stream>>>(a);
   const int status = AKV_LAUNCH_STATUS();
   if (status != 0) return status;
-  join_kernel<T><<<dim3(static_cast<unsigned>(a.tokens), a.q_heads), kThreads, 0, stream>>>(a);
+  join_kernel<T><<<dim3(static_cast<unsigned>(a.tokens), (a.q_heads + kWaves - 1) / kWaves), kThreads, 0, stream>>>(a);
   return AKV_LAUNCH_STATUS();
 }
 
@@ -445,12 +696,12 @@ template <typename T> int run(const Args& a, hipStream_t stream) {
 
 // `sums` and `stats` hold kv_heads * (prefix_segments + own_segments) * tokens * (q_heads / kv_heads) rows of head size and of two
 // floats; segments: prefix_segments of prefix_keys (multiples of 32) cover `shared`, own_segments of own_keys `max_own` keys of a
-// request behind it, at most 512 together.  Operands lie on 16-byte boundaries.
+// request behind it, at most 512 together.  `wide`: the prompt's columns go in tiles of 128 (`walk_wide`).  Operands lie on 16-byte boundaries.
 extern "C" int AKV_NAME(AKV_HEAD_DIM)(const void* q, const void* k_pages, const void* v_pages, void* out, int dtype, float* sums, float* stats,
                                       const int* q_start, const int* seq_lens, const int* block_table, const int* table_rows, int table_width,
                                       int requests, long tokens, int q_heads, int kv_heads, int page_size, long num_pages, float scale,
                                       int shared, int max_own, int max_new, int prefix_segments, int prefix_keys, int own_segments,
-                                      int own_keys, hipStream_t stream) {
+                                      int own_keys, int wide, hipStream_t stream) {
   if (requests <= 0 || tokens <= 0) return 0;
   if (kv_heads <= 0 || q_heads % kv_heads != 0 || page_size < 8 || (page_size & (page_size - 1)) != 0 || shared % page_size != 0 ||
       max_own <= 0 || max_new <= 0 || own_segments < 1 || prefix_segments + own_segments > 512 || prefix_keys % 32 != 0 || own_keys % 32 != 0 ||
@@ -466,10 +717,13 @@ extern "C" int AKV_NAME(AKV_HEAD_DIM)(const void* q, const void* k_pages, const 
   a.num_pages = num_pages; a.scale_log2 = scale * kLog2e; a.group = Divider::of(group);
   while ((1 << a.page_shift) < page_size) ++a.page_shift;
   a.prefix_segments = prefix_segments; a.prefix_keys = prefix_keys; a.own_segments = own_segments; a.own_keys = own_keys;
-  a.prefix_tiles = static_cast<int>((a.rows + 31) / 32);
+  if (wide != 0 && (!kWideFits || dtype != kBF16 || page_size < 16)) return -2;
+  a.prefix_tiles = static_cast<int>(wide != 0 ? (a.rows + kWideColumns - 1) / kWideColumns : (a.rows + 31) / 32);
   a.own_tiles = static_cast<int>((static_cast<long>(max_new) * group + 31) / 32);
   a.prefix_blocks = static_cast<long>(prefix_segments) * kv_heads * a.prefix_tiles;
-  if (dtype == kF32) return run<float>(a, stream);
-  if (dtype == kBF16) return run<bf16_t>(a, stream);
+  if constexpr (kWideFits)
+    if (wide != 0) return run<bf16_t, true>(a, stream);
+  if (dtype == kF32) return run<float, false>(a, stream);
+  if (dtype == kBF16) return run<bf16_t, false>(a, stream);
   return -1;
 }

@@ -23,6 +23,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kLoads = 8;                            // 16-byte pieces a thread
+constexpr int kChooseThreads = 512;
 constexpr int kPart = kThreads * kLoads * 4;         // logits a block
 constexpr int kMostPlaces = 64;                      // rows a request
 constexpr int kMostParts = 64;
@@ -31,7 +32,7 @@ constexpr int kMostParts = 64;
 struct Part {
   double sum;        // of exp((x - top) / t)
   float top;
-  int best;          // the lowest id of the largest logit (a part of minus infinities: none, INT_MAX)
+  int best;          // the lowest id of the largest logit, where nothing is drawn
   int nan;
   int pad;
 };
@@ -68,22 +69,107 @@ __device__ __forceinline__ double exp_of(double z) {
   return ldexp(v, static_cast<int>(k));
 }
 
-// a b - c d with both products rounded: 0 where they are equal, not what the rounding of one leaves of a fused product.
-__device__ __forceinline__ double difference(double a, double b, double c, double d) {
-#pragma clang fp contract(off)
-  const double ab = a * b, cd = c * d;
-  return ab - cd;
+// The same for what is done to whole rows: 2^(z / 32) of z rounded to a whole number k is one of 32 powers (`powers`: in LDS, a bank
+// pair each, so that lanes do not wait for each other), shifted; the rest, at most 1/64 of a power, a polynomial of degree 5 (off by
+// 2e-15).  Rounding is an addition of 1.5 * 2^52, whose lowest bits are k.  A logit is held above -690 t below the row's largest
+// (weights of 1e-299).
+constexpr int kPowers = 32;
+struct Scale {
+  double by, top;      // 32 log2(e) / t; the (possibly none's) logit whose weight is 1
+  float lowest;
+};
+__device__ __forceinline__ Scale scale_of(float t, float top) {
+  return Scale{kPowers * 1.4426950408889634074 / static_cast<double>(t), static_cast<double>(top), fmaxf(top - 690.f * t, -3.4e38f)};
+}
+__device__ __forceinline__ void fill_powers(double* powers) {
+  if (threadIdx.x < kPowers) powers[threadIdx.x] = exp2(threadIdx.x * (1.0 / kPowers));
+}
+// `v` times 2^(a whole power / 32) is e^((x - top) / t)
+__device__ __forceinline__ double split_exp(float x, const Scale& s, const double* powers, double& power) {
+  constexpr double kMagic = 6755399441055744.0, kStep = 0.69314718055994530942 / kPowers;
+  const double d = static_cast<double>(fmaxf(x, s.lowest)) - s.top;
+  const double rounded = fma(d, s.by, kMagic);
+  const int k = __double2loint(rounded);
+  const double f = fma(d, s.by, -(rounded - kMagic));
+  double v = kStep * kStep * kStep * kStep * kStep / 120.0;
+  v = fma(v, f, kStep * kStep * kStep * kStep / 24.0);
+  v = fma(v, f, kStep * kStep * kStep / 6.0);
+  v = fma(v, f, kStep * kStep / 2.0);
+  v = fma(v, f, kStep);
+  power = powers[k & (kPowers - 1)];
+  power = __hiloint2double(__double2hiint(power) + ((k >> 5) << 20), __double2loint(power));
+  return fma(v, f, 1.0);
+}
+__device__ __forceinline__ double add_exp(double sum, float x, const Scale& s, const double* powers) {
+  double power;
+  const double v = split_exp(x, s, powers, power);
+  return fma(v, power, sum);
+}
+__device__ __forceinline__ double just_exp(float x, const Scale& s, const double* powers) {
+  double power;
+  const double v = split_exp(x, s, powers, power);
+  return v * power;
 }
 
-__device__ __forceinline__ double wave_sum64(double v) {
-#pragma unroll
-  for (int offset = kWave / 2; offset > 0; offset >>= 1) v += __shfl_xor(v, offset, kWave);
+// a - b, not contracted with the products that they are: 0 where they are equal, not what the rounding of one leaves.
+__device__ __forceinline__ double difference(double a, double b) {
+#pragma clang fp contract(off)
+  return a - b;
+}
+
+// Sums over the lanes up to each, and over all of them, inside the vector unit: four shifts within rows of 16 lanes, two broadcasts of
+// a row's last lane to the rows behind it (an exchange through LDS takes some hundred cycles, and a sum of 64 bits twelve of them).
+template <int CTRL, int ROWS> __device__ __forceinline__ double moved(double v) {
+  const int low = __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, ROWS, 0xf, false);
+  const int high = __builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, ROWS, 0xf, false);
+  return __hiloint2double(high, low);
+}
+__device__ __forceinline__ double sums_up_to(double v) {
+  v += moved<0x111, 0xf>(v);
+  v += moved<0x112, 0xf>(v);
+  v += moved<0x114, 0xf>(v);
+  v += moved<0x118, 0xf>(v);
+  v += moved<0x142, 0xa>(v);
+  v += moved<0x143, 0xc>(v);
   return v;
 }
+__device__ __forceinline__ double of_lane(double v, int lane) {
+  return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), lane), __builtin_amdgcn_readlane(__double2loint(v), lane));
+}
+__device__ __forceinline__ double wave_sum64(double v) { return of_lane(sums_up_to(v), kWave - 1); }
 
-// Part `part` of a row in registers: piece u of a thread is x[part * kPart + u * 1024 + 4 * thread ..], ids beyond the row minus
+// The largest value of a wave, and the lowest index of those that have it.
+template <int CTRL, int ROWS> __device__ __forceinline__ float larger(float v) {
+  const int low = __float_as_int(-INFINITY);
+  return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(low, __float_as_int(v), CTRL, ROWS, 0xf, false)));
+}
+__device__ __forceinline__ float wave_top(float v) {
+  v = larger<0x111, 0xf>(v);
+  v = larger<0x112, 0xf>(v);
+  v = larger<0x114, 0xf>(v);
+  v = larger<0x118, 0xf>(v);
+  v = larger<0x142, 0xa>(v);
+  v = larger<0x143, 0xc>(v);
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), kWave - 1));
+}
+template <int CTRL, int ROWS> __device__ __forceinline__ int lower(int v) {
+  return min(v, __builtin_amdgcn_update_dpp(0x7fffffff, v, CTRL, ROWS, 0xf, false));
+}
+__device__ __forceinline__ int wave_lowest(int v) {
+  v = lower<0x111, 0xf>(v);
+  v = lower<0x112, 0xf>(v);
+  v = lower<0x114, 0xf>(v);
+  v = lower<0x118, 0xf>(v);
+  v = lower<0x142, 0xa>(v);
+  v = lower<0x143, 0xc>(v);
+  return __builtin_amdgcn_readlane(v, kWave - 1);
+}
+
+// Part `part` of a row in a block's registers: piece u of a thread is x[part * kPart + 4 (u * threads + thread) ..], ids beyond the row minus
 // infinity.  `whole`: rows of whole 16-byte pieces on 16-byte boundaries.
-__device__ __forceinline__ void fetch_part(const float* x, int vocab, int part, bool whole, float (&v)[kLoads][4]) {
+template <int THREADS>
+__device__ __forceinline__ void fetch_part(const float* x, int vocab, int part, bool whole, float (&v)[kPart / 4 / THREADS][4]) {
+  constexpr int kLoads = kPart / 4 / THREADS, kThreads = THREADS;
   const int first = part * kPart + 4 * threadIdx.x;
   if (whole) {
     float4 fetched[kLoads];
@@ -139,48 +225,64 @@ __global__ __launch_bounds__(kThreads) void parts_kernel(Verify a) {
   const float* x = target ? a.logits + static_cast<size_t>(first + place) * a.vocab
                           : a.draft + request * a.draft_request + place * a.draft_place;
   float v[kLoads][4];
-  fetch_part(x, a.vocab, part, whole_pieces(a, x), v);
+  fetch_part<kThreads>(x, a.vocab, part, whole_pieces(a, x), v);
+  __shared__ Part of_waves[kThreads / kWave];
+  __shared__ double powers[kPowers];
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  if (drawn) fill_powers(powers);
+  __syncthreads();
   float top = -INFINITY;
-  int best = 0x7fffffff;
   bool nan = false;
 #pragma unroll
   for (int u = 0; u < kLoads; ++u)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       nan |= v[u][j] != v[u][j];
-      if (v[u][j] > top) { top = v[u][j]; best = part * kPart + u * kThreads * 4 + 4 * static_cast<int>(threadIdx.x) + j; }
+      top = fmaxf(top, v[u][j]);
     }
-  __shared__ float tops[kThreads / kWave];
-  __shared__ int bests[kThreads / kWave];
-  __shared__ double sums[kThreads / kWave];
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-#pragma unroll
-  for (int offset = kWave / 2; offset > 0; offset >>= 1) {
-    const float other = __shfl_xor(top, offset, kWave);
-    const int other_best = __shfl_xor(best, offset, kWave);
-    if (other > top || (other == top && other_best < best)) { top = other; best = other_best; }
-  }
-  if (lane == 0) { tops[wave] = top; bests[wave] = best; }
-  const int any_nan = __syncthreads_or(nan);
-#pragma unroll
-  for (int w = 0; w < kThreads / kWave; ++w)
-    if (tops[w] > top || (tops[w] == top && bests[w] < best)) { top = tops[w]; best = bests[w]; }
+  top = wave_top(top);
+  nan = __any(nan);
+  int best = 0x7fffffff;
   double sum = 0.0;
-  if (drawn && top > -INFINITY && top < INFINITY && any_nan == 0) {
-    const double inverse = 1.0 / static_cast<double>(t), highest = static_cast<double>(top);
+  if (!drawn) {
 #pragma unroll
-    for (int u = 0; u < kLoads; ++u)
+    for (int u = kLoads - 1; u >= 0; --u)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sum += exp_of((static_cast<double>(v[u][j]) - highest) * inverse);
-    sum = wave_sum64(sum);
-    if (lane == 0) sums[wave] = sum;
-    __syncthreads();
-    sum = 0.0;
+      for (int j = 3; j >= 0; --j)
+        if (v[u][j] == top) best = part * kPart + u * kThreads * 4 + 4 * static_cast<int>(threadIdx.x) + j;
+    best = wave_lowest(best);
+  } else if (top > -INFINITY && top < INFINITY && !nan) {
+    const Scale scale = scale_of(t, top);
+    double other = 0.0;                // (two sums: an addition does not wait for the one before it)
 #pragma unroll
-    for (int w = 0; w < kThreads / kWave; ++w) sum += sums[w];
+    for (int u = 0; u < kLoads; ++u) {
+      sum = add_exp(sum, v[u][0], scale, powers);
+      other = add_exp(other, v[u][1], scale, powers);
+      sum = add_exp(sum, v[u][2], scale, powers);
+      other = add_exp(other, v[u][3], scale, powers);
+    }
+    sum = wave_sum64(sum + other);
   }
-  if (threadIdx.x == 0)
-    a.parts[(static_cast<size_t>(request) * (2 * a.places - 1) + blockIdx.y) * a.part_count + part] = Part{sum, top, best, any_nan, 0};
+  if (lane == 0) of_waves[wave] = Part{sum, top, best, nan ? 1 : 0, 0};
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    Part whole = of_waves[0];
+#pragma unroll
+    for (int w = 1; w < kThreads / kWave; ++w) {
+      const Part one = of_waves[w];
+      whole.nan |= one.nan;
+      if (one.top > whole.top || (one.top == whole.top && one.best < whole.best)) { whole.top = one.top; whole.best = one.best; }
+    }
+    whole.sum = 0.0;
+    if (drawn && whole.top > -INFINITY && whole.top < INFINITY) {
+      const double inverse = 1.0 / static_cast<double>(t), highest = static_cast<double>(whole.top);
+#pragma unroll
+      for (int w = 0; w < kThreads / kWave; ++w)
+        if (of_waves[w].top > -INFINITY)
+          whole.sum += of_waves[w].sum * exp_of((static_cast<double>(of_waves[w].top) - highest) * inverse);
+    }
+    a.parts[(static_cast<size_t>(request) * (2 * a.places - 1) + blockIdx.y) * a.part_count + part] = whole;
+  }
 }
 
 // What a whole row's parts say.
@@ -190,29 +292,25 @@ struct Row {
   bool fine;      // it has a next token: no NaN, something above minus infinity, nothing at plus infinity where it is drawn from
 };
 
-__device__ __forceinline__ Row gather_row(const Part* parts, int count, double inverse, bool drawn) {
-  Row row{0.0, -INFINITY, 0x7fffffff, true};
-  float top = -INFINITY;
-  for (int i = 0; i < count; ++i) {
-    const Part part = parts[i];
-    if (part.nan != 0) row.fine = false;
-    if (part.top > top) { top = part.top; row.best = part.best; }
-  }
-  row.top = top;
-  if (top == -INFINITY || (drawn && top == INFINITY)) row.fine = false;
-  if (row.fine && drawn)
-    for (int i = 0; i < count; ++i)
-      if (parts[i].top > -INFINITY) row.sum += parts[i].sum * exp_of((static_cast<double>(parts[i].top) - row.top) * inverse);
+// By one wave, a lane a part.
+__device__ __forceinline__ Row gather_row(const Part& part, double inverse, bool drawn) {
+  const float top = wave_top(part.top);
+  Row row{0.0, static_cast<double>(top), 0x7fffffff, !__any(part.nan != 0) && top > -INFINITY && !(drawn && top == INFINITY)};
+  if (!drawn) row.best = wave_lowest(part.top == top ? part.best : 0x7fffffff);
+  else if (row.fine) row.sum = wave_sum64(part.top > -INFINITY ? part.sum * exp_of((static_cast<double>(part.top) - row.top) * inverse) : 0.0);
   return row;
 }
 
-__global__ __launch_bounds__(kThreads) void choose_kernel(Verify a) {
+// grid (blocks a request, requests): a request's blocks share the parts of the row that is drawn from.
+// (512 threads: what a request waits for is one block's chain of 64-bit operations; blocks of 256 and 1,024 were slower)
+__global__ __launch_bounds__(kChooseThreads) void choose_kernel(Verify a) {
+  constexpr int kThreads = kChooseThreads, kWaves = kThreads / kWave, kLoads = kPart / 4 / kThreads;
   __shared__ Row target[kMostPlaces], draft[kMostPlaces];
   __shared__ unsigned char fine[kMostPlaces];
-  __shared__ double sums[kLoads][kThreads / kWave];
-  __shared__ double scan[kMostParts];
-  __shared__ int found, is_last, last_id;
-  const int part = blockIdx.x, request = blockIdx.y, tid = threadIdx.x;
+  __shared__ double sums[kWaves], powers[kPowers];
+  __shared__ int of_waves[kWaves];
+  __shared__ int is_last;
+  const int block = blockIdx.x, request = blockIdx.y, tid = threadIdx.x;
   const int lane = tid & (kWave - 1), wave = tid / kWave;
   int first;
   const int rows = rows_of(a, request, first);
@@ -220,12 +318,13 @@ __global__ __launch_bounds__(kThreads) void choose_kernel(Verify a) {
   const bool drawn = t > 0.f;
   const double inverse = drawn ? 1.0 / static_cast<double>(t) : 1.0;
   const Part* parts = a.parts + static_cast<size_t>(request) * (2 * a.places - 1) * a.part_count;
-  for (int i = tid; i < 2 * a.places - 1; i += kThreads) {
-    const bool of_target = i < a.places;
-    const int place = of_target ? i : i - a.places;
-    if (of_target && place < rows) target[place] = gather_row(parts + static_cast<size_t>(i) * a.part_count, a.part_count, inverse, drawn);
-    if (!of_target && place < rows - 1 && a.draft != nullptr && drawn)
-      draft[place] = gather_row(parts + static_cast<size_t>(i) * a.part_count, a.part_count, inverse, drawn);
+  const int drafts = a.draft != nullptr && drawn ? rows - 1 : 0;
+  if (drawn) fill_powers(powers);
+  for (int i = wave; i < rows + drafts; i += kWaves) {
+    Part part{0.0, -INFINITY, 0x7fffffff, 0, 0};
+    if (lane < a.part_count) part = parts[static_cast<size_t>(i < rows ? i : a.places + i - rows) * a.part_count + lane];
+    const Row row = gather_row(part, inverse, drawn);
+    if (lane == 0) (i < rows ? target[i] : draft[i - rows]) = row;
   }
   __syncthreads();
   if (tid < rows - 1) {                                   // place `tid`'s draft: kept if all before it are
@@ -253,128 +352,150 @@ __global__ __launch_bounds__(kThreads) void choose_kernel(Verify a) {
   int kept = 0;
   while (kept < rows - 1 && fine[kept] != 0) ++kept;
   int* chosen = a.chosen + static_cast<size_t>(request) * a.places;
-  if (part == 0)
+  if (block == 0)
     for (int i = tid; i < a.places; i += kThreads)
       if (rows == 0 || i != kept) chosen[i] = i < kept ? a.tokens[first + i + 1] : -1;
-  if (part == 0 && tid == 0) a.kept[request] = kept;
+  if (block == 0 && tid == 0) a.kept[request] = kept;
   if (rows == 0) return;
   const Row row = target[kept];
   const bool rejected = kept < rows - 1;
   const bool from_draft = rejected && a.draft != nullptr;
   if (!row.fine || !drawn || (from_draft && !draft[kept].fine)) {
-    if (part == 0 && tid == 0) chosen[kept] = row.fine && !drawn ? row.best : -1;
+    if (block == 0 && tid == 0) chosen[kept] = row.fine && !drawn ? row.best : -1;
     return;
   }
   const int refused = rejected && a.draft == nullptr ? a.tokens[first + kept + 1] : -1;    // (all of q lies on it)
   const float* x = a.logits + static_cast<size_t>(first + kept) * a.vocab;
   const float* y = from_draft ? a.draft + request * a.draft_request + kept * a.draft_place : nullptr;
-  // the weights of a part, of `plain` p or of what q leaves of it
-  auto weigh = [&](int of_part, bool plain, double (&w)[kLoads][4]) {
+  // (a logit of `top + t log(sum)` would have a probability of 1: probabilities come without a product)
+  Scale of_row = scale_of(t, static_cast<float>(row.top)), of_draft = of_row;
+  of_row.top += static_cast<double>(t) * log(row.sum);
+  if (from_draft) {
+    of_draft = scale_of(t, static_cast<float>(draft[kept].top));
+    of_draft.top += static_cast<double>(t) * log(draft[kept].sum);
+  }
+  // the weight of an id: p's, `plain`, or what q leaves of it (logits of minus infinity count 1e-299: no more than a rounding)
+  auto weight_of = [&](float logit, float draft_logit, int id, bool plain) {
+    const double p = just_exp(logit, of_row, powers);
+    if (from_draft && !plain) return fmax(difference(p, just_exp(draft_logit, of_draft, powers)), 0.0);
+    return !plain && id == refused ? 0.0 : p;
+  };
+  // the sum of the weights of a part, the same in every thread
+  auto sum_part = [&](int of_part, bool plain) {
     float v[kLoads][4], z[kLoads][4];
-    fetch_part(x, a.vocab, of_part, whole_pieces(a, x), v);
-    const bool less = from_draft && !plain;
-    if (less) fetch_part(y, a.vocab, of_part, whole_pieces(a, y), z);
-    const double scale = 1.0 / row.sum, draft_scale = less ? 1.0 / draft[kept].sum : 0.0, draft_top = less ? draft[kept].top : 0.0;
+    fetch_part<kThreads>(x, a.vocab, of_part, whole_pieces(a, x), v);
+    if (from_draft) fetch_part<kThreads>(y, a.vocab, of_part, whole_pieces(a, y), z);
+    double sum = 0.0;
 #pragma unroll
     for (int u = 0; u < kLoads; ++u)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        double p = exp_of((static_cast<double>(v[u][j]) - row.top) * inverse);
-        p = less ? fmax(difference(p, scale, exp_of((static_cast<double>(z[u][j]) - draft_top) * inverse), draft_scale), 0.0) : p * scale;
-        if (!plain && of_part * kPart + u * kThreads * 4 + 4 * tid + j == refused) p = 0.0;
-        w[u][j] = p;
-      }
+      for (int j = 0; j < 4; ++j) sum += weight_of(v[u][j], z[u][j], of_part * kPart + u * kThreads * 4 + 4 * tid + j, plain);
+    sum = wave_sum64(sum);
+    if (lane == 0) sums[wave] = sum;
+    __syncthreads();
+    sum = wave_sum64(lane < kWaves ? sums[lane] : 0.0);
+    __syncthreads();
+    return sum;
   };
-  double w[kLoads][4];
-  weigh(part, false, w);
-  double sum = 0.0;
-#pragma unroll
-  for (int u = 0; u < kLoads; ++u) sum += (w[u][0] + w[u][1]) + (w[u][2] + w[u][3]);
-  sum = wave_sum64(sum);
-  if (lane == 0) sums[0][wave] = sum;
-  __syncthreads();
-  if (tid == 0) {
-    sum = 0.0;
-    for (int i = 0; i < kThreads / kWave; ++i) sum += sums[0][i];
-    __hip_atomic_store(a.weights + static_cast<size_t>(request) * a.part_count + part, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    is_last = arrive(a.arrivals + request) == static_cast<unsigned>(a.part_count - 1) ? 1 : 0;
-  }
-  __syncthreads();
-  if (is_last == 0) return;
-  // the request's last block: which part the draw falls into, then which id
-  if (tid < a.part_count)
-    scan[tid] = __hip_atomic_load(a.weights + static_cast<size_t>(request) * a.part_count + tid, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  __syncthreads();
-  double total = 0.0;
-  for (int i = 0; i < a.part_count; ++i) total += scan[i];
-  const bool plain = !(total > 0.0);
-  if (plain) {                                             // q leaves nothing of p: p itself, from the parts of the first launch
-    __syncthreads();
-    if (tid < a.part_count) {
-      const Part one = parts[static_cast<size_t>(kept) * a.part_count + tid];
-      scan[tid] = one.top > -INFINITY ? one.sum * exp_of((static_cast<double>(one.top) - row.top) * inverse) / row.sum : 0.0;
+  // Of p alone the parts' weights are known from the first launch, all but the one of the refused draft; what q leaves of it has to
+  // be summed, by all of the request's blocks.
+  double weight = 0.0;                 // lane i: part i's
+  bool plain = !rejected;
+  auto weights_of_p = [&]() {
+    weight = 0.0;
+    if (lane < a.part_count) {
+      const Part one = parts[static_cast<size_t>(kept) * a.part_count + lane];
+      if (one.top > -INFINITY) weight = one.sum * exp_of((static_cast<double>(one.top) - row.top) * inverse) / row.sum;
     }
+  };
+  if (from_draft) {
+    for (int i = block; i < a.part_count; i += gridDim.x) {
+      const double sum = sum_part(i, false);
+      if (tid == 0)
+        __hip_atomic_store(a.weights + static_cast<size_t>(request) * a.part_count + i, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    if (tid == 0) is_last = arrive(a.arrivals + request) == gridDim.x - 1 ? 1 : 0;
     __syncthreads();
-    total = 0.0;
-    for (int i = 0; i < a.part_count; ++i) total += scan[i];
+    if (is_last == 0) return;
+    if (lane < a.part_count)
+      weight = __hip_atomic_load(a.weights + static_cast<size_t>(request) * a.part_count + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  } else {
+    if (block != 0) return;
+    weights_of_p();
+    if (rejected && refused >= 0 && refused < a.vocab) {
+      const double sum = sum_part(refused / kPart, false);
+      if (lane == refused / kPart) weight = sum;
+    }
+  }
+  // by the request's last (or only) block: the part that the draw falls into
+  double upto = sums_up_to(weight), total = of_lane(upto, kWave - 1);
+  if (!(total > 0.0)) {                // nothing is left of p: p itself
+    plain = true;
+    weights_of_p();
+    upto = sums_up_to(weight);
+    total = of_lane(upto, kWave - 1);
   }
   // (a number of 1 or more is the end of the line whatever the sums' last bits say)
-  const float u = a.uniforms[static_cast<size_t>(request) * a.places + a.places - 1];
-  const double goal = u < 1.f ? static_cast<double>(u) * total : INFINITY;
-  // the first part whose end lies beyond the goal, or the last one of any weight
-  int at = -1;
-  double before = 0.0, upto = 0.0;
-  for (int i = 0; i < a.part_count; ++i) {
-    if (scan[i] > 0.0) { at = i; before = upto; }
-    upto += scan[i];
-    if (at == i && upto > goal) break;
-  }
-  if (at != part) weigh(at, plain, w);
-  else if (plain) weigh(at, true, w);
-  if (tid == 0) { found = 0x7fffffff; last_id = -1; }
-  double ends[kLoads];       // of a piece's four ids over the lanes up to this one, then over everything before the piece as well
+  const float number = a.uniforms[static_cast<size_t>(request) * a.places + a.places - 1];
+  const double goal = number < 1.f ? static_cast<double>(number) * total : INFINITY;
+  // the first lane with weight whose sum lies beyond the goal, or the last lane with weight
+  auto lane_of = [&](double value, double sum) {
+    const unsigned long long some = __ballot(value > 0.0), beyond = __ballot(value > 0.0 && sum > goal);
+    return beyond != 0ull ? __builtin_ctzll(beyond) : some != 0ull ? kWave - 1 - __builtin_clzll(some) : -1;
+  };
+  const int at = max(0, lane_of(weight, upto));
+  const double before = of_lane(upto, at) - of_lane(weight, at);
+  // the part's ids, kLoads * 4 neighbours a thread: which thread, and then which of its ids
+  constexpr int kEach = kLoads * 4;
+  const int id0 = at * kPart + tid * kEach;
+  double w[kEach], own = 0.0;
+  {
+    float v[kEach], z[kEach];
+    auto fetch_run = [&](const float* from, float (&to)[kEach]) {
+      if (whole_pieces(a, from)) {
 #pragma unroll
-  for (int u = 0; u < kLoads; ++u) {
-    double s = (w[u][0] + w[u][1]) + (w[u][2] + w[u][3]);
+        for (int u = 0; u < kLoads; ++u) {
+          const float4 four = *reinterpret_cast<const float4*>(from + min(id0 + 4 * u, a.vocab - 4));
+          to[4 * u] = four.x; to[4 * u + 1] = four.y; to[4 * u + 2] = four.z; to[4 * u + 3] = four.w;
+        }
+      } else {
 #pragma unroll
-    for (int offset = 1; offset < kWave; offset <<= 1) {
-      const double other = __shfl_up(s, offset, kWave);
-      if (lane >= offset) s += other;
-    }
-    ends[u] = s;
-    if (lane == kWave - 1) sums[u][wave] = s;
-  }
-  __syncthreads();
-  int mine = 0x7fffffff, last = -1;
-  double base = before;
-  for (int u = 0; u < kLoads; ++u)
-    for (int i = 0; i < kThreads / kWave; ++i) {
-      if (i == wave) {
-#pragma unroll
-        for (int v = 0; v < kLoads; ++v)
-          if (v == u) {
-            double s = base + ends[v] - ((w[v][0] + w[v][1]) + (w[v][2] + w[v][3]));
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              s += w[v][j];
-              const int id = at * kPart + v * kThreads * 4 + 4 * tid + j;
-              if (w[v][j] > 0.0) {
-                last = id;
-                if (s > goal && id < mine) mine = id;
-              }
-            }
-          }
+        for (int e = 0; e < kEach; ++e) to[e] = from[min(id0 + e, a.vocab - 1)];
       }
-      base += sums[u][i];
-    }
+    };
+    fetch_run(x, v);
+    if (from_draft) fetch_run(y, z);
 #pragma unroll
-  for (int offset = kWave / 2; offset > 0; offset >>= 1) {
-    mine = min(mine, __shfl_xor(mine, offset, kWave));
-    last = max(last, __shfl_xor(last, offset, kWave));
+    for (int e = 0; e < kEach; ++e) {
+      w[e] = id0 + e < a.vocab && v[e] > -INFINITY ? weight_of(v[e], z[e], id0 + e, plain) : 0.0;
+      own += w[e];
+    }
   }
-  if (lane == 0) { atomicMin(&found, mine); atomicMax(&last_id, last); }
+  double end = sums_up_to(own);
+  if (lane == kWave - 1) sums[wave] = end;
   __syncthreads();
-  if (tid == 0) chosen[kept] = found != 0x7fffffff ? found : last_id;
+  end += before + wave_sum64(lane < wave ? sums[lane] : 0.0);
+  const int here = lane_of(own, end);
+  const bool beyond = here >= 0 && of_lane(end, max(here, 0)) > goal;
+  // the first wave that goes beyond the goal has it, or else the last one with any weight
+  if (lane == 0) of_waves[wave] = here < 0 ? 0 : beyond ? 2 : 1;
+  __syncthreads();
+  const int of_wave = lane < kWaves ? of_waves[lane] : 0;
+  const unsigned long long some = __ballot(of_wave == 1), over = __ballot(of_wave == 2);
+  const int chosen_wave = over != 0ull ? __builtin_ctzll(over) : some != 0ull ? kWave - 1 - __builtin_clzll(some) : -1;
+  if (wave != chosen_wave || lane != here) return;
+  double sum = end - own;
+  int last = -1;
+  bool done = false;
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    sum += w[e];
+    if (w[e] > 0.0 && !done) {
+      last = id0 + e;
+      done = sum > goal;
+    }
+  }
+  chosen[kept] = last;
 }
 
 int part_count_of(int vocab) { return (vocab + kPart - 1) / kPart; }
@@ -415,6 +536,8 @@ extern "C" int akv_verify_drafts(const float* logits, int rows, int vocab, const
   parts_kernel<<<dim3(parts, of_requests, requests), kThreads, 0, stream>>>(a);
   const int first = AKV_LAUNCH_STATUS();
   if (first != 0) return first;
-  choose_kernel<<<dim3(parts, requests), kThreads, 0, stream>>>(a);
+  // (as many blocks as the device holds at once, two a unit: every block decides for itself first, which takes it as long as two parts)
+  const int blocks = max(1, min(parts, 2 * device_facts().compute_units / requests));
+  choose_kernel<<<dim3(blocks, requests), kChooseThreads, 0, stream>>>(a);
   return AKV_LAUNCH_STATUS();
 }

@@ -21,11 +21,16 @@ def _ptr(t):
     return ctypes.c_void_p(t.data_ptr()) if t is not None else ctypes.c_void_p(0)
 
 
-def cut_prefix(rows: int, kv_heads: int, shared: int, units: int) -> tuple[int, int]:
-    """(segments, keys of one) of a shared prompt: two blocks a unit, segments of 128 keys - a step for each wave - at least."""
+def wide_tiles(rows: int, head_dim: int, page_size: int, dtype) -> bool:
+    """Whether the prompt's keys are multiplied for tiles of 128 columns that share them (`walk_wide`) rather than of 32."""
+    return dtype == torch.bfloat16 and head_dim in (64, 128) and page_size >= 16 and rows > 32
+
+
+def cut_prefix(columns: int, rows: int, kv_heads: int, shared: int, units: int) -> tuple[int, int]:
+    """(segments, keys of one) of a shared prompt: two blocks of `columns` rows a unit, segments of 128 keys at least."""
     if shared == 0:
         return 0, 32
-    blocks = kv_heads * ((rows + 31) // 32)
+    blocks = kv_heads * ((rows + columns - 1) // columns)
     segments = max(1, min(2 * units // blocks, (shared + 127) // 128, 128))
     keys = ((shared + segments - 1) // segments + 127) // 128 * 128
     return (shared + keys - 1) // keys, keys
@@ -135,7 +140,8 @@ class RoundKernels:
             raise self._error("there are no pages")
         group = q_heads // kv_heads
         max_new_tokens = min(max_new_tokens, tokens)
-        prefix_segments, prefix_keys = cut_prefix(tokens * group, kv_heads, shared, self.compute_units)
+        wide = wide_tiles(tokens * group, head_dim, page_size, q.dtype)
+        prefix_segments, prefix_keys = cut_prefix(128 if wide else 32, tokens * group, kv_heads, shared, self.compute_units)
         own_segments, own_keys = cut_own(requests, max_new_tokens * group, kv_heads, max_seq_len - shared, self.compute_units)
         segments = prefix_segments + own_segments
         # (from torch's pool: a recorded call then has room of its own, and calls on other streams do not meet in one)
@@ -145,7 +151,7 @@ class RoundKernels:
             _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(out), _DTYPE_CODE[q.dtype], _ptr(sums), _ptr(stats), _ptr(q_start), _ptr(seq_lens),
             _ptr(block_table), _ptr(rows), block_table.shape[1], requests, ctypes.c_long(tokens), q_heads, kv_heads, page_size,
             ctypes.c_long(num_pages), ctypes.c_float(scale), shared, max_seq_len - shared, max_new_tokens, prefix_segments, prefix_keys,
-            own_segments, own_keys, self._stream()), "attention_shared_prefix")
+            own_segments, own_keys, int(wide), self._stream()), "attention_shared_prefix")
 
     # ---- drafted tokens ------------------------------------------------------------------------------------------------
     def verify_drafts(self, logits, tokens, q_start, temperature, uniforms, kept, chosen, draft_logits=None):
