@@ -5,8 +5,8 @@
 //   has_r   = max(had_r, ceil(after_r / page))      its new pages: free[cursor + (new pages of requests before r) + 0, 1, ...]
 //   token j of request r: position length_r + j, slot = page of that position * page size + position within the page
 //
-// One launch.  Every block runs the prefix sums over the requests for itself, in LDS (a few hundred requests: cheaper than a
-// launch of its own or a wait between blocks), and then takes its share of the tokens and of the table's entries.  A token's page
+// One launch.  Every block runs the prefix sums over the requests for itself (a few hundred requests: cheaper than a launch of its
+// own or a wait between blocks), keeps what it has read of them in LDS, and then takes its share of the tokens and of the table's entries.  A token's page
 // is computed, not read back from the table entries that another block may be writing: an entry below `had` was there
 // before the call (or is the prompt's), one from `had` on follows from the free list.  So no block reads what another writes.
 // Nothing but `status` is written where the step cannot be laid out: every block finds that out before it writes.
@@ -19,98 +19,106 @@ using namespace akv;
 
 namespace {
 
-constexpr int kMost = 4096;       // requests: three ints each in LDS
-constexpr int kThreads = 256;
+constexpr int kMost = 4096;       // requests: five ints each in LDS, and two of the hash
+constexpr int kThreads = 1024;
 
 struct Place {
   const int *lengths, *counts, *held, *free_pages, *cursor, *rows, *prefix_pages;
   int *table, *q_start, *seq_lens, *held_after, *cursor_after, *positions, *seq_of_token, *slot_map, *status;
   long free_count;
   int table_rows, table_width, page_size, prefix_count, requests, tokens;
+  int hash_places;                // a power of two, at least twice the requests
   Divider page;
 };
 
-// Inclusive sums over the block's threads of two counts at once (64 bits hold any sum of a request's 31-bit counts).
-__device__ __forceinline__ void scan_pair(long& a, long& b, long (*scratch)[2]) {
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-#pragma unroll
-  for (int offset = 1; offset < kWave; offset <<= 1) {
-    const long x = __shfl_up(a, offset, kWave), y = __shfl_up(b, offset, kWave);
-    if (lane >= offset) { a += x; b += y; }
-  }
-  __syncthreads();
-  if (lane == kWave - 1) { scratch[wave][0] = a; scratch[wave][1] = b; }
-  __syncthreads();
-  for (int w = 0; w < wave; ++w) { a += scratch[w][0]; b += scratch[w][1]; }
+// Sums over the lanes up to each, inside the vector unit: four shifts within rows of 16 lanes, two broadcasts of a row's last lane.
+template <int CTRL, int ROWS> __device__ __forceinline__ long moved(long v) {
+  const int low = __builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xf, false);
+  const int high = __builtin_amdgcn_update_dpp(0, static_cast<int>(v >> 32), CTRL, ROWS, 0xf, false);
+  return (static_cast<long>(high) << 32) | static_cast<uint32_t>(low);
+}
+__device__ __forceinline__ long sums_up_to(long v) {
+  v += moved<0x111, 0xf>(v);
+  v += moved<0x112, 0xf>(v);
+  v += moved<0x114, 0xf>(v);
+  v += moved<0x118, 0xf>(v);
+  v += moved<0x142, 0xa>(v);
+  v += moved<0x143, 0xc>(v);
+  return v;
 }
 
 __global__ __launch_bounds__(kThreads) void place_kernel(Place p) {
-  __shared__ int first_token[kMost + 1];     // tokens before a request's
-  __shared__ int first_page[kMost + 1];      // pages taken before a request's
-  __shared__ int had_of[kMost];
-  __shared__ long scratch[kThreads / kWave][2];
-  __shared__ int rows_seen[2 * kMost];       // a hash of the table's rows that requests name, by open addressing
-  const int tid = threadIdx.x;
+  constexpr int kWaves = kThreads / kWave;
+  extern __shared__ int lds[];
+  __shared__ long of_waves[2][kWaves];
+  __shared__ int wrong;
+  const int n = p.requests;
+  int* first_token = lds;               // [n + 1] tokens before a request's
+  int* first_page = first_token + n + 1;    // [n + 1] pages taken before a request's
+  int* had_of = first_page + n + 1;     // [n] pages before the call; of a request that starts on the prompt's, -1 - their number
+  int* length_of = had_of + n;          // [n]
+  int* row_of = length_of + n;          // [n]
+  int* rows_seen = row_of + n;          // a hash of the table's rows that requests name, by open addressing
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+  const int cursor = p.cursor[0];
+  if (tid == 0) wrong = 0;
+  if (p.rows != nullptr)
+    for (int i = tid; i < p.hash_places; i += kThreads) rows_seen[i] = -1;
+  __syncthreads();
   long tokens_before = 0, pages_before = 0;
-  int wrong = 0;           // 1 a length or count that cannot be, 2 a table row that is too narrow, not there or named twice
-  int places = kThreads;   // of the hash: a power of two, at least twice the requests
-  while (places < 2 * p.requests) places *= 2;
-  if (p.rows != nullptr) {
-    for (int i = tid; i < places; i += kThreads) rows_seen[i] = -1;
-    __syncthreads();
-  }
-  for (int r0 = 0; r0 < p.requests; r0 += kThreads) {
+  for (int r0 = 0; r0 < n; r0 += kThreads) {
     const int r = r0 + tid;
     long count = 0, taken = 0;
-    if (r < p.requests) {
+    int fault = 0;           // 1 a length or count that cannot be, 2 a table row that is too narrow, not there or named twice
+    if (r < n) {
       const int length = p.lengths[r], held = p.held[r], brings = p.counts[r];
       const int row = p.rows != nullptr ? p.rows[r] : r;
       const long after = static_cast<long>(length) + brings;
-      int had = held;
+      const int had = held == 0 ? p.prefix_count : held;
       if (length < 0 || brings < 0 || held < 0 || after > 0x7fffffffL) {
-        wrong |= 1;
+        fault = 1;
       } else {
-        if (held == 0) had = p.prefix_count;
-        const int quotient = p.page.quotient(static_cast<int>(after));
-        const int need = quotient + (p.page.rest(static_cast<int>(after), quotient) != 0 ? 1 : 0);
+        const int whole = p.page.quotient(static_cast<int>(after)), old = p.page.quotient(length);
+        const int need = whole + (p.page.rest(static_cast<int>(after), whole) != 0 ? 1 : 0);
         // (what a request held before has to lie on pages that it has: the entries of those are read)
-        const int old = p.page.quotient(length) + (p.page.rest(length, p.page.quotient(length)) != 0 ? 1 : 0);
-        if (had < old) wrong |= 1;
+        if (had < old + (p.page.rest(length, old) != 0 ? 1 : 0)) fault = 1;
         count = brings;
         taken = max(0, need - had);
         if (row < 0 || row >= p.table_rows || had + taken > p.table_width) {
-          wrong |= 2;
+          fault |= 2;
         } else if (p.rows != nullptr) {
           // (as many rows as requests at most in twice as many places: the walk ends at a free place or at the row's own)
-          for (int at = (row * 0x9E3779B1u >> 8) & (places - 1);; at = (at + 1) & (places - 1)) {
+          for (int at = (row * 0x9E3779B1u >> 8) & (p.hash_places - 1);; at = (at + 1) & (p.hash_places - 1)) {
             const int there = atomicCAS(&rows_seen[at], -1, row);
-            if (there == row) wrong |= 2;
+            if (there == row) fault |= 2;
             if (there == row || there == -1) break;
           }
         }
       }
-      had_of[r] = had;
+      had_of[r] = held == 0 && p.prefix_count > 0 ? -1 - had : had;
+      length_of[r] = length;
+      row_of[r] = row;
     }
-    long token_end = count, page_end = taken;
-    scan_pair(token_end, page_end, scratch);
-    if (r < p.requests) {
-      // (sums beyond 31 bits are refused below, by their totals)
-      first_token[r] = static_cast<int>(tokens_before + token_end - count);
-      first_page[r] = static_cast<int>(pages_before + page_end - taken);
+    if (fault != 0) atomicOr(&wrong, fault);
+    const long token_end = sums_up_to(count), page_end = sums_up_to(taken);      // (64 bits hold any sum of 4,096 requests')
+    if (lane == kWave - 1) { of_waves[0][wave] = token_end; of_waves[1][wave] = page_end; }
+    __syncthreads();
+    long tokens_here = tokens_before + token_end - count, pages_here = pages_before + page_end - taken;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const long a = of_waves[0][w], b = of_waves[1][w];
+      if (w < wave) { tokens_here += a; pages_here += b; }
+      tokens_before += a;
+      pages_before += b;
     }
-    __syncthreads();
-    if (tid == kThreads - 1) { scratch[0][0] = token_end; scratch[0][1] = page_end; }    // the last thread's sums are the totals
-    __syncthreads();
-    tokens_before += scratch[0][0];
-    pages_before += scratch[0][1];
+    // (sums beyond 31 bits are refused below, by their totals)
+    if (r < n) { first_token[r] = static_cast<int>(tokens_here); first_page[r] = static_cast<int>(pages_here); }
     __syncthreads();
   }
-  const bool bad_numbers = __syncthreads_or(wrong & 1), bad_rows = __syncthreads_or(wrong & 2);
-  const int cursor = p.cursor[0];
   int verdict = pages_before > 0x7fffffffL ? -1 : static_cast<int>(pages_before);
-  if (bad_numbers) verdict = -4;
+  if ((wrong & 1) != 0) verdict = -4;
   else if (tokens_before > p.tokens) verdict = -3;
-  else if (bad_rows) verdict = -2;
+  else if ((wrong & 2) != 0) verdict = -2;
   else if (cursor < 0 || cursor + pages_before > p.free_count) verdict = -1;
   if (blockIdx.x == 0 && tid == 0) {
     p.status[0] = verdict;
@@ -118,54 +126,43 @@ __global__ __launch_bounds__(kThreads) void place_kernel(Place p) {
   }
   if (verdict < 0) return;
   const int tokens = static_cast<int>(tokens_before), pages = static_cast<int>(pages_before);
-  if (tid == 0) { first_token[p.requests] = tokens; first_page[p.requests] = pages; }
+  if (tid == 0) { first_token[n] = tokens; first_page[n] = pages; }
   __syncthreads();
   const int begin = blockIdx.x * kThreads + tid, stride = gridDim.x * kThreads;
-  for (int r = begin; r < p.requests; r += stride) {
-    p.q_start[r] = first_token[r];
-    p.seq_lens[r] = p.lengths[r] + first_token[r + 1] - first_token[r];
-    p.held_after[r] = had_of[r] + first_page[r + 1] - first_page[r];
-  }
-  if (begin == 0) p.q_start[p.requests] = tokens;
-  // the last request whose first number is <= n (requests that bring nothing are stepped over)
-  auto owner = [&](const int* first, int n) {
-    int low = 0, high = p.requests;       // first[low] <= n < first[high]
+  auto pages_had = [&](int r) { return had_of[r] < 0 ? -1 - had_of[r] : had_of[r]; };
+  // the last request whose first number is <= i (requests that bring nothing are stepped over)
+  auto owner = [&](const int* first, int i) {
+    int low = 0, high = n;       // first[low] <= i < first[high]
     while (high - low > 1) {
       const int middle = (low + high) >> 1;
-      if (first[middle] <= n) low = middle; else high = middle;
+      if (first[middle] <= i) low = middle; else high = middle;
     }
     return low;
   };
-  for (int n = begin; n < pages; n += stride) {
-    const int r = owner(first_page, n);
-    const int row = p.rows != nullptr ? p.rows[r] : r;
-    p.table[static_cast<size_t>(row) * p.table_width + had_of[r] + n - first_page[r]] = p.free_pages[cursor + n];
-  }
-  if (p.prefix_count > 0) {               // requests that hold nothing yet start on the prompt's pages: a wave each
-    const int lane = tid & (kWave - 1), wave = begin / kWave, waves = stride / kWave;
-    for (int r = wave; r < p.requests; r += waves) {
-      if (p.held[r] != 0) continue;
-      const int row = p.rows != nullptr ? p.rows[r] : r;
-      for (int i = lane; i < p.prefix_count; i += kWave) p.table[static_cast<size_t>(row) * p.table_width + i] = p.prefix_pages[i];
-    }
-  }
-  for (int n = begin; n < tokens; n += stride) {
-    const int r = owner(first_token, n);
-    const int position = p.lengths[r] + n - first_token[r];
+  for (int i = begin; i < tokens; i += stride) {
+    const int r = owner(first_token, i);
+    const int position = length_of[r] + i - first_token[r], had = pages_had(r);
     const int at = p.page.quotient(position), inside = p.page.rest(position, at);
-    int id;
-    if (at >= had_of[r]) {
-      id = p.free_pages[cursor + first_page[r] + at - had_of[r]];
-    } else if (p.held[r] == 0) {
-      id = p.prefix_pages[at];
-    } else {
-      const int row = p.rows != nullptr ? p.rows[r] : r;
-      id = p.table[static_cast<size_t>(row) * p.table_width + at];
-    }
-    p.positions[n] = position;
-    p.seq_of_token[n] = r;
-    p.slot_map[n] = id < 0 ? -1 : id * p.page_size + inside;
+    const int id = at >= had ? p.free_pages[cursor + first_page[r] + at - had]
+                   : had_of[r] < 0 ? p.prefix_pages[at] : p.table[static_cast<size_t>(row_of[r]) * p.table_width + at];
+    p.positions[i] = position;
+    p.seq_of_token[i] = r;
+    p.slot_map[i] = id < 0 ? -1 : id * p.page_size + inside;
   }
+  for (int i = begin; i < pages; i += stride) {
+    const int r = owner(first_page, i);
+    p.table[static_cast<size_t>(row_of[r]) * p.table_width + pages_had(r) + i - first_page[r]] = p.free_pages[cursor + i];
+  }
+  for (int r = begin; r < n; r += stride) {
+    p.q_start[r] = first_token[r];
+    p.seq_lens[r] = length_of[r] + first_token[r + 1] - first_token[r];
+    p.held_after[r] = pages_had(r) + first_page[r + 1] - first_page[r];
+  }
+  if (begin == 0) p.q_start[n] = tokens;
+  if (p.prefix_count > 0)                 // requests that hold nothing yet start on the prompt's pages: a wave each
+    for (int r = begin / kWave; r < n; r += stride / kWave)
+      if (had_of[r] < 0)
+        for (int i = lane; i < p.prefix_count; i += kWave) p.table[static_cast<size_t>(row_of[r]) * p.table_width + i] = p.prefix_pages[i];
 }
 
 }  // namespace
@@ -182,10 +179,20 @@ extern "C" int akv_place_tokens(const int* lengths, const int* counts, const int
                                 int* held_after, int* cursor_after, int* positions, int* seq_of_token, int* slot_map, int* status,
                                 hipStream_t stream) {
   if (requests < 0 || requests > kMost || tokens < 0 || page_size <= 0 || table_width < 0 || table_rows < 0 || prefix_count < 0) return -2;
+  int places = kWave;
+  while (places < 2 * requests) places *= 2;
   const Place p{lengths, counts, held, free_pages, cursor, rows, prefix_pages, table, q_start, seq_lens, held_after, cursor_after,
                 positions, seq_of_token, slot_map, status, free_count, table_rows, table_width, page_size, prefix_count, requests,
-                tokens, Divider::of(page_size)};
-  const int blocks = max(1, min(256, (max(tokens, requests) + kThreads - 1) / kThreads));
-  place_kernel<<<blocks, kThreads, 0, stream>>>(p);
+                tokens, places, Divider::of(page_size)};
+  // (a wave takes a forked request's entries, some hundred reads and writes of the prompt's pages: with blocks enough for all of them)
+  const long entries = max(static_cast<long>(max(tokens, requests)), static_cast<long>(requests) * min(prefix_count, kWave));
+  const int blocks = static_cast<int>(max(1L, min(256L, (entries + kThreads - 1) / kThreads)));
+  const size_t lds = (5 * static_cast<size_t>(requests) + 2 + (rows != nullptr ? places : 0)) * sizeof(int);
+  if (lds > 60 * 1024) {
+    const hipError_t status = hipFuncSetAttribute(reinterpret_cast<const void*>(place_kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                                  static_cast<int>(lds));
+    if (status != hipSuccess) return static_cast<int>(status);
+  }
+  place_kernel<<<blocks, kThreads, lds, stream>>>(p);
   return AKV_LAUNCH_STATUS();
 }

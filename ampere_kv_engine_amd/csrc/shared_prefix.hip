@@ -32,6 +32,7 @@ constexpr int KC = D / 16;             // steps of 16 dims of the score product
 constexpr int DT = (D + 31) / 32;      // tiles of 32 dims of the output (the last may be half empty)
 constexpr int kThreads = 256, kWaves = 4;
 constexpr int kRow = D + 4;            // floats a column takes in LDS: rows then lie 4 banks apart
+constexpr size_t narrow_lds(int waves) { return (waves * 32 * kRow + waves * 32 * 2) * sizeof(float); }     // of `walk`
 constexpr float kLog2e = 1.4426950408889634f;
 
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
@@ -159,10 +160,10 @@ __device__ __forceinline__ float sum_over_halves(float v) {
 
 // One tile of 32 columns over the keys first_key .. end_key - 1, by the block's waves in turn, 32 keys a step.
 // `row0`: the tile's first row of the kv head's, `columns` how many of the 32 are there.  A column sees the keys below `visible`
-// (its lane's), `all_see` the least of them over the tile.
+// (its lane's), `all_see` the least of them over the tile.  `wanted`: a bit for each column whose results are written.
 template <typename T, int WAVES>
 __device__ __forceinline__ void walk(const Args& a, const int* table, int head, long row0, int columns, int first_key, int end_key,
-                                     int visible, int all_see, int segment, float* lds) {
+                                     int visible, int all_see, int segment, float* lds, uint32_t wanted = 0xffffffffu) {
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   const int r = lane & 31, half = lane >> 5;
   const int group = static_cast<int>(a.group.by), segments = a.prefix_segments + a.own_segments;
@@ -320,7 +321,7 @@ __device__ __forceinline__ void walk(const Args& a, const int* table, int head, 
       }
     }
   __syncthreads();
-  if (wave == 0 && half == 0 && r < columns) {
+  if (wave == 0 && half == 0 && r < columns && ((wanted >> r) & 1u) != 0u) {
     float* at = a.stats + ((static_cast<size_t>(head) * a.rows + row0 + r) * segments + segment) * 2;
     at[0] = top;
     at[1] = whole;
@@ -328,6 +329,7 @@ __device__ __forceinline__ void walk(const Args& a, const int* table, int head, 
   float* sums = a.sums + ((static_cast<size_t>(head) * segments + segment) * a.rows + row0) * D;
   for (int i = threadIdx.x; i < columns * (D / 4); i += (WAVES * kWave)) {
     const int column = i / (D / 4), at = i % (D / 4) * 4;
+    if (((wanted >> column) & 1u) == 0u) continue;
     floatx4 sum = *reinterpret_cast<const floatx4*>(lds + column * kRow + at);
 #pragma unroll
     for (int w = 1; w < WAVES; ++w) sum += *reinterpret_cast<const floatx4*>(lds + (w * 32 + column) * kRow + at);
@@ -336,20 +338,24 @@ __device__ __forceinline__ void walk(const Args& a, const int* table, int head, 
 }
 
 // ---- a prompt's keys for many columns ---------------------------------------------------------------------------------------
-// bfloat16 heads of 64 and 128 on pages of 16 tokens and more.  A block's four waves take 32 columns each and share every step of 32
-// keys through LDS, which loads write directly (16 bytes a lane in the lanes' order), in rings of four steps.  In LDS a key's row
-// stands where the matrix instruction wants it, its pieces of 16 bytes exchanged by the row's number, and values lie [16 keys][32
-// dims] an instruction's operand after the other: every read of an operand is a run of 1 KB or goes over all banks.
-// A turn multiplies the scores of step j + 1, turns those of step j into weights and adds the values of step j - 1: the three do not
-// wait for each other, so the matrix cores and the vector unit, which has as much to do, work beside each other.
-// The weights are rounded to bfloat16, once: where the products bound the time a second part would cost half as much again, and the sum
-// that they are divided by is the sum of the rounded ones, so that what is left is the error of an average over the keys.
+// bfloat16 heads of 64 and 128 on pages of 16 tokens and more.  A block's eight waves take 32 columns each and share the keys and values
+// of 64 tokens, a stage, through LDS, which loads write directly (16 bytes a lane in the lanes' order), in rings of four stages.  In
+// LDS a key's row stands where the matrix instruction wants it, its pieces of 16 bytes exchanged by the row's number, and values lie
+// [16 keys][32 dims] one operand after the other: every read of an operand is a run of 1 KB or goes over all banks.
+// A turn multiplies the scores of step u + 1 (32 keys), turns those of step u into weights and adds the values of step u - 1: the three
+// do not wait for each other, and nothing in it depends on what the scores are.  A column's weights are taken below a fixed point,
+// the maximum of the segment's first step, and may grow: bfloat16 and float32 reach to 2^127, and a sum that is divided by another of the
+// same scale loses nothing.  Where a column's weights pass 2^40, or there is no such point (nothing but minus infinity, a NaN), the column
+// is done again by `walk`, which keeps a running maximum: what a column gets hangs on nothing beside it.  (A branch that moves the point in the loop costs it half as much again: the
+// compiler then keeps the sums in two sets of registers.)
+// The weights are rounded to bfloat16, once: a second part would cost half the matrix instructions again, and the sum that they are
+// divided by is the sum of the rounded ones, so that what is left is the error of an average over the keys.
 constexpr bool kWideFits = D == 64 || D == 128;
-constexpr int kWideWaves = 4, kWideColumns = 32 * kWideWaves;
-constexpr int kStepBytes = 32 * D * 2;              // of a step's keys, and of its values
-constexpr int kWideLoads = kStepBytes / 1024 / kWideWaves;      // instructions a wave for either
-constexpr int kWideLds = 8 * kStepBytes;
-constexpr float kSlack = 8.f;      // weights grow to 2^8 before the reference point follows a column's maximum
+constexpr int kWideWaves = 8, kWideColumns = 32 * kWideWaves;
+constexpr int kStepBytes = (kWideFits ? 32 * D : 32 * 64) * 2, kStageBytes = 2 * kStepBytes;      // of a step's or a stage's keys, and of its values
+constexpr int kWideLoads = kStageBytes / 1024 / kWideWaves;               // instructions a wave for a stage's keys, and for its values
+constexpr size_t kWideLds = 8 * kStageBytes, kWideNarrowLds = kWideFits ? narrow_lds(kWideWaves) : 0;
+constexpr float kLimit = 0x1p40f;  // what a lane's sixteen weights of a step may sum up to
 
 typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
 
@@ -369,16 +375,19 @@ __device__ __forceinline__ void load_to_lds(const char* from, uint32_t offset, u
 #pragma clang diagnostic pop
 }
 
-__device__ __forceinline__ void walk_wide(const Args& a, const int* table, int head, long row0, int first_key, int end_key, int segment,
-                                          float* lds) {
+// Leaves in over[wave] a bit for each of a wave's columns whose weights passed their bounds, and writes the others.
+__device__ __forceinline__ void walk_wide(const Args& a, const int* table, int head, long row0, long rows, int first_key, int end_key,
+                                          int segment, float* lds, uint32_t* over_of) {
   typedef const __attribute__((address_space(3))) char* lds_chars;
+  // (the table is not written while the kernel runs: read as constant memory, by the scalar unit, or each lookup would be a wait for
+  // every load on its way)
+  typedef const __attribute__((address_space(4))) int* constant_ints;
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int r = lane & 31, half = lane >> 5;
   const int group = static_cast<int>(a.group.by);
   const long my_row = row0 + 32 * wave + r;
-  const uint32_t keys_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_chars)(reinterpret_cast<char*>(lds))));
-  const uint32_t values_at = keys_at + 4 * kStepBytes;
-  // what this wave fetches of a step: rows or operands of one half of its keys, 1 KB an instruction
+  const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_chars)(reinterpret_cast<char*>(lds))));
+  // what this wave fetches of a stage: half of the rows or operands of one of its four pieces of 16 keys, 1 KB an instruction
   const int chunk = wave >> 1;
   uint32_t key_from[kWideLoads], value_from[kWideLoads];
 #pragma unroll
@@ -387,162 +396,206 @@ __device__ __forceinline__ void walk_wide(const Args& a, const int* table, int h
     constexpr int kPieces = D / 8, kRows = 64 / kPieces;         // pieces of a row, rows of an instruction
     const int row = n * kRows + lane / kPieces, slot = lane % kPieces;
     const int piece = slot ^ (D == 128 ? row & 15 : (row >> 1) & 7);
-    const int key = 8 * ((row >> 2) & 1) + 4 * ((row >> 3) & 1) + (row & 3);      // (within the half)
+    const int key = 8 * ((row >> 2) & 1) + 4 * ((row >> 3) & 1) + (row & 3);      // (within the 16)
     key_from[i] = static_cast<uint32_t>(key * D * 2 + piece * 16);
     const int dim = n % DT * 32 + r;
     value_from[i] = (static_cast<uint32_t>(dim) << (a.page_shift + 1)) + half * 16u;
   }
-  const int steps = (end_key - first_key + 31) / 32;
-  const int last_page = (end_key - 1) >> a.page_shift, page_mask = (1 << a.page_shift) - 1;
+  const int steps = (end_key - first_key + 31) / 32, stages = (steps + 1) / 2;
+  const int last_chunk = (end_key - 1) & ~15, page_mask = (1 << a.page_shift) - 1;
   const uint32_t page_count = static_cast<uint32_t>(min(a.num_pages, 0x7fffffffL));
-  const size_t page_bytes = static_cast<size_t>(D * 2) << a.page_shift;
+  const size_t page_bytes = static_cast<size_t>(D * 2) << a.page_shift, head_bytes = page_bytes * head;
+  const size_t block_bytes = page_bytes * a.kv_heads;
   bool bad = false;
-  // (a last half behind the prompt's end reads the prompt's last page: such scores are masked, such values left out)
-  // (the table is not written while the kernel runs: read as constant memory, by the scalar unit, or each lookup would be a wait for
-  // every load on its way)
-  typedef const __attribute__((address_space(4))) int* constant_ints;
   const constant_ints pages = (constant_ints)reinterpret_cast<uintptr_t>(table);
-  auto lookup = [&](int step) { return pages[min((first_key + min(step, steps - 1) * 32 + 16 * chunk) >> a.page_shift, last_page)]; };
+  // (pieces behind the last key are fetched from the last one's page: their scores are masked, their values left out)
+  auto key_of = [&](int stage) { return min(first_key + stage * 64 + 16 * chunk, last_chunk); };
+  auto lookup = [&](int stage) { return pages[key_of(stage) >> a.page_shift]; };
   auto page_at = [&](int page) {
     const bool outside = static_cast<uint32_t>(page) >= page_count;
     bad |= outside;
-    return (static_cast<size_t>(outside ? 0 : page) * a.kv_heads + head) * page_bytes;
+    return static_cast<size_t>(outside ? 0 : page) * block_bytes + head_bytes;
   };
-  const char* k_bytes = static_cast<const char*>(a.k_pages);
-  const char* v_bytes = static_cast<const char*>(a.v_pages);
-  auto fetch_keys = [&](int step, size_t page) {
-    const int inside = (first_key + min(step, steps - 1) * 32 + 16 * chunk) & page_mask;
-    const char* from = k_bytes + page + static_cast<uint32_t>(inside) * (D * 2u);
+  auto fetch_keys = [&](int stage, size_t page) {
+    if (stage >= stages) return;
+    const char* from = static_cast<const char*>(a.k_pages) + page + static_cast<uint32_t>(key_of(stage) & page_mask) * (D * 2u);
+    const uint32_t to = lds_at + (stage & 3) * kStageBytes + wave * kWideLoads * 1024u;
 #pragma unroll
-    for (int i = 0; i < kWideLoads; ++i) load_to_lds(from, key_from[i], keys_at + (step & 3) * kStepBytes + (wave * kWideLoads + i) * 1024u);
+    for (int i = 0; i < kWideLoads; ++i) load_to_lds(from, key_from[i], to + i * 1024u);
   };
-  auto fetch_values = [&](int step, size_t page) {
-    const int inside = (first_key + min(max(step, 0), steps - 1) * 32 + 16 * chunk) & page_mask;
-    const char* from = v_bytes + page + static_cast<uint32_t>(inside) * 2u;
+  auto fetch_values = [&](int stage, size_t page) {
+    if (stage >= stages) return;
+    const char* from = static_cast<const char*>(a.v_pages) + page + static_cast<uint32_t>(key_of(stage) & page_mask) * 2u;
+    const uint32_t to = lds_at + (4 + (stage & 3)) * kStageBytes + wave * kWideLoads * 1024u;
 #pragma unroll
-    for (int i = 0; i < kWideLoads; ++i)
-      load_to_lds(from, value_from[i], values_at + (step & 3) * kStepBytes + (wave * kWideLoads + i) * 1024u);
+    for (int i = 0; i < kWideLoads; ++i) load_to_lds(from, value_from[i], to + i * 1024u);
   };
   Piece<bf16_t> qf[KC];
   {
-    const long row = min(my_row, a.rows - 1), token = group == 1 ? row : row / group;
+    const long row = min(my_row, rows - 1), token = group == 1 ? row : row / group;
     const bf16_t* q = static_cast<const bf16_t*>(a.q) + (token * a.q_heads + static_cast<long>(head) * group + (row - token * group)) * D + 8 * half;
 #pragma unroll
     for (int c = 0; c < KC; ++c) qf[c] = load_piece<bf16_t>(q + 16 * c);
   }
-  floatx16 o[DT], s, next;
+  // After the middle of stage T's turns nobody reads its keys or the values before it any more: stage T + 4's keys and T + 3's values are
+  // asked for there, where stage T + 2's keys and T + 1's values, asked for two stages earlier, have to have arrived (a turn ends with
+  // reads for the next one).
+  size_t at0 = page_at(lookup(0)), at1 = page_at(lookup(min(1, stages - 1))), at2 = page_at(lookup(min(2, stages - 1)));
+  size_t at3 = page_at(lookup(min(3, stages - 1)));
+  int pending = lookup(min(4, stages - 1));
+  fetch_keys(0, at0);
+  fetch_keys(1, at1); fetch_values(0, at0);
+  fetch_keys(2, at2); fetch_values(1, at1);
+  auto meet = [&](int stage) {
+    constexpr int kL = kWideLoads;
+    if (stage + 3 < stages) arrived<2 * kL>();
+    else if (stage + 2 < stages) arrived<kL>();
+    else arrived<0>();
+  };
+  char* ring = reinterpret_cast<char*>(lds);
+  // (the first turn adds the values of a step -1, of no weight: zeros, until the fourth stage's values come)
+  for (int i = threadIdx.x; i < kStepBytes / 16; i += kWideWaves * kWave)
+    *reinterpret_cast<uintx4*>(ring + 7 * kStageBytes + kStepBytes + i * 16) = uintx4{0u, 0u, 0u, 0u};
+  meet(-1);
+  fetch_keys(3, at3); fetch_values(2, at2);
+
+  floatx16 o[DT], s[2];                    // (scores and weights of two steps, by the step's parity)
+  Piece<bf16_t> weights[2][2];
 #pragma unroll
   for (int t = 0; t < DT; ++t)
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[t][i] = 0.f;
-  float reference = -INFINITY, l = 0.f;
-  Piece<bf16_t> weights[2];
-  const int swizzle = D == 128 ? r & 15 : (r >> 1) & 7;
-  const char* keys = reinterpret_cast<const char*>(lds);
-  auto scores = [&](int step) {
-    const char* row = keys + (step & 3) * kStepBytes + r * D * 2;
-    floatx16 sum;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) sum[i] = 0.f;
-#pragma unroll
-    for (int c = 0; c < KC; ++c) sum = multiply(Piece<bf16_t>{*reinterpret_cast<const uintx4*>(row + (((2 * c + half) ^ swizzle) << 4))}, qf[c], sum);
-    return sum;
+  weights[1][0] = weights[1][1] = empty_piece(bf16_t{});
+  const bf16x2 ones = {static_cast<__bf16>(1.f), static_cast<__bf16>(1.f)};
+  // Where a step's operands begin, hidden from the compiler, which would otherwise add up each operand's place by itself (beyond 64 KB of
+  // LDS places do not fit an instruction).  A key's piece is found by the exchange of the bits above its half, values lie in a row.
+  typedef const __attribute__((address_space(3))) uintx4* lds_pieces;
+  const uint32_t key_lane = lds_at + r * (D * 2u) + ((half ^ (D == 128 ? r & 15 : (r >> 1) & 7)) << 4);
+  const uint32_t value_lane = lds_at + 4 * kStageBytes + lane * 16;
+  auto keys_of = [&](int stage, int which) {
+    uint32_t at = key_lane + ((stage & 3) * kStageBytes + which * kStepBytes);
+    asm volatile("" : "+v"(at));
+    return at;
   };
-  auto add_values = [&](int step, int chunks) {
-    const char* from = keys + 4 * kStepBytes + (step & 3) * kStepBytes + lane * 16;
+  auto values_of = [&](int stage, int which) {
+    uint32_t at = value_lane + ((stage & 3) * kStageBytes + which * kStepBytes);
+    asm volatile("" : "+v"(at));
+    return at;
+  };
+  auto key_operand = [&](uint32_t at, int c) { return *(lds_pieces)(at ^ (c << 5)); };
+  auto value_operand = [&](uint32_t at, int n) { return *(lds_pieces)(at + n * 1024); };
+  uint32_t keys = keys_of(0, 0);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) s[0][i] = 0.f;
+#pragma unroll
+  for (int c = 0; c < KC; ++c) s[0] = multiply(Piece<bf16_t>{key_operand(keys, c)}, qf[c], s[0]);
+  float below = s[0][0], l = 0.f;
+#pragma unroll
+  for (int i = 1; i < 16; ++i) below = fmaxf(below, s[0][i]);
+  if (end_key - first_key < 32) {      // (one step of 16 keys: the others are no scores)
+    below = s[0][0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) below = fmaxf(below, s[0][i]);
+  }
+  below = max_over_halves(below) * a.scale_log2;
+  bool over = !(fabsf(below) < INFINITY);
+  auto pair_of = [&](const floatx16& x, int i) {
+    return bf16_pair(__builtin_amdgcn_exp2f(fmaf(x[i], a.scale_log2, -below)), __builtin_amdgcn_exp2f(fmaf(x[i + 1], a.scale_log2, -below)));
+  };
+  // A turn's order is written down: a matrix instruction, the read of the operand four further on (the next turn's at its end), and as
+  // much of the weights as the vector unit does in the meantime.  The scores come first, so that they are there when the next turn
+  // begins.  `second`: whether step u is a stage's second, known to the compiler: no scores or weights are moved from one turn to the next.
+  constexpr int kSlots = 2 * KC, kAhead = 4;
+  Piece<bf16_t> operand[kAhead];
+  keys = keys_of(0, 1);
+#pragma unroll
+  for (int n = 0; n < kAhead; ++n) operand[n].v = key_operand(keys, n);
+  auto turn = [&](int stage, auto second) {
+    constexpr int B = decltype(second)::value;
+    floatx16 &now = s[B], &next = s[1 - B];
+    Piece<bf16_t> (&made)[2] = weights[B], (&before)[2] = weights[1 - B];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) next[i] = 0.f;
+    float sum = 0.f;
+    const uint32_t values = values_of(stage - 1 + B, 1 - B), further = keys_of(stage + 1, B);
+#pragma unroll
+    for (int n = 0; n < kSlots; ++n) {
+      if (n < KC) next = multiply(operand[n % kAhead], qf[n], next);
+      else o[(n - KC) % DT] = multiply(operand[n % kAhead], before[(n - KC) / DT], o[(n - KC) % DT]);
+      if (n + kAhead < KC) operand[n % kAhead].v = key_operand(keys, n + kAhead);
+      else if (n + kAhead < kSlots) operand[n % kAhead].v = value_operand(values, n + kAhead - KC);
+      else operand[n % kAhead].v = key_operand(further, n + kAhead - kSlots);
+#pragma unroll
+      for (int i = 16 * n / kSlots; i < 16 * (n + 1) / kSlots; ++i)
+        if ((i & 1) != 0) {
+          const uint32_t pair = pair_of(now, i - 1);
+          made[i >> 3].v[(i & 7) >> 1] = pair;
+          sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pair), ones, sum, false);
+        }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    asm volatile("" : "+v"(made[0].v), "+v"(made[1].v), "+v"(sum));     // (made here, beside the products, not where they are used)
+    over |= !(sum <= kLimit);
+    l += sum;
+    keys = further;
+  };
+  typedef std::integral_constant<int, 0> first;
+  typedef std::integral_constant<int, 1> second;
+  int stage = 0;
+  for (; 2 * stage + 2 < steps; ++stage) {
+    turn(stage, first{});
+    at2 = at3;
+    at3 = page_at(pending);
+    pending = lookup(min(stage + 5, stages - 1));
+    meet(stage);
+    fetch_keys(stage + 4, at3);
+    fetch_values(stage + 3, at2);
+    turn(stage, second{});
+  }
+  // the last step: values of the one before it, then its own
+  auto add_values = [&](int of_stage, int which, const Piece<bf16_t> (&w)[2], int chunks) {
+    const uint32_t values = values_of(of_stage, which);
 #pragma unroll
     for (int c = 0; c < 2; ++c)
       if (c < chunks)
 #pragma unroll
-        for (int t = 0; t < DT; ++t) o[t] = multiply(Piece<bf16_t>{*reinterpret_cast<const uintx4*>(from + (c * DT + t) * 1024)}, weights[c], o[t]);
+        for (int t = 0; t < DT; ++t) o[t] = multiply(Piece<bf16_t>{value_operand(values, c * DT + t)}, w[c], o[t]);
   };
-  // the weights of the scores in `s`, and what the sums so far have to be multiplied by: a column's reference point follows its
-  // maximum where weights would pass 2^kSlack
-  float by = 1.f;
-  auto weigh_scores = [&](Piece<bf16_t> (&made)[2]) {
-    float top = s[0];
-#pragma unroll
-    for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
-    top = max_over_halves(top) * a.scale_log2;
-    const float moved = top > reference + kSlack ? top : reference;
-    const float below = moved == -INFINITY ? 0.f : moved;
-    by = __builtin_amdgcn_exp2f(reference - below);
-    l *= by;
-    reference = moved;
-    const bf16x2 ones = {static_cast<__bf16>(1.f), static_cast<__bf16>(1.f)};
-#pragma unroll
-    for (int c = 0; c < 2; ++c)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t pair = bf16_pair(__builtin_amdgcn_exp2f(fmaf(s[8 * c + 2 * i], a.scale_log2, -below)),
-                                        __builtin_amdgcn_exp2f(fmaf(s[8 * c + 2 * i + 1], a.scale_log2, -below)));
-        made[c].v[i] = pair;
-        l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pair), ones, l, false);
-      }
-  };
-  auto rescale = [&]() {
-    if (!__any(by != 1.f)) return;
-#pragma unroll
-    for (int t = 0; t < DT; ++t)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) o[t][i] *= by;
-  };
-  // Turn j asks for the keys of step j + 4 and the values of step j + 2; it needs the keys of step j + 1 and the values of step j - 1,
-  // which turn j - 3 asked for.  (Steps behind the last are asked for as the last again, into slots that nobody reads any more.)
-  constexpr int kOnTheirWay = 4 * kWideLoads;       // of the two turns before
-  size_t at0, at1, at2;                             // pages of steps j + 2, j + 3 and j + 4
-  at0 = page_at(lookup(0));
-  at1 = page_at(lookup(1));
-  at2 = page_at(lookup(2));
-  const size_t at3 = page_at(lookup(3));
-  int pending = lookup(4);
-  fetch_keys(0, at0); fetch_values(0, at0);
-  fetch_keys(1, at1); fetch_values(0, at0);         // (twice: every turn asks for as much)
-  fetch_keys(2, at2); fetch_values(0, at0);
-  arrived<kOnTheirWay>();
-  fetch_keys(3, at3); fetch_values(1, at1);
-  s = scores(0);
-  at0 = at2;
-  at1 = at3;
-  for (int j = 0; j + 1 < steps; ++j) {
-    at2 = page_at(pending);
-    pending = lookup(j + 5);
-    arrived<kOnTheirWay>();
-    fetch_keys(j + 4, at2);
-    fetch_values(j + 2, at0);
-    at0 = at1;
-    at1 = at2;
-    next = scores(j + 1);
-    Piece<bf16_t> made[2];
-    weigh_scores(made);
-    if (j > 0) add_values(j - 1, 2);
-    asm volatile("" : "+v"(made[0].v), "+v"(made[1].v), "+v"(l));     // (made here, beside the products, and not behind the branch)
-    rescale();
-    weights[0] = made[0];
-    weights[1] = made[1];
-    s = next;
+  const int there = end_key - first_key - (steps - 1) * 32;     // keys of the last step: 16 or 32
+  int second_step = 0;
+  if (2 * stage + 1 < steps) {
+    turn(stage, first{});
+    second_step = 1;
+    s[0] = s[1];
+    weights[1][0] = weights[0][0];
+    weights[1][1] = weights[0][1];
   }
   arrived<0>();
-  if (steps > 1) add_values(steps - 2, 2);
-  const int there = end_key - first_key - (steps - 1) * 32;       // keys of the last step: 16 or 32
+  add_values(stage - 1 + second_step, 1 - second_step, weights[1], 2);
   if (there < 32) {
 #pragma unroll
-    for (int i = 8; i < 16; ++i) s[i] = -INFINITY;
+    for (int i = 8; i < 16; ++i) s[0][i] = -INFINITY;
   }
-  Piece<bf16_t> made[2];
-  weigh_scores(made);
-  rescale();
-  weights[0] = made[0];
-  weights[1] = made[1];
-  if (there < 32) add_values(steps - 1, 1);
-  else add_values(steps - 1, 2);
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; i += 2) {
+    const uint32_t pair = pair_of(s[0], i);
+    weights[0][i >> 3].v[(i & 7) >> 1] = pair;
+    sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pair), ones, sum, false);
+  }
+  over |= !(sum <= kLimit);
+  l += sum;
+  add_values(stage, second_step, weights[0], there < 32 ? 1 : 2);
   l = sum_over_halves(l);
+  const unsigned long long passed = __ballot(over && my_row < rows);
+  const uint32_t mask = static_cast<uint32_t>(passed) | static_cast<uint32_t>(passed >> 32);
+  if (lane == 0) over_of[wave] = mask;
   const bool spoilt = __syncthreads_or(bad);
-  if (my_row >= a.rows) return;
+  if (my_row >= rows || ((mask >> r) & 1u) != 0u) return;
   const int segments = a.prefix_segments + a.own_segments;
   if (half == 0) {
     float* at = a.stats + ((static_cast<size_t>(head) * a.rows + my_row) * segments + segment) * 2;
-    at[0] = reference;
+    at[0] = below;
     at[1] = spoilt ? NAN : l;
   }
   float* sums = a.sums + ((static_cast<size_t>(head) * segments + segment) * a.rows + my_row) * D + 4 * half;
@@ -552,10 +605,34 @@ __device__ __forceinline__ void walk_wide(const Args& a, const int* table, int h
     for (int i = 0; i < 4; ++i) *reinterpret_cast<floatx4*>(sums + 32 * t + 8 * i) = floatx4{o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]};
 }
 
+// Blocks take (segment and head, tile of 256 columns) of the prefix.
+__global__ __launch_bounds__(kWideWaves * kWave, 2) void wide_prefix_kernel(Args a) {
+  extern __shared__ __attribute__((aligned(1024))) float aligned_lds[];     // (a row's pieces are exchanged by the low bits of their places)
+  float* lds = aligned_lds;
+  // Blocks go to the XCDs in turn: the tiles of one segment and head, which read the same pages, stand eight apart, on one XCD.
+  const int items = a.prefix_segments * a.kv_heads, run = static_cast<int>(blockIdx.x / (kXcds * a.prefix_tiles)) * kXcds;
+  const int in_run = static_cast<int>(blockIdx.x) - run * a.prefix_tiles, wide = min(kXcds, items - run);
+  const int tile = in_run / wide, item = run + in_run % wide, head = item % a.kv_heads, segment = item / a.kv_heads;
+  const int first = segment * a.prefix_keys, end = min(a.shared, first + a.prefix_keys);
+  const int* table = a.block_table + (a.table_rows != nullptr ? static_cast<size_t>(a.table_rows[0]) * a.table_width : 0);
+  // (rows behind the last request's may hold anything, and nobody asks for them)
+  const long rows = min(a.rows, static_cast<long>(max(a.q_start[a.requests], 0)) * static_cast<long>(a.group.by));
+  const long row0 = static_cast<long>(kWideColumns) * tile;
+  __shared__ uint32_t over[kWideWaves];
+  if (row0 >= rows) return;
+  walk_wide(a, table, head, row0, rows, first, end, segment, lds, over);
+  for (int w = 0; w < kWideWaves; ++w) {
+    if (over[w] == 0u) continue;
+    __syncthreads();
+    const long at = row0 + 32 * w;
+    walk<bf16_t, kWideWaves>(a, table, head, at, static_cast<int>(min(32L, rows - at)), first, end, end, end, segment, lds, over[w]);
+  }
+}
+
 // Blocks 0 .. prefix_blocks - 1 take (segment and head, tile) of the prefix, the others (request, head, tile, segment) of the requests'
 // own keys.
-template <typename T, bool WIDE>
-__global__ __launch_bounds__(WIDE ? kWideWaves * kWave : kThreads, (sizeof(T) == 4 || D > 128 ? 1 : 2)) void shared_prefix_kernel(Args a) {
+template <typename T>
+__global__ __launch_bounds__(kThreads, (sizeof(T) == 4 || D > 128 ? 1 : 2)) void shared_prefix_kernel(Args a) {
   extern __shared__ float lds[];
   long block = blockIdx.x;
   const int lane = threadIdx.x & (kWave - 1), r = lane & 31;
@@ -568,12 +645,6 @@ __global__ __launch_bounds__(WIDE ? kWideWaves * kWave : kThreads, (sizeof(T) ==
     const int tile = in_run / wide, item = run + in_run % wide;
     head = item % a.kv_heads;
     segment = item / a.kv_heads;
-    if constexpr (WIDE) {
-      const int from = segment * a.prefix_keys;
-      const int* table = a.block_table + (a.table_rows != nullptr ? static_cast<size_t>(a.table_rows[0]) * a.table_width : 0);
-      walk_wide(a, table, head, static_cast<long>(kWideColumns) * tile, from, min(a.shared, from + a.prefix_keys), segment, lds);
-      return;
-    }
     row0 = 32L * tile;
     columns = static_cast<int>(min(32L, a.rows - row0));
     first = segment * a.prefix_keys;
@@ -601,15 +672,19 @@ __global__ __launch_bounds__(WIDE ? kWideWaves * kWave : kThreads, (sizeof(T) ==
     segment += a.prefix_segments;
   }
   const int row = a.table_rows != nullptr ? a.table_rows[request] : request;
-  walk<T, WIDE ? kWideWaves : kWaves>(a, a.block_table + static_cast<size_t>(row) * a.table_width, head, row0, columns, first, end, visible, all_see, segment, lds);
+  walk<T, kWaves>(a, a.block_table + static_cast<size_t>(row) * a.table_width, head, row0, columns, first, end, visible, all_see, segment, lds);
 }
 
-// A wave a (token, query head), four of a token a block: the row's segments joined.  What a row waits for is a chain of reads - whose
-// the token is, the segments' maxima and sums, their values -, so many short waves run beside each other: no wave waits for another.
-template <typename T>
+// A row - (token, query head) - a wave, four of a token a block, or, SHARE, where there are too few rows to fill the device, a block: its
+// waves then take the segments in turn.  What a row waits for is a chain of reads - whose the token is, the segments' maxima and sums,
+// their values -, so many short waves run beside each other.
+template <typename T, bool SHARE>
 __global__ __launch_bounds__(kThreads) void join_kernel(Args a) {
   constexpr int kEach = (D + kWave - 1) / kWave;                // dims of a lane, kEach in a row (the last lanes may have none)
-  const int token = blockIdx.x, q_head = blockIdx.y * kWaves + threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
+  constexpr int kStride = SHARE ? kWaves : 1;
+  __shared__ float shares[SHARE ? kWaves : 1][kEach * kWave];
+  const int token = blockIdx.x, lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const int q_head = SHARE ? blockIdx.y : blockIdx.y * kWaves + wave;
   if (q_head >= a.q_heads) return;
   const int group = static_cast<int>(a.group.by), head = a.group.quotient(q_head);
   int before = 0;                                               // requests whose first row is this token's or lies before it
@@ -647,18 +722,18 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Args a) {
       total += wave_sum(weight * one.y);
       const int run = min(kWave, used - i0);
       constexpr int kAhead = 8;                                 // segments whose values are on their way together
-      for (int i = 0; i < run; i += kAhead) {
+      for (int i = SHARE ? wave : 0; i < run; i += kAhead * kStride) {
         float fetched[kAhead][kEach];
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-          const float* at = sums + static_cast<size_t>(i0 + min(i + u, run - 1)) * a.rows * D;
+          const float* at = sums + static_cast<size_t>(i0 + min(i + u * kStride, run - 1)) * a.rows * D;
 #pragma unroll
           for (int e = 0; e < kEach; ++e) fetched[u][e] = at[e];
         }
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-          const float by = __shfl(weight, min(i + u, run - 1), kWave);
-          if (i + u < run) {
+          const float by = __shfl(weight, min(i + u * kStride, run - 1), kWave);
+          if (i + u * kStride < run) {
 #pragma unroll
             for (int e = 0; e < kEach; ++e) sum[e] = fmaf(by, fetched[u][e], sum[e]);
           }
@@ -666,26 +741,54 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Args a) {
       }
     }
   }
+  if constexpr (SHARE) {
+    if (wave != 0) {
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) shares[wave][e * kWave + lane] = sum[e];
+    }
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w)
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) sum[e] += shares[w][e * kWave + lane];
+  }
   if (here) {
 #pragma unroll
     for (int e = 0; e < kEach; ++e) out[e] = from_float<T>(sum[e] / total);
   }
 }
 
-template <typename T, bool WIDE> int run(const Args& a, hipStream_t stream) {
-  constexpr int waves = WIDE ? kWideWaves : kWaves;
-  constexpr size_t narrow = (waves * 32 * kRow + waves * 32 * 2) * sizeof(float);
-  constexpr size_t lds = WIDE && kWideLds > narrow ? kWideLds : narrow;
-  static_assert(lds <= 160 * 1024, "LDS of a compute unit");
+template <typename K> int room_for(K kernel, size_t lds) {
+  static_assert(kWideLds <= 160 * 1024 && kWideNarrowLds <= 160 * 1024, "LDS of a compute unit");
+  return static_cast<int>(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
+}
+
+// `wide`: the prefix goes to `wide_prefix_kernel`, and the requests' own keys alone to the other one, which holds twice as many blocks a
+// unit.
+template <typename T> int run(const Args& all, bool wide, hipStream_t stream) {
+  constexpr size_t lds = narrow_lds(kWaves);
+  Args a = all;
+  int status = 0;
+  if constexpr (kWideFits && sizeof(T) == 2)
+    if (wide && a.prefix_blocks > 0) {
+      constexpr size_t wide_lds = kWideLds > kWideNarrowLds ? kWideLds : kWideNarrowLds;
+      if (a.prefix_blocks > 0x7fffffffL) return -2;
+      if ((status = room_for(wide_prefix_kernel, wide_lds)) != 0) return status;
+      wide_prefix_kernel<<<static_cast<unsigned>(a.prefix_blocks), kWideWaves * kWave, wide_lds, stream>>>(a);
+      if ((status = AKV_LAUNCH_STATUS()) != 0) return status;
+      a.prefix_blocks = 0;
+    }
   const long blocks = a.prefix_blocks + static_cast<long>(a.requests) * a.kv_heads * a.own_tiles * a.own_segments;
   if (blocks > 0x7fffffffL || a.q_heads > 65535) return -2;
-  if (hipFuncSetAttribute(reinterpret_cast<const void*>(shared_prefix_kernel<T, WIDE>), hipFuncAttributeMaxDynamicSharedMemorySize,
-                          static_cast<int>(lds)) != hipSuccess)
-    return static_cast<int>(hipGetLastError());
-  shared_prefix_kernel<T, WIDE><<<static_cast<unsigned>(blocks), waves * kWave, lds, stream>>>(a);
-  const int status = AKV_LAUNCH_STATUS();
-  if (status != 0) return status;
-  join_kernel<T><<<dim3(static_cast<unsigned>(a.tokens), (a.q_heads + kWaves - 1) / kWaves), kThreads, 0, stream>>>(a);
+  if ((status = room_for(shared_prefix_kernel<T>, lds)) != 0) return status;
+  shared_prefix_kernel<T><<<static_cast<unsigned>(blocks), kThreads, lds, stream>>>(a);
+  if ((status = AKV_LAUNCH_STATUS()) != 0) return status;
+  // (a wave a row where they are 2,048 and more, eight of a unit's thirty-two)
+  if (a.tokens * a.q_heads >= 8L * device_facts().compute_units)
+    join_kernel<T, false><<<dim3(static_cast<unsigned>(a.tokens), (a.q_heads + kWaves - 1) / kWaves), kThreads, 0, stream>>>(a);
+  else
+    join_kernel<T, true><<<dim3(static_cast<unsigned>(a.tokens), a.q_heads), kThreads, 0, stream>>>(a);
   return AKV_LAUNCH_STATUS();
 }
 
@@ -696,7 +799,7 @@ template <typename T, bool WIDE> int run(const Args& a, hipStream_t stream) {
 
 // `sums` and `stats` hold kv_heads * (prefix_segments + own_segments) * tokens * (q_heads / kv_heads) rows of head size and of two
 // floats; segments: prefix_segments of prefix_keys (multiples of 32) cover `shared`, own_segments of own_keys `max_own` keys of a
-// request behind it, at most 512 together.  `wide`: the prompt's columns go in tiles of 128 (`walk_wide`).  Operands lie on 16-byte boundaries.
+// request behind it, at most 512 together.  `wide`: the prompt's columns go in tiles of 256 (`walk_wide`).  Operands lie on 16-byte boundaries.
 extern "C" int AKV_NAME(AKV_HEAD_DIM)(const void* q, const void* k_pages, const void* v_pages, void* out, int dtype, float* sums, float* stats,
                                       const int* q_start, const int* seq_lens, const int* block_table, const int* table_rows, int table_width,
                                       int requests, long tokens, int q_heads, int kv_heads, int page_size, long num_pages, float scale,
@@ -721,9 +824,7 @@ extern "C" int AKV_NAME(AKV_HEAD_DIM)(const void* q, const void* k_pages, const 
   a.prefix_tiles = static_cast<int>(wide != 0 ? (a.rows + kWideColumns - 1) / kWideColumns : (a.rows + 31) / 32);
   a.own_tiles = static_cast<int>((static_cast<long>(max_new) * group + 31) / 32);
   a.prefix_blocks = static_cast<long>(prefix_segments) * kv_heads * a.prefix_tiles;
-  if constexpr (kWideFits)
-    if (wide != 0) return run<bf16_t, true>(a, stream);
-  if (dtype == kF32) return run<float, false>(a, stream);
-  if (dtype == kBF16) return run<bf16_t, false>(a, stream);
+  if (dtype == kF32) return run<float>(a, false, stream);
+  if (dtype == kBF16) return run<bf16_t>(a, wide != 0, stream);
   return -1;
 }

@@ -22,26 +22,31 @@ def _ptr(t):
 
 
 def wide_tiles(rows: int, head_dim: int, page_size: int, dtype) -> bool:
-    """Whether the prompt's keys are multiplied for tiles of 128 columns that share them (`walk_wide`) rather than of 32."""
+    """Whether the prompt's keys are multiplied for tiles of 256 columns that share them (`walk_wide`) rather than of 32."""
     return dtype == torch.bfloat16 and head_dim in (64, 128) and page_size >= 16 and rows > 32
 
 
-def cut_prefix(columns: int, rows: int, kv_heads: int, shared: int, units: int) -> tuple[int, int]:
-    """(segments, keys of one) of a shared prompt: two blocks of `columns` rows a unit, segments of 128 keys at least."""
+def cut_own(requests: int, rows: int, kv_heads: int, most: int, units: int) -> tuple[int, int]:
+    """(segments, keys of one) of up to `most` keys that a request of up to `rows` rows a kv head holds behind the prompt: 256 keys, two
+    steps for each of a block's waves, so that a long request's blocks do not outlast the others'; 128 where that leaves units idle; more
+    where the bound is loose, as blocks without keys cost a look at the lengths each."""
+    blocks = requests * kv_heads * ((rows + 31) // 32)
+    keys = 128 if blocks * ((most + 255) // 256) < units else 256
+    segments = max(1, min((most + keys - 1) // keys, max(1, 16 * units // blocks), 256))
+    keys = ((most + segments - 1) // segments + 127) // 128 * 128
+    return (most + keys - 1) // keys, keys
+
+
+def cut_prefix(columns: int, rows: int, kv_heads: int, shared: int, units: int, own_blocks: int) -> tuple[int, int]:
+    """The same of a shared prompt, whose blocks take `columns` rows each: as many as the device holds at once, one a unit of
+    256 columns or two of 32, segments of 128 keys at least.  Tiles of 32 columns wait for reads, and leave room for up to half as many blocks of the requests' own keys beside them."""
     if shared == 0:
         return 0, 32
     blocks = kv_heads * ((rows + columns - 1) // columns)
-    segments = max(1, min(2 * units // blocks, (shared + 127) // 128, 128))
+    room = 2 * units - min(own_blocks, units) if columns == 32 else units
+    segments = max(1, min(room // blocks, (shared + 127) // 128, 128))
     keys = ((shared + segments - 1) // segments + 127) // 128 * 128
     return (shared + keys - 1) // keys, keys
-
-
-def cut_own(requests: int, rows: int, kv_heads: int, most: int, units: int) -> tuple[int, int]:
-    """The same of up to `most` keys that a request of up to `rows` rows a kv head holds behind the prompt."""
-    blocks = requests * kv_heads * ((rows + 31) // 32)
-    segments = max(1, min(4 * units // blocks, (most + 127) // 128, 128))
-    keys = ((most + segments - 1) // segments + 127) // 128 * 128
-    return (most + keys - 1) // keys, keys
 
 
 class RoundKernels:
@@ -141,8 +146,9 @@ class RoundKernels:
         group = q_heads // kv_heads
         max_new_tokens = min(max_new_tokens, tokens)
         wide = wide_tiles(tokens * group, head_dim, page_size, q.dtype)
-        prefix_segments, prefix_keys = cut_prefix(128 if wide else 32, tokens * group, kv_heads, shared, self.compute_units)
         own_segments, own_keys = cut_own(requests, max_new_tokens * group, kv_heads, max_seq_len - shared, self.compute_units)
+        own_blocks = requests * kv_heads * own_segments
+        prefix_segments, prefix_keys = cut_prefix(256 if wide else 32, tokens * group, kv_heads, shared, self.compute_units, own_blocks)
         segments = prefix_segments + own_segments
         # (from torch's pool: a recorded call then has room of its own, and calls on other streams do not meet in one)
         room = torch.empty(segments * tokens * q_heads * (head_dim + 2), dtype=torch.float32, device=self.device)
