@@ -32,7 +32,9 @@ constexpr int KC = D / 16;             // steps of 16 dims of the score product
 constexpr int DT = (D + 31) / 32;      // tiles of 32 dims of the output (the last may be half empty)
 constexpr int kThreads = 256, kWaves = 4;
 constexpr int kRow = D + 4;            // floats a column takes in LDS: rows then lie 4 banks apart
-constexpr size_t narrow_lds(int waves) { return (waves * 32 * kRow + waves * 32 * 2) * sizeof(float); }     // of `walk`
+template <typename T> constexpr size_t narrow_lds(int waves) {      // of `walk`
+  return (waves / 2 * 32 * kRow + waves * 32 * 2 + 64) * sizeof(float) + D * 32 * sizeof(T);
+}
 constexpr float kLog2e = 1.4426950408889634f;
 
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
@@ -164,47 +166,53 @@ __device__ __forceinline__ float sum_over_halves(float v) {
 template <typename T, int WAVES>
 __device__ __forceinline__ void walk(const Args& a, const int* table, int head, long row0, int columns, int first_key, int end_key,
                                      int visible, int all_see, int segment, float* lds, uint32_t wanted = 0xffffffffu) {
+  constexpr int kBuffers = WAVES / 2;
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   const int r = lane & 31, half = lane >> 5;
   const int group = static_cast<int>(a.group.by), segments = a.prefix_segments + a.own_segments;
   const int page_mask = (1 << a.page_shift) - 1;
-  Piece<T> qf[KC];
-  {
-    const long row = row0 + min(r, columns - 1);
-    const long token = group == 1 ? row : row / group;
-    const T* q = static_cast<const T*>(a.q) + (token * a.q_heads + static_cast<long>(head) * group + (row - token * group)) * D + 8 * half;
-#pragma unroll
-    for (int c = 0; c < KC; ++c) qf[c] = load_piece<T>(q + 16 * c);
-  }
-  floatx16 o[DT];
-#pragma unroll
-  for (int t = 0; t < DT; ++t)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) o[t][i] = 0.f;
-  float m = -INFINITY, l = 0.f;       // (m is the column's, l what this lane's keys add to its sum)
-  bool bad = false;
-  // the key of the step that this lane's row of A holds
+  // in LDS: half the waves' results, a row a column; every wave's maxima and sums; what a column sees; the queries, as operands
+  float* shares = lds + kBuffers * 32 * kRow;         // [waves][32][2]
+  int* seen = reinterpret_cast<int*>(shares + WAVES * 32 * 2);      // [32], and whether a masked value was not finite
+  Piece<T>* queries = reinterpret_cast<Piece<T>*>(seen + 64);       // [KC][lane]
+  // the key of a step that this lane's row of A holds
   const int key_at = 16 * (r >> 4) + 8 * ((r >> 2) & 1) + 4 * ((r >> 3) & 1) + (r & 3);
-  auto page_of = [&](int key) {
-    const int page = table[key >> a.page_shift];
+  bool bad = false;
+  // A step's loads are asked for while the step before is worked on - its keys when those before have been multiplied, its values when
+  // those before have -, and what the table says of their pages a step earlier still.
+  int key_page = 0, value_pages[2] = {0, 0};
+  auto lookup = [&](int base) {
+    key_page = table[min(base + key_at, end_key - 1) >> a.page_shift];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) value_pages[c] = table[min(base + 16 * c + 8 * half, end_key - 1) >> a.page_shift];
+  };
+  auto place_of = [&](int page) {
     const bool outside = page < 0 || page >= a.num_pages;
     bad |= outside;
     return static_cast<size_t>(outside ? 0 : page) * a.kv_heads + head;
   };
-  // A step's loads are asked for while the step before is worked on: its keys when those before have been multiplied, its values when
-  // those before have.
+  const int first_base = first_key + 32 * wave;
+  if (first_base < end_key) lookup(first_base);
+  for (int c = wave; c < KC; c += WAVES) {
+    const long row = row0 + min(r, columns - 1);
+    const long token = group == 1 ? row : row / group;
+    const T* q = static_cast<const T*>(a.q) + (token * a.q_heads + static_cast<long>(head) * group + (row - token * group)) * D + 8 * half;
+    queries[c * kWave + lane] = load_piece<T>(q + 16 * c);
+  }
+  if (wave == 0 && half == 0) seen[r] = visible;
+  if (threadIdx.x == 0) seen[32] = 0;
   Piece<T> kf[KC], vf[2][DT];
-  auto fetch_keys = [&](int base) {
+  auto fetch_keys = [&](int base, int page) {
     const int key = min(base + key_at, end_key - 1);
-    const T* k = static_cast<const T*>(a.k_pages) + ((page_of(key) << a.page_shift) + (key & page_mask)) * D + 8 * half;
+    const T* k = static_cast<const T*>(a.k_pages) + ((place_of(page) << a.page_shift) + (key & page_mask)) * D + 8 * half;
 #pragma unroll
     for (int c = 0; c < KC; ++c) kf[c] = load_piece<T>(k + 16 * c);
   };
-  auto fetch_values = [&](int base) {
+  auto fetch_values = [&](int base, const int (&pages)[2]) {
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const int octet = min(base + 16 * c + 8 * half, (end_key - 1) & ~7);
-      const T* v = static_cast<const T*>(a.v_pages) + ((page_of(octet) * D + r) << a.page_shift) + (octet & page_mask);
+      const T* v = static_cast<const T*>(a.v_pages) + ((place_of(pages[c]) * D + r) << a.page_shift) + (octet & page_mask);
 #pragma unroll
       for (int t = 0; t < DT; ++t) {
         if (D % 32 == 0 || t + 1 < DT || r < 16) vf[c][t] = load_piece<T>(v + (static_cast<size_t>(32 * t) << a.page_shift));
@@ -212,21 +220,31 @@ __device__ __forceinline__ void walk(const Args& a, const int* table, int head, 
       }
     }
   };
-  float* mine = lds + wave * 32 * kRow;       // the wave's results, a row a column
-  bool odd = false;                           // whether values that are not finite stand there already
-  const int first_base = first_key + 32 * wave;
+  floatx16 o[DT];
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[t][i] = 0.f;
+  float m = -INFINITY, l = 0.f;       // (m is the column's, l what this lane's keys add to its sum)
+  bool odd = false;                   // whether a value that some column does not see was not finite
   if (first_base < end_key) {
-    fetch_keys(first_base);
-    fetch_values(first_base);
+    fetch_keys(first_base, key_page);
+    fetch_values(first_base, value_pages);
+    if (first_base + 32 * WAVES < end_key) lookup(first_base + 32 * WAVES);
   }
+  __syncthreads();
   for (int base = first_base; base < end_key; base += 32 * WAVES) {
     floatx16 s;
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] = 0.f;
 #pragma unroll
-    for (int c = 0; c < KC; ++c) s = multiply(kf[c], qf[c], s);
+    for (int c = 0; c < KC; ++c) s = multiply(kf[c], queries[c * kWave + lane], s);
     const bool more = base + 32 * WAVES < end_key;
-    if (more) fetch_keys(base + 32 * WAVES);
+    const int next_pages[2] = {value_pages[0], value_pages[1]};
+    if (more) {
+      fetch_keys(base + 32 * WAVES, key_page);
+      if (base + 64 * WAVES < end_key) lookup(base + 64 * WAVES);
+    }
     const bool ends = base + 32 > end_key, masked = all_see < end_key && base + 32 > all_see;
     if (ends || masked) {
       const int limit = min(visible, end_key) - base - 8 * half;
@@ -260,46 +278,33 @@ __device__ __forceinline__ void walk(const Args& a, const int* table, int head, 
       p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.scale_log2, -reference));
       l += p[i];
     }
-    bool fine = true;
     if (masked) {
+      // A key that some column does not see may have a value that is not finite, and 0 times it would reach that column: such values are
+      // left out of the product, and added to the columns that see their key when the results are written.
+      bool fine = true;
 #pragma unroll
       for (int c = 0; c < 2; ++c)
 #pragma unroll
         for (int t = 0; t < DT; ++t) fine = fine && all_finite(vf[c][t]);
-    }
-    if (!__all(fine)) {
-      // A key that some column does not see has a value that is not finite, and 0 times it would reach that column: such values are
-      // left out of the product and added, as they are, to the dims of the columns that see their key (any weight times them is
-      // the same), in LDS until the waves' results are joined.
-      if (!odd)
-        for (int i = lane; i < 32 * kRow; i += kWave) mine[i] = 0.f;
-      odd = true;
-      __builtin_amdgcn_wave_barrier();
-      for (int dim = half; dim < D; dim += 2) {
-        float sum = 0.f;
-        for (int j = base; j < min(base + 32, min(end_key, visible)); ++j) {
-          const float v = to_float(static_cast<const T*>(a.v_pages)[((page_of(j) * D + dim) << a.page_shift) + (j & page_mask)]);
-          if (!(fabsf(v) < INFINITY)) sum += v;
-        }
-        mine[r * kRow + dim] += sum;
+      if (!__all(fine)) {
+        odd = true;
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int t = 0; t < DT; ++t) keep_finite(vf[c][t]);
       }
-#pragma unroll
-      for (int c = 0; c < 2; ++c)
-#pragma unroll
-        for (int t = 0; t < DT; ++t) keep_finite(vf[c][t]);
     }
 #pragma unroll
     for (int c = 0; c < 2; ++c)
 #pragma unroll
       for (int t = 0; t < DT; ++t) o[t] = weigh(vf[c][t], p + 8 * c, o[t]);
-    if (more) fetch_values(base + 32 * WAVES);
+    if (more) fetch_values(base + 32 * WAVES, next_pages);
   }
   l = sum_over_halves(l);
   if (__any(bad)) m = l = NAN;
-  // the waves' results, joined through LDS
-  float* shares = lds + WAVES * 32 * kRow;     // [waves][32][2]
-  __syncthreads();
+  // the waves' results, joined through LDS: half of the waves hand theirs to the others, whose sums the block adds up
   if (half == 0) { shares[(wave * 32 + r) * 2] = m; shares[(wave * 32 + r) * 2 + 1] = l; }
+  if (odd && lane == 0) seen[32] = 1;          // (every writer stores the same value)
   __syncthreads();
   float top = -INFINITY, whole = 0.f;
 #pragma unroll
@@ -308,31 +313,46 @@ __device__ __forceinline__ void walk(const Args& a, const int* table, int head, 
 #pragma unroll
   for (int w = 0; w < WAVES; ++w) whole += shares[(w * 32 + r) * 2 + 1] * __builtin_amdgcn_exp2f(shares[(w * 32 + r) * 2] - reference);
   const float by = __builtin_amdgcn_exp2f(m - reference);
+  float* mine = lds + ((wave % kBuffers) * 32 + r) * kRow;
 #pragma unroll
-  for (int t = 0; t < DT; ++t)
+  for (int turn = 0; turn < 2; ++turn) {
+    if ((wave < kBuffers) == (turn == 1) && r < columns) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int dim = 32 * t + 8 * q + 4 * half;
-      if (D % 32 == 0 || dim < D) {
-        floatx4 four = {o[t][4 * q] * by, o[t][4 * q + 1] * by, o[t][4 * q + 2] * by, o[t][4 * q + 3] * by};
-        floatx4* at = reinterpret_cast<floatx4*>(mine + r * kRow + dim);
-        if (odd) four += *at;
-        *at = four;
-      }
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int dim = 32 * t + 8 * q + 4 * half;
+          if (D % 32 == 0 || dim < D) {
+            floatx4 four = {o[t][4 * q] * by, o[t][4 * q + 1] * by, o[t][4 * q + 2] * by, o[t][4 * q + 3] * by};
+            floatx4* at = reinterpret_cast<floatx4*>(mine + dim);
+            *at = turn == 0 ? four : four + *at;
+          }
+        }
     }
-  __syncthreads();
+    __syncthreads();
+  }
   if (wave == 0 && half == 0 && r < columns && ((wanted >> r) & 1u) != 0u) {
     float* at = a.stats + ((static_cast<size_t>(head) * a.rows + row0 + r) * segments + segment) * 2;
     at[0] = top;
     at[1] = whole;
   }
   float* sums = a.sums + ((static_cast<size_t>(head) * segments + segment) * a.rows + row0) * D;
-  for (int i = threadIdx.x; i < columns * (D / 4); i += (WAVES * kWave)) {
+  const bool any_odd = seen[32] != 0;
+  for (int i = threadIdx.x; i < columns * (D / 4); i += WAVES * kWave) {
     const int column = i / (D / 4), at = i % (D / 4) * 4;
     if (((wanted >> column) & 1u) == 0u) continue;
     floatx4 sum = *reinterpret_cast<const floatx4*>(lds + column * kRow + at);
 #pragma unroll
-    for (int w = 1; w < WAVES; ++w) sum += *reinterpret_cast<const floatx4*>(lds + (w * 32 + column) * kRow + at);
+    for (int w = 1; w < kBuffers; ++w) sum += *reinterpret_cast<const floatx4*>(lds + (w * 32 + column) * kRow + at);
+    if (any_odd)      // (any weight times such a value is the same; only keys that some column does not see were looked at)
+      for (int j = first_key + (max(0, all_see - first_key) & ~31); j < min(end_key, seen[column]); ++j) {
+        const size_t place = place_of(table[j >> a.page_shift]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float v = to_float(static_cast<const T*>(a.v_pages)[((place * D + at + e) << a.page_shift) + (j & page_mask)]);
+          if (!(fabsf(v) < INFINITY)) sum[e] += v;
+        }
+      }
     *reinterpret_cast<floatx4*>(sums + static_cast<size_t>(column) * D + at) = sum;
   }
 }
@@ -354,7 +374,7 @@ constexpr bool kWideFits = D == 64 || D == 128;
 constexpr int kWideWaves = 8, kWideColumns = 32 * kWideWaves;
 constexpr int kStepBytes = (kWideFits ? 32 * D : 32 * 64) * 2, kStageBytes = 2 * kStepBytes;      // of a step's or a stage's keys, and of its values
 constexpr int kWideLoads = kStageBytes / 1024 / kWideWaves;               // instructions a wave for a stage's keys, and for its values
-constexpr size_t kWideLds = 8 * kStageBytes, kWideNarrowLds = kWideFits ? narrow_lds(kWideWaves) : 0;
+constexpr size_t kWideLds = 8 * kStageBytes, kWideNarrowLds = kWideFits ? narrow_lds<bf16_t>(kWideWaves) : 0;
 constexpr float kLimit = 0x1p40f;  // what a lane's sixteen weights of a step may sum up to
 
 typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
@@ -605,14 +625,21 @@ __device__ __forceinline__ void walk_wide(const Args& a, const int* table, int h
     for (int i = 0; i < 4; ++i) *reinterpret_cast<floatx4*>(sums + 32 * t + 8 * i) = floatx4{o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]};
 }
 
+// Blocks go to the XCDs in turn: the tiles of one item, which read the same pages, stand eight apart, on one XCD and in its cache.
+__device__ __forceinline__ void tile_of(long block, long items, int tiles, long& item, int& tile) {
+  const long run = block / (static_cast<long>(kXcds) * tiles) * kXcds, in_run = block - run * tiles, wide = min(static_cast<long>(kXcds), items - run);
+  tile = static_cast<int>(in_run / wide);
+  item = run + in_run % wide;
+}
+
 // Blocks take (segment and head, tile of 256 columns) of the prefix.
 __global__ __launch_bounds__(kWideWaves * kWave, 2) void wide_prefix_kernel(Args a) {
   extern __shared__ __attribute__((aligned(1024))) float aligned_lds[];     // (a row's pieces are exchanged by the low bits of their places)
   float* lds = aligned_lds;
-  // Blocks go to the XCDs in turn: the tiles of one segment and head, which read the same pages, stand eight apart, on one XCD.
-  const int items = a.prefix_segments * a.kv_heads, run = static_cast<int>(blockIdx.x / (kXcds * a.prefix_tiles)) * kXcds;
-  const int in_run = static_cast<int>(blockIdx.x) - run * a.prefix_tiles, wide = min(kXcds, items - run);
-  const int tile = in_run / wide, item = run + in_run % wide, head = item % a.kv_heads, segment = item / a.kv_heads;
+  long item;
+  int tile;
+  tile_of(blockIdx.x, static_cast<long>(a.prefix_segments) * a.kv_heads, a.prefix_tiles, item, tile);
+  const int head = static_cast<int>(item % a.kv_heads), segment = static_cast<int>(item / a.kv_heads);
   const int first = segment * a.prefix_keys, end = min(a.shared, first + a.prefix_keys);
   const int* table = a.block_table + (a.table_rows != nullptr ? static_cast<size_t>(a.table_rows[0]) * a.table_width : 0);
   // (rows behind the last request's may hold anything, and nobody asks for them)
@@ -636,27 +663,24 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 || D > 128 ? 1 : 2)) void
   extern __shared__ float lds[];
   long block = blockIdx.x;
   const int lane = threadIdx.x & (kWave - 1), r = lane & 31;
-  int head, segment, request = 0, columns, first, end, visible, all_see;
-  long row0;
+  int head, segment, request = 0, columns, first, end, visible, all_see, tile;
+  long row0, item;
   if (block < a.prefix_blocks) {
-    // Blocks go to the XCDs in turn: the tiles of one segment and head, which read the same pages, stand eight apart, on one XCD.
-    const int items = a.prefix_segments * a.kv_heads, run = static_cast<int>(block / (kXcds * a.prefix_tiles)) * kXcds;
-    const int in_run = static_cast<int>(block - static_cast<long>(run) * a.prefix_tiles), wide = min(kXcds, items - run);
-    const int tile = in_run / wide, item = run + in_run % wide;
-    head = item % a.kv_heads;
-    segment = item / a.kv_heads;
+    tile_of(block, static_cast<long>(a.prefix_segments) * a.kv_heads, a.prefix_tiles, item, tile);
+    head = static_cast<int>(item % a.kv_heads);
+    segment = static_cast<int>(item / a.kv_heads);
     row0 = 32L * tile;
     columns = static_cast<int>(min(32L, a.rows - row0));
     first = segment * a.prefix_keys;
     visible = all_see = end = min(a.shared, first + a.prefix_keys);
   } else {
     block -= a.prefix_blocks;
-    segment = static_cast<int>(block % a.own_segments);
-    block /= a.own_segments;
-    const int tile = static_cast<int>(block % a.own_tiles);
-    block /= a.own_tiles;
-    head = static_cast<int>(block % a.kv_heads);
-    request = static_cast<int>(block / a.kv_heads);
+    tile_of(block, static_cast<long>(a.requests) * a.kv_heads * a.own_segments, a.own_tiles, item, tile);
+    // (segments last: with them first, every eighth block - one XCD's - would be of the segments that short requests do not have)
+    head = static_cast<int>(item % a.kv_heads);
+    item /= a.kv_heads;
+    request = static_cast<int>(item % a.requests);
+    segment = static_cast<int>(item / a.requests);
     const int begin = a.q_start[request], count = a.q_start[request + 1] - begin, length = a.seq_lens[request], before = length - count;
     // (what the host could not see: numbers outside its bounds are left alone here and answered with NaN by the join)
     if (count <= 0 || count > a.max_new || begin < 0 || begin + count > a.tokens || length - a.shared > a.max_own || before < a.shared) return;
@@ -767,7 +791,7 @@ template <typename K> int room_for(K kernel, size_t lds) {
 // `wide`: the prefix goes to `wide_prefix_kernel`, and the requests' own keys alone to the other one, which holds twice as many blocks a
 // unit.
 template <typename T> int run(const Args& all, bool wide, hipStream_t stream) {
-  constexpr size_t lds = narrow_lds(kWaves);
+  constexpr size_t lds = narrow_lds<T>(kWaves);
   Args a = all;
   int status = 0;
   if constexpr (kWideFits && sizeof(T) == 2)

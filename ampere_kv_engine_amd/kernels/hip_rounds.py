@@ -17,22 +17,32 @@ from ..csrc.build import ensure_rounds, ensure_shared_prefix
 _DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1}
 
 
-def _ptr(t):
-    return ctypes.c_void_p(t.data_ptr()) if t is not None else ctypes.c_void_p(0)
+def _address(t):
+    return t.data_ptr() if t is not None else None
 
 
-def wide_tiles(rows: int, head_dim: int, page_size: int, dtype) -> bool:
-    """Whether the prompt's keys are multiplied for tiles of 256 columns that share them (`walk_wide`) rather than of 32."""
-    return dtype == torch.bfloat16 and head_dim in (64, 128) and page_size >= 16 and rows > 32
+def wide_tiles_fit(head_dim: int, page_size: int, dtype) -> bool:
+    """What `wide_prefix_kernel` takes."""
+    return dtype == torch.bfloat16 and head_dim in (64, 128) and page_size >= 16
+
+
+def wide_tiles(rows: int, kv_heads: int, shared: int, units: int) -> bool:
+    """Whether the prompt's keys are multiplied in tiles of 256 columns that share them through LDS (`wide_prefix_kernel`, a launch of its
+    own) rather than of 32 beside the requests' own keys.  The shared ones cost 8 to 10 us more at their start and end and half as much a
+    column and key.  Whole calls, narrow / wide us, 256 units: 32 heads over 8 of 128, 128 own keys, 8,192 shared, 128 rows 26 / 36, 256
+    44 / 50; 32,768 shared, 64 rows 36 / 50, 128 58 / 56, 192 84 / 64, 256 100 / 71; 16 over 4 of 64, 32,768 shared, 128 rows 26 / 30, 192
+    35 / 32, 256 41 / 34."""
+    return rows * kv_heads * shared >= 110_000 * units
 
 
 def cut_own(requests: int, rows: int, kv_heads: int, most: int, units: int) -> tuple[int, int]:
-    """(segments, keys of one) of up to `most` keys that a request of up to `rows` rows a kv head holds behind the prompt: 256 keys, two
-    steps for each of a block's waves, so that a long request's blocks do not outlast the others'; 128 where that leaves units idle; more
-    where the bound is loose, as blocks without keys cost a look at the lengths each."""
+    """(segments, keys of one) of up to `most` keys that a request of up to `rows` rows a kv head holds behind the prompt.  Six blocks a unit:
+    a unit holds two, and what a block waits for at its start and end is a good part of its time; but a long request's keys are not to
+    outlast the others'.  Segments of 128 keys - a step for each of a block's waves - at least.  (64 requests of up to 2,053 keys, 8 kv
+    heads, whole calls, us: segments of 256 keys 84, 512 82, 768 83, 1,024 83; 27 of 2,005: 69, 68, 70, 69, and of 384 65; 64 of 517 with 40
+    rows each: 158, 148, 139, 138.)"""
     blocks = requests * kv_heads * ((rows + 31) // 32)
-    keys = 128 if blocks * ((most + 255) // 256) < units else 256
-    segments = max(1, min((most + keys - 1) // keys, max(1, 16 * units // blocks), 256))
+    segments = max(1, min((most + 127) // 128, 6 * units // blocks, 256))
     keys = ((most + segments - 1) // segments + 127) // 128 * 128
     return (most + keys - 1) // keys, keys
 
@@ -52,14 +62,21 @@ def cut_prefix(columns: int, rows: int, kv_heads: int, shared: int, units: int, 
 class RoundKernels:
     """Mixed into `HipKernels` (which provides `_dense`, `_check`, `_pages`, `_stream`, `device`)."""
 
+    wide_prefix_tiles = None        # a shared prompt's keys for tiles of 256 columns, where heads and pages allow it: None = by the sizes
     _rounds_lib = None
 
     def _rounds(self):
         if self._rounds_lib is None:
-            self._rounds_lib = self._load(ensure_rounds())
-            for name in ("akv_place_tokens", "akv_place_most_requests", "akv_verify_drafts"):
-                getattr(self._rounds_lib, name).restype = ctypes.c_int
-            self._rounds_lib.akv_verify_workspace.restype = ctypes.c_long
+            lib = self._load(ensure_rounds())
+            p, i, n = ctypes.c_void_p, ctypes.c_int, ctypes.c_long      # (with the types known, addresses are handed over as they are)
+            for name, result, types in (
+                    ("akv_place_most_requests", i, ()),
+                    ("akv_place_tokens", i, (p, p, p, p, n, p, p, p, i, i, i, p, i, i, i, p, p, p, p, p, p, p, p, p)),
+                    ("akv_verify_workspace", n, (i, i, i)),
+                    ("akv_verify_drafts", i, (p, i, i, p, p, p, p, i, i, p, n, n, p, p, p, p))):
+                getattr(lib, name).restype, getattr(lib, name).argtypes = result, types
+            self._place_most = lib.akv_place_most_requests()
+            self._rounds_lib = lib
         return self._rounds_lib
 
     def _load(self, path: str):
@@ -77,7 +94,9 @@ class RoundKernels:
         entries = self.__dict__.setdefault("_shared_prefix_entries", {})
         if head_dim not in entries:
             entry = getattr(self._load(ensure_shared_prefix(head_dim)), f"akv_attention_shared_prefix_d{head_dim}")
-            entry.restype = ctypes.c_int
+            p, i, n = ctypes.c_void_p, ctypes.c_int, ctypes.c_long
+            entry.restype = i
+            entry.argtypes = (p, p, p, p, i, p, p, p, p, p, p, i, i, n, i, i, i, n, ctypes.c_float, i, i, i, i, i, i, i, i, p)
             entries[head_dim] = entry
         return entries[head_dim]
 
@@ -85,16 +104,20 @@ class RoundKernels:
         if not isinstance(t, torch.Tensor) or not t.is_cuda or t.get_device() != self.device.index:
             raise self._error(f"{name} must be a tensor on {self.device}, got {getattr(t, 'device', type(t))}")
 
-    def _apart(self, outputs: dict, inputs: dict) -> None:
-        """Refuses outputs that lie in each other or in an input (kernels of several blocks read while others write)."""
-        spans = [(name, t, t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), out)
-                 for out, named in ((True, outputs), (False, inputs)) for name, t in named.items() if t is not None and t.numel()]
-        spans.sort(key=lambda span: span[2])
+    def _apart(self, outputs: tuple, inputs: tuple) -> None:
+        """Refuses outputs - (tensor, name) - that lie in each other or in an input: kernels of several blocks read while others write."""
+        spans = []
+        for named, out in ((outputs, True), (inputs, False)):
+            for t, name in named:
+                if t is not None:
+                    low = t.data_ptr()
+                    spans.append((low, low + t.numel() * t.element_size(), out, name))
+        spans.sort()
         end, of, of_out = 0, None, False
-        for name, _, low, high, out in spans:
-            if low < end and (out or of_out):
+        for low, high, out, name in spans:
+            if low < end and (out or of_out) and high > low:
                 raise self._error(f"{name} and {of} share memory")
-            if high > end or out:
+            if high > end or (out and high > low):
                 end, of, of_out = max(high, end), name, out
 
     # ---- attention -----------------------------------------------------------------------------------------------------
@@ -137,27 +160,28 @@ class RoundKernels:
             raise self._error(f"the scores' scale must be positive and finite, not {scale}")
         if (q.data_ptr() | k_pages.data_ptr() | v_pages.data_ptr() | out.data_ptr()) % 16:
             raise self._error("queries, pages and the output must lie on 16-byte boundaries")
-        self._apart({"out": out}, {"q": q, "k_pages": k_pages, "v_pages": v_pages, "block_table": block_table, "q_start": q_start,
-                                   "seq_lens": seq_lens, "table rows": rows})
+        self._apart(((out, "out"),), ((q, "q"), (k_pages, "k_pages"), (v_pages, "v_pages"), (block_table, "block_table"), (q_start, "q_start"),
+                                      (seq_lens, "seq_lens"), (rows, "table rows")))
         if tokens == 0 or requests == 0:
             return
         if num_pages == 0:
             raise self._error("there are no pages")
         group = q_heads // kv_heads
         max_new_tokens = min(max_new_tokens, tokens)
-        wide = wide_tiles(tokens * group, head_dim, page_size, q.dtype)
+        wide = wide_tiles_fit(head_dim, page_size, q.dtype) and (
+            self.wide_prefix_tiles if self.wide_prefix_tiles is not None else wide_tiles(tokens * group, kv_heads, shared, self.compute_units))
         own_segments, own_keys = cut_own(requests, max_new_tokens * group, kv_heads, max_seq_len - shared, self.compute_units)
         own_blocks = requests * kv_heads * own_segments
         prefix_segments, prefix_keys = cut_prefix(256 if wide else 32, tokens * group, kv_heads, shared, self.compute_units, own_blocks)
         segments = prefix_segments + own_segments
         # (from torch's pool: a recorded call then has room of its own, and calls on other streams do not meet in one)
         room = torch.empty(segments * tokens * q_heads * (head_dim + 2), dtype=torch.float32, device=self.device)
-        sums, stats = room, room[segments * tokens * q_heads * head_dim:]
+        sums = room.data_ptr()
         self._check(self._shared_prefix_entry(head_dim)(
-            _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(out), _DTYPE_CODE[q.dtype], _ptr(sums), _ptr(stats), _ptr(q_start), _ptr(seq_lens),
-            _ptr(block_table), _ptr(rows), block_table.shape[1], requests, ctypes.c_long(tokens), q_heads, kv_heads, page_size,
-            ctypes.c_long(num_pages), ctypes.c_float(scale), shared, max_seq_len - shared, max_new_tokens, prefix_segments, prefix_keys,
-            own_segments, own_keys, int(wide), self._stream()), "attention_shared_prefix")
+            q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), _DTYPE_CODE[q.dtype], sums,
+            sums + 4 * segments * tokens * q_heads * head_dim, q_start.data_ptr(), seq_lens.data_ptr(), block_table.data_ptr(), _address(rows),
+            block_table.shape[1], requests, tokens, q_heads, kv_heads, page_size, num_pages, scale, shared, max_seq_len - shared, max_new_tokens,
+            prefix_segments, prefix_keys, own_segments, own_keys, int(wide), self._stream()), "attention_shared_prefix")
 
     # ---- drafted tokens ------------------------------------------------------------------------------------------------
     def verify_drafts(self, logits, tokens, q_start, temperature, uniforms, kept, chosen, draft_logits=None):
@@ -192,8 +216,8 @@ class RoundKernels:
             strides = draft_logits.stride()[:2]
         elif draft_logits is not None:
             draft_logits = None
-        self._apart({"kept": kept, "chosen": chosen}, {"logits": logits, "tokens": tokens, "q_start": q_start, "temperature": temperature,
-                                                       "uniforms": uniforms})
+        self._apart(((kept, "kept"), (chosen, "chosen")), ((logits, "logits"), (tokens, "tokens"), (q_start, "q_start"),
+                                                           (temperature, "temperature"), (uniforms, "uniforms"), (draft_logits, "draft_logits")))
         if requests == 0:
             return
         lib = self._rounds()
@@ -202,8 +226,9 @@ class RoundKernels:
             raise self._error(f"verify_drafts: {requests} requests of up to {places} rows of {vocab} logits: at most 65,535, 64 and 524,288 are taken")
         workspace = torch.empty(room, dtype=torch.uint8, device=self.device)
         self._check(lib.akv_verify_drafts(
-            _ptr(logits), count, vocab, _ptr(tokens), _ptr(q_start), _ptr(temperature), _ptr(uniforms), requests, places, _ptr(draft_logits),
-            ctypes.c_long(strides[0]), ctypes.c_long(strides[1]), _ptr(kept), _ptr(chosen), _ptr(workspace), self._stream()), "verify_drafts")
+            logits.data_ptr(), count, vocab, tokens.data_ptr(), q_start.data_ptr(), temperature.data_ptr(), uniforms.data_ptr(), requests, places,
+            _address(draft_logits), strides[0], strides[1], kept.data_ptr(), chosen.data_ptr(), workspace.data_ptr(), self._stream()),
+            "verify_drafts")
 
     # ---- a step's layout -----------------------------------------------------------------------------------------------
     def place_tokens(self, lengths, counts, held, free_pages, cursor, table, page_size, q_start, seq_lens, held_after, cursor_after, positions,
@@ -218,29 +243,38 @@ class RoundKernels:
         narrow or that two requests name, -3 more tokens than the maps have room for, -4 a negative number, or fewer pages than a length fills."""
         requests, tokens = lengths.shape[0], positions.shape[0]
         lib = self._rounds()
-        named = dict(lengths=lengths, counts=counts, held=held, q_start=q_start, seq_lens=seq_lens, held_after=held_after, cursor=cursor,
-                     cursor_after=cursor_after, positions=positions, seq_of_token=seq_of_token, slot_map=slot_map, status=status)
-        sizes = dict(q_start=requests + 1, cursor=1, cursor_after=1, status=1, positions=tokens, seq_of_token=tokens, slot_map=tokens)
-        for name, t in named.items():
-            self._dense(t, name, torch.int32, (sizes.get(name, requests),))
-        self._dense(free_pages, "free_pages", torch.int32, (free_pages.shape[0],))
-        self._dense(table, "table", torch.int32)
+        i32, of_requests, of_tokens, dense = torch.int32, (requests,), (tokens,), self._dense
+        dense(lengths, "lengths", i32, of_requests)
+        dense(counts, "counts", i32, of_requests)
+        dense(held, "held", i32, of_requests)
+        dense(free_pages, "free_pages", i32, (free_pages.shape[0],))
+        dense(cursor, "cursor", i32, (1,))
+        dense(table, "table", i32)
+        dense(q_start, "q_start", i32, (requests + 1,))
+        dense(seq_lens, "seq_lens", i32, of_requests)
+        dense(held_after, "held_after", i32, of_requests)
+        dense(cursor_after, "cursor_after", i32, (1,))
+        dense(positions, "positions", i32, of_tokens)
+        dense(seq_of_token, "seq_of_token", i32, of_tokens)
+        dense(slot_map, "slot_map", i32, of_tokens)
+        dense(status, "status", i32, (1,))
         if table.dim() != 2 or (rows is None and table.shape[0] < requests):
             raise self._error(f"table must be a matrix with a row for each of {requests} requests, got {tuple(table.shape)}")
         if rows is not None:
-            self._dense(rows, "table rows", torch.int32, (requests,))
+            dense(rows, "table rows", i32, of_requests)
         if prefix_pages is not None:
-            self._dense(prefix_pages, "prefix_pages", torch.int32, (prefix_pages.shape[0],))
+            dense(prefix_pages, "prefix_pages", i32, (prefix_pages.shape[0],))
         if int(page_size) < 1:
             raise self._error(f"page_size {page_size} must be positive")
-        if requests > lib.akv_place_most_requests():
-            raise self._error(f"{requests} requests in one step; at most {lib.akv_place_most_requests()} are taken")
-        written = ("q_start", "seq_lens", "held_after", "cursor_after", "positions", "seq_of_token", "slot_map", "status")
-        self._apart({**{name: named[name] for name in written}, "table": table},
-                    {"lengths": lengths, "counts": counts, "held": held, "cursor": cursor, "free_pages": free_pages, "table rows": rows,
-                     "prefix_pages": prefix_pages})
+        if requests > self._place_most:
+            raise self._error(f"{requests} requests in one step; at most {self._place_most} are taken")
+        self._apart(((q_start, "q_start"), (seq_lens, "seq_lens"), (held_after, "held_after"), (cursor_after, "cursor_after"),
+                     (positions, "positions"), (seq_of_token, "seq_of_token"), (slot_map, "slot_map"), (status, "status"), (table, "table")),
+                    ((lengths, "lengths"), (counts, "counts"), (held, "held"), (cursor, "cursor"), (free_pages, "free_pages"),
+                     (rows, "table rows"), (prefix_pages, "prefix_pages")))
         self._check(lib.akv_place_tokens(
-            _ptr(lengths), _ptr(counts), _ptr(held), _ptr(free_pages), ctypes.c_long(free_pages.shape[0]), _ptr(cursor), _ptr(table), _ptr(rows),
-            table.shape[0], table.shape[1], int(page_size), _ptr(prefix_pages), prefix_pages.shape[0] if prefix_pages is not None else 0, requests,
-            tokens, _ptr(q_start), _ptr(seq_lens), _ptr(held_after), _ptr(cursor_after), _ptr(positions), _ptr(seq_of_token), _ptr(slot_map),
-            _ptr(status), self._stream()), "place_tokens")
+            lengths.data_ptr(), counts.data_ptr(), held.data_ptr(), free_pages.data_ptr(), free_pages.shape[0], cursor.data_ptr(),
+            table.data_ptr(), _address(rows), table.shape[0], table.shape[1], int(page_size), _address(prefix_pages),
+            prefix_pages.shape[0] if prefix_pages is not None else 0, requests, tokens, q_start.data_ptr(), seq_lens.data_ptr(),
+            held_after.data_ptr(), cursor_after.data_ptr(), positions.data_ptr(), seq_of_token.data_ptr(), slot_map.data_ptr(),
+            status.data_ptr(), self._stream()), "place_tokens")

@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from ampere_kv_engine_amd.kernels.hip_rounds import wide_tiles
+from ampere_kv_engine_amd.kernels.hip_rounds import wide_tiles, wide_tiles_fit
 from plain import rounds_plain
 
 pytestmark = pytest.mark.gpu
@@ -13,9 +13,22 @@ DEV = "cuda:0"
 
 
 @pytest.fixture(scope="module")
-def kernels():
+def kernel_set():
     from ampere_kv_engine_amd.kernels.hip import HipKernels
     return HipKernels(DEV)
+
+
+@pytest.fixture(params=[False, True], ids=["narrow", "wide"])
+def tiled(kernel_set, request):
+    """The kernel set with a prompt's keys for tiles of 32 columns or, where heads and pages allow it, of 256."""
+    kernel_set.wide_prefix_tiles = request.param
+    yield kernel_set
+    kernel_set.wide_prefix_tiles = None
+
+
+@pytest.fixture
+def kernels(kernel_set):
+    return kernel_set
 
 
 def ints(values):
@@ -74,7 +87,7 @@ def attend(kernels, case, **changes):
     return arguments["out"]
 
 
-def within(case, got, rows=None):
+def within(kernels, case, got, rows=None):
     """Every element within what rounding allows.  A score is a sum of `dim` products in 32 bits: off by (dim + 2) 2^-24 of the sum of
     |q||k|, times the scale; a weight's relative error is that, 2^-22 for its power and as much for its reference point's scaling
     (exponents up to some tens, 2^-24 relative each: 2^-18); sums of n weights in order add n 2^-24, bfloat16 weights in two parts 2^-16.
@@ -88,7 +101,10 @@ def within(case, got, rows=None):
     if dtype == torch.bfloat16:
         relative = relative + 2.0 ** -16
     allowed = 2 * relative * weighed * 1.01 + torch.finfo(dtype).eps / 2 * want.abs() * 1.01
-    if wide_tiles(len(case["q"]) * case["heads"] // case["kv_heads"], dim, case["page"], dtype):
+    wide = kernels.wide_prefix_tiles
+    if wide is None:
+        wide = wide_tiles(len(case["q"]) * case["heads"] // case["kv_heads"], case["kv_heads"], case["shared"], kernels.compute_units)
+    if wide and wide_tiles_fit(dim, case["page"], dtype):
         allowed = allowed + 2.0 ** -8 / (1 - 2.0 ** -8) * (weighed + want.abs()) * 1.01
     got = got.double().cpu()
     if rows is not None:
@@ -119,53 +135,53 @@ SHAPES = [
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
 @pytest.mark.parametrize("shape", SHAPES, ids=lambda s: f"h{s[0]}x{s[1]}d{s[2]}p{s[3]}s{s[4]}r{len(s[5])}")
-def test_attention_matches_64_bits(kernels, dtype, shape):
+def test_attention_matches_64_bits(tiled, dtype, shape):
     heads, kv_heads, dim, page, shared, own, counts = shape
     case = batch(dtype, heads, kv_heads, dim, page, shared, own, counts, seed=heads + dim)
     clear_behind(case, math.nan)          # what no token holds is never looked at
-    within(case, attend(kernels, case))
+    within(tiled, case, attend(tiled, case))
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
-def test_attention_finds_rows_of_a_persistent_table(kernels, dtype):
+def test_attention_finds_rows_of_a_persistent_table(tiled, dtype):
     case = batch(dtype, 8, 2, 64, 16, 96, (3, 40, 0), (2, 1, 1), seed=5)
     rows = [4, 0, 2]
     table = torch.full((6, case["table"].shape[1] + 2), -1, dtype=torch.int32)
     for r, row in enumerate(rows):
         table[row, :case["table"].shape[1]] = case["table"][r]
-    within(case, attend(kernels, case, block_table=table.to(DEV), rows=ints(rows), max_seq_len=table.shape[1] * 16, max_new_tokens=9))
+    within(tiled, case, attend(tiled, case, block_table=table.to(DEV), rows=ints(rows), max_seq_len=table.shape[1] * 16, max_new_tokens=9))
 
 
-def test_attention_leaves_rows_behind_the_last_request(kernels):
+def test_attention_leaves_rows_behind_the_last_request(tiled):
     case = batch(torch.bfloat16, 8, 2, 64, 16, 64, (3, 40), (2, 1), seed=6)
     q = torch.cat((case["q"], torch.full((5, 8 * 64), math.nan, dtype=torch.bfloat16)))
-    out = attend(kernels, case, q=q.to(DEV), out=torch.full((8, 512), 7.0, dtype=torch.bfloat16, device=DEV))
-    within(case, out[:3])
+    out = attend(tiled, case, q=q.to(DEV), out=torch.full((8, 512), 7.0, dtype=torch.bfloat16, device=DEV))
+    within(tiled, case, out[:3])
     assert bool((out[3:] == 7.0).all())
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
 @pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
-def test_values_that_are_not_finite_reach_only_who_sees_them(kernels, dtype, value):
+def test_values_that_are_not_finite_reach_only_who_sees_them(tiled, dtype, value):
     """A drafted token's value is not finite: the tokens before it, in the same tile, do not see it."""
     case = batch(dtype, 8, 2, 128, 16, 64, (3, 40), (4, 3), seed=7)
-    finite = attend(kernels, case)
+    finite = attend(tiled, case)
     position = case["lengths"][0] - 2                      # the third of the first request's four tokens
     id = int(case["table"][0, position // 16])
     case["v"][id, 1, 5, position % 16] = value             # one dim of the second kv head
-    got = attend(kernels, case).view(7, 8, 128)
+    got = attend(tiled, case).view(7, 8, 128)
     reached = torch.zeros(7, 8, 128, dtype=torch.bool, device=DEV)
     reached[2:4, 4:, 5] = True
     assert torch.equal(got[~reached], finite.view(7, 8, 128)[~reached])
     assert bool((got[reached].isnan() if math.isnan(value) else got[reached] == value).all())
 
 
-def test_keys_that_are_not_finite_reach_only_who_sees_them(kernels):
+def test_keys_that_are_not_finite_reach_only_who_sees_them(tiled):
     case = batch(torch.bfloat16, 8, 2, 64, 16, 64, (3, 40), (4, 3), seed=8)
-    finite = attend(kernels, case)
+    finite = attend(tiled, case)
     position = case["lengths"][0] - 2
     case["k"][int(case["table"][0, position // 16]), 0, position % 16] = math.nan
-    got = attend(kernels, case).view(7, 8, 64)
+    got = attend(tiled, case).view(7, 8, 64)
     reached = torch.zeros(7, 8, 64, dtype=torch.bool, device=DEV)
     reached[2:4, :4] = True
     assert torch.equal(got[~reached], finite.view(7, 8, 64)[~reached])
@@ -173,39 +189,39 @@ def test_keys_that_are_not_finite_reach_only_who_sees_them(kernels):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
-def test_scores_far_apart(kernels, dtype):
+def test_scores_far_apart(tiled, dtype):
     """Scores of some hundreds: all but one key of a segment, and all but one segment, underflow."""
     case = batch(dtype, 4, 1, 64, 16, 512, (130, 3), (2, 1), seed=9)
     case["q"] *= 40
     case["k"] *= 4
-    within(case, attend(kernels, case))
+    within(tiled, case, attend(tiled, case))
 
 
-def test_what_the_host_cannot_see_is_answered_with_nan(kernels):
+def test_what_the_host_cannot_see_is_answered_with_nan(tiled):
     case = batch(torch.bfloat16, 8, 2, 64, 16, 64, (3, 40, 9, 5), (2, 1, 1, 1), seed=10)
-    good = attend(kernels, case)
-    within(case, good)
+    good = attend(tiled, case)
+    within(tiled, case, good)
     table = case["table"].clone()
     table[0, 4] = case["k"].shape[0]                        # a page outside the pool: the first request's own
-    out = attend(kernels, case, block_table=table.to(DEV))
+    out = attend(tiled, case, block_table=table.to(DEV))
     assert bool(out[:2].isnan().all()) and torch.equal(out[2:], good[2:])
     table = case["table"].clone()
     table[:, 1] = -1                                        # the same in the prompt
-    assert bool(attend(kernels, case, block_table=table.to(DEV)).isnan().all())
-    out = attend(kernels, case, max_seq_len=80)             # the second request is longer than that
+    assert bool(attend(tiled, case, block_table=table.to(DEV)).isnan().all())
+    out = attend(tiled, case, max_seq_len=80)             # the second request is longer than that
     assert bool(out[2].isnan().all()) and torch.equal(out[[0, 1, 3, 4]], good[[0, 1, 3, 4]])
-    out = attend(kernels, case, max_new_tokens=1)
+    out = attend(tiled, case, max_new_tokens=1)
     assert bool(out[:2].isnan().all()) and torch.equal(out[2:], good[2:])
-    out = attend(kernels, case, seq_lens=ints([case["lengths"][0], 64, case["lengths"][2], case["lengths"][3]]))   # within the prompt
+    out = attend(tiled, case, seq_lens=ints([case["lengths"][0], 64, case["lengths"][2], case["lengths"][3]]))   # within the prompt
     assert bool(out[2].isnan().all()) and torch.equal(out[[0, 1, 3, 4]], good[[0, 1, 3, 4]])
 
 
-def test_a_request_gives_the_same_whatever_stands_beside_it(kernels):
+def test_a_request_gives_the_same_whatever_stands_beside_it(tiled):
     """The prompt's product has a column per row of the batch: no column reaches another."""
     case = batch(torch.bfloat16, 8, 2, 128, 16, 640, tuple(range(0, 150, 6)), (1,) * 25, seed=11)
-    good = attend(kernels, case)
+    good = attend(tiled, case)
     case["q"][::2] = math.nan
-    out = attend(kernels, case)
+    out = attend(tiled, case)
     assert torch.equal(out[1::2], good[1::2]) and bool(out[::2].isnan().all())
 
 
@@ -219,8 +235,8 @@ def test_attention_agrees_with_the_engines_own(kernels):
                           host_seq_lens=case["lengths"], max_seq_len=max(case["lengths"]), num_tokens=3)
     meta = SimpleNamespace(block_table=case["table"].to(DEV), width=case["table"].shape[1])
     kernels.attention(q, case["k"].to(DEV), case["v"].to(DEV), ctx, meta, 16, 4, 128, case["scale"], None, other)
-    within(case, attend(kernels, case))
-    within(case, other)
+    within(kernels, case, attend(kernels, case))
+    within(kernels, case, other)
 
 
 # ---- drafted tokens ---------------------------------------------------------------------------------------------------------
@@ -518,8 +534,8 @@ def test_rounds_follow_each_other_on_the_device(kernels, every):
             k[slot // page, :, slot % page] = one["k"][n]
             v[slot // page, :, :, slot % page] = one["v"][n]
         case = dict(q=one["q"], k=k, v=v, table=torch.tensor(table, dtype=torch.int32), starts=placed["q_start"], lengths=placed["seq_lens"],
-                    heads=heads, kv_heads=kv_heads, dim=dim, page=page, scale=dim ** -0.5)
-        within(case, got)
+                    heads=heads, kv_heads=kv_heads, dim=dim, page=page, shared=shared, scale=dim ** -0.5)
+        within(kernels, case, got)
         want = rounds_plain.verify(one["logits"], one["tokens"], placed["q_start"], temperature, one["uniforms"])
         assert got_kept.tolist() == want[0] and got_chosen.tolist() == want[1]
         all_kept += sum(want[0])
