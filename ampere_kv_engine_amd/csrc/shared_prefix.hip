@@ -53,7 +53,7 @@ struct Args {
   const int* seq_lens;        // [requests] tokens held, the new ones among them
   const int* block_table;     // [.., table_width]
   const int* table_rows;      // null, or [requests]: a request's row of the table
-  int table_width, requests;
+  int table_width, table_count, requests;     // (the table has table_count rows)
   long tokens, rows;          // rows = tokens * group: columns of a kv head
   int q_heads, kv_heads, page_shift, shared, max_own, max_new;
   long num_pages;
@@ -64,6 +64,18 @@ struct Args {
   int prefix_tiles, own_tiles;         // tiles of columns: of all rows, of the most rows a request brings
   long prefix_blocks;
 };
+
+// What the host could not see of a request: whether its tokens lie within q, its lengths within the bounds and behind the prompt.  The
+// walks leave other requests alone, and the join answers their tokens with NaN.
+__device__ __forceinline__ bool within_bounds(const Args& a, int begin, int count, int length) {
+  return begin >= 0 && count > 0 && count <= a.max_new && static_cast<long>(begin) + count <= a.tokens && length >= count &&
+         length - count >= a.shared && length - a.shared <= a.max_own;
+}
+// A request's row of the table, or null where there is none.
+__device__ __forceinline__ const int* table_of(const Args& a, int request) {
+  const int row = a.table_rows != nullptr ? a.table_rows[request] : request;
+  return row < 0 || row >= a.table_count ? nullptr : a.block_table + static_cast<size_t>(row) * a.table_width;
+}
 
 // Eight neighbouring elements of an operand: what a lane holds of 16 dims (or keys).
 template <typename T> struct Piece;
@@ -641,12 +653,12 @@ __global__ __launch_bounds__(kWideWaves * kWave, 2) void wide_prefix_kernel(Args
   tile_of(blockIdx.x, static_cast<long>(a.prefix_segments) * a.kv_heads, a.prefix_tiles, item, tile);
   const int head = static_cast<int>(item % a.kv_heads), segment = static_cast<int>(item / a.kv_heads);
   const int first = segment * a.prefix_keys, end = min(a.shared, first + a.prefix_keys);
-  const int* table = a.block_table + (a.table_rows != nullptr ? static_cast<size_t>(a.table_rows[0]) * a.table_width : 0);
+  const int* table = table_of(a, 0);
   // (rows behind the last request's may hold anything, and nobody asks for them)
   const long rows = min(a.rows, static_cast<long>(max(a.q_start[a.requests], 0)) * static_cast<long>(a.group.by));
   const long row0 = static_cast<long>(kWideColumns) * tile;
   __shared__ uint32_t over[kWideWaves];
-  if (row0 >= rows) return;
+  if (row0 >= rows || table == nullptr) return;
   walk_wide(a, table, head, row0, rows, first, end, segment, lds, over);
   for (int w = 0; w < kWideWaves; ++w) {
     if (over[w] == 0u) continue;
@@ -682,8 +694,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 || D > 128 ? 1 : 2)) void
     request = static_cast<int>(item % a.requests);
     segment = static_cast<int>(item / a.requests);
     const int begin = a.q_start[request], count = a.q_start[request + 1] - begin, length = a.seq_lens[request], before = length - count;
-    // (what the host could not see: numbers outside its bounds are left alone here and answered with NaN by the join)
-    if (count <= 0 || count > a.max_new || begin < 0 || begin + count > a.tokens || length - a.shared > a.max_own || before < a.shared) return;
+    if (!within_bounds(a, begin, count, length)) return;
     const int group = static_cast<int>(a.group.by);
     columns = min(32, count * group - 32 * tile);
     if (columns <= 0) return;
@@ -695,8 +706,9 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 || D > 128 ? 1 : 2)) void
     row0 = static_cast<long>(begin) * group + 32 * tile;
     segment += a.prefix_segments;
   }
-  const int row = a.table_rows != nullptr ? a.table_rows[request] : request;
-  walk<T, kWaves>(a, a.block_table + static_cast<size_t>(row) * a.table_width, head, row0, columns, first, end, visible, all_see, segment, lds);
+  const int* table = table_of(a, request);
+  if (table == nullptr) return;
+  walk<T, kWaves>(a, table, head, row0, columns, first, end, visible, all_see, segment, lds);
 }
 
 // A row - (token, query head) - a wave, four of a token a block, or, SHARE, where there are too few rows to fill the device, a block: its
@@ -724,7 +736,8 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Args a) {
   float sum[kEach], total = 0.f;
 #pragma unroll
   for (int e = 0; e < kEach; ++e) sum[e] = 0.f;
-  if (count > a.max_new || length - a.shared > a.max_own || length - count < a.shared) {
+  if (!within_bounds(a, begin, count, length) || token - begin >= count || table_of(a, request) == nullptr ||
+      (a.shared > 0 && table_of(a, 0) == nullptr)) {
     total = NAN;
   } else {
     const int used = a.prefix_segments + (seen - a.shared + a.own_keys - 1) / a.own_keys;
@@ -785,6 +798,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Args a) {
 
 template <typename K> int room_for(K kernel, size_t lds) {
   static_assert(kWideLds <= 160 * 1024 && kWideNarrowLds <= 160 * 1024, "LDS of a compute unit");
+  if (lds <= 64 * 1024) return 0;
   return static_cast<int>(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
 }
 
@@ -825,7 +839,7 @@ template <typename T> int run(const Args& all, bool wide, hipStream_t stream) {
 // floats; segments: prefix_segments of prefix_keys (multiples of 32) cover `shared`, own_segments of own_keys `max_own` keys of a
 // request behind it, at most 512 together.  `wide`: the prompt's columns go in tiles of 256 (`walk_wide`).  Operands lie on 16-byte boundaries.
 extern "C" int AKV_NAME(AKV_HEAD_DIM)(const void* q, const void* k_pages, const void* v_pages, void* out, int dtype, float* sums, float* stats,
-                                      const int* q_start, const int* seq_lens, const int* block_table, const int* table_rows, int table_width,
+                                      const int* q_start, const int* seq_lens, const int* block_table, const int* table_rows, int table_width, int table_count,
                                       int requests, long tokens, int q_heads, int kv_heads, int page_size, long num_pages, float scale,
                                       int shared, int max_own, int max_new, int prefix_segments, int prefix_keys, int own_segments,
                                       int own_keys, int wide, hipStream_t stream) {
@@ -839,7 +853,7 @@ extern "C" int AKV_NAME(AKV_HEAD_DIM)(const void* q, const void* k_pages, const 
   const int group = q_heads / kv_heads;
   a.q = q; a.k_pages = k_pages; a.v_pages = v_pages; a.out = out; a.sums = sums; a.stats = stats;
   a.q_start = q_start; a.seq_lens = seq_lens; a.block_table = block_table; a.table_rows = table_rows;
-  a.table_width = table_width; a.requests = requests; a.tokens = tokens; a.rows = tokens * group;
+  a.table_width = table_width; a.table_count = table_count; a.requests = requests; a.tokens = tokens; a.rows = tokens * group;
   a.q_heads = q_heads; a.kv_heads = kv_heads; a.shared = shared; a.max_own = max_own; a.max_new = max_new;
   a.num_pages = num_pages; a.scale_log2 = scale * kLog2e; a.group = Divider::of(group);
   while ((1 << a.page_shift) < page_size) ++a.page_shift;

@@ -96,7 +96,7 @@ class RoundKernels:
             entry = getattr(self._load(ensure_shared_prefix(head_dim)), f"akv_attention_shared_prefix_d{head_dim}")
             p, i, n = ctypes.c_void_p, ctypes.c_int, ctypes.c_long
             entry.restype = i
-            entry.argtypes = (p, p, p, p, i, p, p, p, p, p, p, i, i, n, i, i, i, n, ctypes.c_float, i, i, i, i, i, i, i, i, p)
+            entry.argtypes = (p, p, p, p, i, p, p, p, p, p, p, i, i, i, n, i, i, i, n, ctypes.c_float, i, i, i, i, i, i, i, i, p)
             entries[head_dim] = entry
         return entries[head_dim]
 
@@ -104,21 +104,32 @@ class RoundKernels:
         if not isinstance(t, torch.Tensor) or not t.is_cuda or t.get_device() != self.device.index:
             raise self._error(f"{name} must be a tensor on {self.device}, got {getattr(t, 'device', type(t))}")
 
-    def _apart(self, outputs: tuple, inputs: tuple) -> None:
-        """Refuses outputs - (tensor, name) - that lie in each other or in an input: kernels of several blocks read while others write."""
-        spans = []
-        for named, out in ((outputs, True), (inputs, False)):
-            for t, name in named:
-                if t is not None:
-                    low = t.data_ptr()
-                    spans.append((low, low + t.numel() * t.element_size(), out, name))
+    def _vectors(self, spans: list, entries) -> list:
+        """Checks int32 vectors - (tensor, name, length, whether it is written) - and adds what memory they take to `spans`.  (One loop with
+        the comparisons in it: a call has fifteen of them and takes the device five microseconds.)"""
+        index, i32 = self.device.index, torch.int32
+        for t, name, count, out in entries:
+            if t.dtype is not i32 or t.get_device() != index or t.dim() != 1 or t.numel() != count or not t.is_contiguous():
+                self._dense(t, name, i32, (count,))
+            low = t.data_ptr()
+            spans.append((low, low + 4 * count, out, name))
+        return spans
+
+    def _apart(self, spans: list) -> None:
+        """Refuses outputs that lie in each other or in an input - `spans` of (begin, end, whether it is written, name) -: kernels of several
+        blocks read while others write."""
         spans.sort()
         end, of, of_out = 0, None, False
         for low, high, out, name in spans:
             if low < end and (out or of_out) and high > low:
                 raise self._error(f"{name} and {of} share memory")
             if high > end or (out and high > low):
-                end, of, of_out = max(high, end), name, out
+                end, of, of_out = (high if high > end else end), name, out
+
+    @staticmethod
+    def _span(t, out: bool, name: str) -> tuple:
+        low = t.data_ptr()
+        return low, low + t.numel() * t.element_size(), out, name
 
     # ---- attention -----------------------------------------------------------------------------------------------------
     def attention_shared_prefix(self, q, k_pages, v_pages, block_table, q_start, seq_lens, shared, q_heads, kv_heads, head_dim, scale, out,
@@ -131,8 +142,8 @@ class RoundKernels:
         more than `max_seq_len` tokens or brings more than `max_new_tokens` (0 is fine, and any number from there on; prompts of
         thousands of tokens are `attention`'s).
         float32 or bfloat16; head sizes as `check_attention_sizes` has them; pages of 8 tokens or more, a power of two.
-        A token gets NaN where its request's table names a page outside the pool, where its request exceeds the bounds, or where it
-        stands within the prompt.  Rows of `out` behind the last request's are left as they are."""
+        A token gets NaN where its request's table (or the first one's, of the prompt) names a page outside the pool or is no row of
+        block_table, where its request exceeds the bounds, or where it stands within the prompt.  Rows of `out` behind the last request's are left as they are."""
         tokens, requests = q.shape[0], seq_lens.shape[0]
         self.check_attention_sizes(q_heads, kv_heads, head_dim, 1)
         if q.dtype not in _DTYPE_CODE:
@@ -142,13 +153,17 @@ class RoundKernels:
         num_pages, page_size = self._pages(k_pages, v_pages, kv_heads, head_dim, q.dtype)
         if page_size < 8 or page_size & (page_size - 1):
             raise self._error(f"pages of {page_size} tokens: attention over a shared prompt takes 8 or more, a power of two")
-        self._dense(q_start, "q_start", torch.int32, (requests + 1,))
-        self._dense(seq_lens, "seq_lens", torch.int32, (requests,))
+        spans = [self._span(out, True, "out"), self._span(q, False, "q"), self._span(k_pages, False, "k_pages"),
+                 self._span(v_pages, False, "v_pages")]
+        entries = [(q_start, "q_start", requests + 1, False), (seq_lens, "seq_lens", requests, False)]
+        if rows is not None:
+            entries.append((rows, "table rows", requests, False))
+        self._vectors(spans, entries)
         self._dense(block_table, "block_table", torch.int32)
         if block_table.dim() != 2 or (rows is None and block_table.shape[0] != requests):
             raise self._error(f"block_table must be [{requests if rows is None else 'rows'}, pages], got {tuple(block_table.shape)}")
-        if rows is not None:
-            self._dense(rows, "table rows", torch.int32, (requests,))
+        spans.append(self._span(block_table, False, "block_table"))
+        self._apart(spans)
         shared, max_seq_len, max_new_tokens = int(shared), int(max_seq_len), int(max_new_tokens)
         if shared < 0 or shared % page_size:
             raise self._error(f"a shared prompt of {shared} tokens is not whole pages of {page_size}")
@@ -160,8 +175,6 @@ class RoundKernels:
             raise self._error(f"the scores' scale must be positive and finite, not {scale}")
         if (q.data_ptr() | k_pages.data_ptr() | v_pages.data_ptr() | out.data_ptr()) % 16:
             raise self._error("queries, pages and the output must lie on 16-byte boundaries")
-        self._apart(((out, "out"),), ((q, "q"), (k_pages, "k_pages"), (v_pages, "v_pages"), (block_table, "block_table"), (q_start, "q_start"),
-                                      (seq_lens, "seq_lens"), (rows, "table rows")))
         if tokens == 0 or requests == 0:
             return
         if num_pages == 0:
@@ -180,7 +193,7 @@ class RoundKernels:
         self._check(self._shared_prefix_entry(head_dim)(
             q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), _DTYPE_CODE[q.dtype], sums,
             sums + 4 * segments * tokens * q_heads * head_dim, q_start.data_ptr(), seq_lens.data_ptr(), block_table.data_ptr(), _address(rows),
-            block_table.shape[1], requests, tokens, q_heads, kv_heads, page_size, num_pages, scale, shared, max_seq_len - shared, max_new_tokens,
+            block_table.shape[1], block_table.shape[0], requests, tokens, q_heads, kv_heads, page_size, num_pages, scale, shared, max_seq_len - shared, max_new_tokens,
             prefix_segments, prefix_keys, own_segments, own_keys, int(wide), self._stream()), "attention_shared_prefix")
 
     # ---- drafted tokens ------------------------------------------------------------------------------------------------
@@ -193,19 +206,19 @@ class RoundKernels:
         draft_logits [requests, places - 1, vocab] float32: what the drafts were drawn from, at the same temperature - any strides, rows
         contiguous; None: drafts that were not drawn (looked up in a text), kept with the target's probability of them.
         kept [requests], chosen [requests, places] int32: the kept drafts, the token that follows, -1 behind it.
-        A request without rows gets 0 and -1.  A row that has no next token - a NaN, nothing above minus infinity, or (where it is
+        A request without rows, or with rows that are not among the logits, gets 0 and -1; rows beyond `places` are not looked at.  A row that has no next token - a NaN, nothing above minus infinity, or (where it is
         drawn from) plus infinity, in the target's or the draft's - ends the walk with -1 as the token.  A draft that is no id of the
         vocabulary is not kept."""
         if logits.dim() != 2 or uniforms.dim() != 2:
             raise self._error("logits and uniforms must be matrices")
         (count, vocab), (requests, places) = logits.shape, uniforms.shape
         self._dense(logits, "logits", torch.float32)
-        self._dense(tokens, "tokens", torch.int32, (count,))
-        self._dense(q_start, "q_start", torch.int32, (requests + 1,))
+        spans = self._vectors([], ((tokens, "tokens", count, False), (q_start, "q_start", requests + 1, False), (kept, "kept", requests, True)))
         self._dense(temperature, "temperature", torch.float32, (requests,))
         self._dense(uniforms, "uniforms", torch.float32)
-        self._dense(kept, "kept", torch.int32, (requests,))
         self._dense(chosen, "chosen", torch.int32, (requests, places))
+        spans += [self._span(chosen, True, "chosen"), self._span(logits, False, "logits"), self._span(temperature, False, "temperature"),
+                  self._span(uniforms, False, "uniforms")]
         strides = (0, 0)
         if draft_logits is not None and places > 1:
             self._placed(draft_logits, "draft_logits")
@@ -216,8 +229,11 @@ class RoundKernels:
             strides = draft_logits.stride()[:2]
         elif draft_logits is not None:
             draft_logits = None
-        self._apart(((kept, "kept"), (chosen, "chosen")), ((logits, "logits"), (tokens, "tokens"), (q_start, "q_start"),
-                                                           (temperature, "temperature"), (uniforms, "uniforms"), (draft_logits, "draft_logits")))
+        if draft_logits is not None:      # (any strides: from its first element to its last)
+            low = draft_logits.data_ptr()
+            last = sum((n - 1) * stride for n, stride in zip(draft_logits.shape, draft_logits.stride())) if draft_logits.numel() else -1
+            spans.append((low, low + 4 * (last + 1), False, "draft_logits"))
+        self._apart(spans)
         if requests == 0:
             return
         lib = self._rounds()
@@ -243,35 +259,25 @@ class RoundKernels:
         narrow or that two requests name, -3 more tokens than the maps have room for, -4 a negative number, or fewer pages than a length fills."""
         requests, tokens = lengths.shape[0], positions.shape[0]
         lib = self._rounds()
-        i32, of_requests, of_tokens, dense = torch.int32, (requests,), (tokens,), self._dense
-        dense(lengths, "lengths", i32, of_requests)
-        dense(counts, "counts", i32, of_requests)
-        dense(held, "held", i32, of_requests)
-        dense(free_pages, "free_pages", i32, (free_pages.shape[0],))
-        dense(cursor, "cursor", i32, (1,))
-        dense(table, "table", i32)
-        dense(q_start, "q_start", i32, (requests + 1,))
-        dense(seq_lens, "seq_lens", i32, of_requests)
-        dense(held_after, "held_after", i32, of_requests)
-        dense(cursor_after, "cursor_after", i32, (1,))
-        dense(positions, "positions", i32, of_tokens)
-        dense(seq_of_token, "seq_of_token", i32, of_tokens)
-        dense(slot_map, "slot_map", i32, of_tokens)
-        dense(status, "status", i32, (1,))
+        entries = [(lengths, "lengths", requests, False), (counts, "counts", requests, False), (held, "held", requests, False),
+                   (free_pages, "free_pages", free_pages.shape[0], False), (cursor, "cursor", 1, False), (q_start, "q_start", requests + 1, True),
+                   (seq_lens, "seq_lens", requests, True), (held_after, "held_after", requests, True), (cursor_after, "cursor_after", 1, True),
+                   (positions, "positions", tokens, True), (seq_of_token, "seq_of_token", tokens, True), (slot_map, "slot_map", tokens, True),
+                   (status, "status", 1, True)]
+        if rows is not None:
+            entries.append((rows, "table rows", requests, False))
+        if prefix_pages is not None:
+            entries.append((prefix_pages, "prefix_pages", prefix_pages.shape[0], False))
+        spans = self._vectors([], entries)
+        self._dense(table, "table", torch.int32)
         if table.dim() != 2 or (rows is None and table.shape[0] < requests):
             raise self._error(f"table must be a matrix with a row for each of {requests} requests, got {tuple(table.shape)}")
-        if rows is not None:
-            dense(rows, "table rows", i32, of_requests)
-        if prefix_pages is not None:
-            dense(prefix_pages, "prefix_pages", i32, (prefix_pages.shape[0],))
-        if int(page_size) < 1:
-            raise self._error(f"page_size {page_size} must be positive")
+        spans.append(self._span(table, True, "table"))
+        if page_size < 1 or page_size != int(page_size):
+            raise self._error(f"page_size {page_size} must be a positive number of tokens")
         if requests > self._place_most:
             raise self._error(f"{requests} requests in one step; at most {self._place_most} are taken")
-        self._apart(((q_start, "q_start"), (seq_lens, "seq_lens"), (held_after, "held_after"), (cursor_after, "cursor_after"),
-                     (positions, "positions"), (seq_of_token, "seq_of_token"), (slot_map, "slot_map"), (status, "status"), (table, "table")),
-                    ((lengths, "lengths"), (counts, "counts"), (held, "held"), (cursor, "cursor"), (free_pages, "free_pages"),
-                     (rows, "table rows"), (prefix_pages, "prefix_pages")))
+        self._apart(spans)
         self._check(lib.akv_place_tokens(
             lengths.data_ptr(), counts.data_ptr(), held.data_ptr(), free_pages.data_ptr(), free_pages.shape[0], cursor.data_ptr(),
             table.data_ptr(), _address(rows), table.shape[0], table.shape[1], int(page_size), _address(prefix_pages),

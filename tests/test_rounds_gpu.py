@@ -210,6 +210,11 @@ def test_what_the_host_cannot_see_is_answered_with_nan(tiled):
     assert bool(attend(tiled, case, block_table=table.to(DEV)).isnan().all())
     out = attend(tiled, case, max_seq_len=80)             # the second request is longer than that
     assert bool(out[2].isnan().all()) and torch.equal(out[[0, 1, 3, 4]], good[[0, 1, 3, 4]])
+    out = attend(tiled, case, rows=ints([0, 1, 4, 3]))      # a row that the table does not have
+    assert bool(out[3].isnan().all()) and torch.equal(out[[0, 1, 2, 4]], good[[0, 1, 2, 4]])
+    assert bool(attend(tiled, case, rows=ints([-1, 1, 2, 3])).isnan().all())        # the prompt is read from the first
+    out = attend(tiled, case, q_start=ints([0, 2, 3, 4, 9]))                        # more tokens than there are
+    assert bool(out[4].isnan().all()) and torch.equal(out[:4], good[:4])
     out = attend(tiled, case, max_new_tokens=1)
     assert bool(out[:2].isnan().all()) and torch.equal(out[2:], good[2:])
     out = attend(tiled, case, seq_lens=ints([case["lengths"][0], 64, case["lengths"][2], case["lengths"][3]]))   # within the prompt
