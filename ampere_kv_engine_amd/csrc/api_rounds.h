@@ -8,6 +8,10 @@
 
 extern "C" {
 
+// -(1000 + 64 i + j): spans i and j overlap, of which i is written (see `shared_spans` in common.h); the spans' order stands at each entry.
+// (For checks: the same for any spans.)
+int akv_shared_spans(const void* const* begins, const long* bytes, int written, int count);
+
 // The most requests `akv_place_tokens` takes.
 int akv_place_most_requests();
 int akv_place_tokens(const int* lengths, const int* counts, const int* held, const int* free_pages, long free_count,

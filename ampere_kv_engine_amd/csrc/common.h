@@ -152,6 +152,23 @@ struct Divider {
 
 namespace akv {
 
+// Memory that a call reads or writes.  Kernels of several blocks read while others write, so what is written may lie neither in
+// anything else that is written nor in what is read: 0, or -(1000 + 64 i + j) for the spans i and j > i that overlap; the first `written`
+// of `count` are written.
+struct Span {
+  const void* begin;
+  long bytes;
+};
+inline int shared_spans(const Span* spans, int written, int count) {
+  for (int i = 0; i < written; ++i)
+    for (int j = i + 1; j < count; ++j) {
+      const char *a = static_cast<const char*>(spans[i].begin), *b = static_cast<const char*>(spans[j].begin);
+      if (a == nullptr || b == nullptr || spans[i].bytes <= 0 || spans[j].bytes <= 0) continue;
+      if (a < b + spans[j].bytes && b < a + spans[i].bytes) return -(1000 + 64 * i + j);
+    }
+  return 0;
+}
+
 // What the host needs to know of the device it launches on to cut work into blocks: asked of the runtime once per
 // device.  (The number of XCDs is not among a device's attributes: gfx950 parts have 8, each with an L2 of its own.)
 struct DeviceFacts {

@@ -167,6 +167,13 @@ __global__ __launch_bounds__(kThreads) void place_kernel(Place p) {
 
 }  // namespace
 
+extern "C" int akv_shared_spans(const void* const* begins, const long* bytes, int written, int count) {
+  Span spans[64];
+  if (count < 0 || count > 64) return -2;
+  for (int i = 0; i < count; ++i) spans[i] = Span{begins[i], bytes[i]};
+  return shared_spans(spans, written, count);
+}
+
 extern "C" int akv_place_most_requests() { return kMost; }
 
 // `status` [1]: the pages taken, or why nothing but `status` was written: -1 too few free pages, -2 a request's row is not in the
@@ -179,6 +186,13 @@ extern "C" int akv_place_tokens(const int* lengths, const int* counts, const int
                                 int* held_after, int* cursor_after, int* positions, int* seq_of_token, int* slot_map, int* status,
                                 hipStream_t stream) {
   if (requests < 0 || requests > kMost || tokens < 0 || page_size <= 0 || table_width < 0 || table_rows < 0 || prefix_count < 0) return -2;
+  const long of_requests = 4L * requests, of_tokens = 4L * tokens;
+  const Span spans[] = {{q_start, of_requests + 4}, {seq_lens, of_requests}, {held_after, of_requests}, {cursor_after, 4}, {positions, of_tokens},
+                        {seq_of_token, of_tokens}, {slot_map, of_tokens}, {status, 4}, {table, 4L * table_rows * table_width},
+                        {lengths, of_requests}, {counts, of_requests}, {held, of_requests}, {cursor, 4}, {free_pages, 4 * free_count},
+                        {rows, of_requests}, {prefix_pages, 4L * prefix_count}};
+  const int shared = shared_spans(spans, 9, 16);
+  if (shared != 0) return shared;
   int places = kWave;
   while (places < 2 * requests) places *= 2;
   const Place p{lengths, counts, held, free_pages, cursor, rows, prefix_pages, table, q_start, seq_lens, held_after, cursor_after,

@@ -849,6 +849,11 @@ extern "C" int AKV_NAME(AKV_HEAD_DIM)(const void* q, const void* k_pages, const 
       static_cast<long>(prefix_segments) * prefix_keys < shared || static_cast<long>(own_segments) * own_keys < max_own ||
       (static_cast<long>(shared) + max_own + page_size - 1) / page_size > table_width)
     return -2;
+  const long size = dtype == kF32 ? 4 : 2, of_q = tokens * q_heads * D * size, of_pages = num_pages * kv_heads * page_size * D * size;
+  const Span spans[] = {{out, of_q}, {q, of_q}, {k_pages, of_pages}, {v_pages, of_pages}, {block_table, 4L * table_width * table_count},
+                        {q_start, 4L * requests + 4}, {seq_lens, 4L * requests}, {table_rows, 4L * requests}};
+  const int overlap = shared_spans(spans, 1, 8);
+  if (overlap != 0) return overlap;
   Args a{};
   const int group = q_heads / kv_heads;
   a.q = q; a.k_pages = k_pages; a.v_pages = v_pages; a.out = out; a.sums = sums; a.stats = stats;

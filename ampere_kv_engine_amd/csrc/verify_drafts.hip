@@ -7,12 +7,16 @@
 //   id whose cumulative weight exceeds u_last times the whole, or the last id of any weight
 //   t <= 0: a draft is kept where it is the target's largest logit (ties: the lowest id), and the next token is the largest
 //
-// The rows are read once, a block a part of kPart logits held in registers (`parts_kernel`: the part's largest, and its sum of
-// exponentials below that).  A second launch (`choose_kernel`) decides - every block of a request for itself, from the parts' few
+// The rows are read once, a block two parts of kPart logits held in registers (`parts_kernel`: the largest, and each part's sum of
+// exponentials below it).  A second launch (`choose_kernel`) decides - every block of a request for itself, from the parts' few
 // numbers -, sums the weights of its part of the row that is drawn from, and the request's last block finds the part and the id.
 // Everything that is compared with a random number is summed in 64 bits: the draw looks for a place among up to 151,936 cumulative
 // weights, and sums in 32 bits, off by 1e-7, would choose another id for one draw in thirty; off by 1e-13, for none.  The vector units
-// have 64-bit products at the rate of 32-bit ones, and 2^f of a reduced argument is a polynomial of ten of them.
+// have 64-bit products at the rate of 32-bit ones, so that the exponentials cost nine operations each and not much more time than
+// the reads: 64 requests of five rows and four draft rows of 151,936 logits (350 MB) take 73 us, 4.8 TB/s of the 6.2 that plain reads
+// reach, and the second launch, which reads two rows of each request again (78 MB), 29 us; a single request 5.7 and 6.3 us, which are a
+// launch's way to the first data and back.  Two parts a block: with one the first launch takes 78 us (its ends are paid twice as often),
+// while parts of twice the size cost the second launch 17 us more, since one block ends with a whole part.
 
 #include "common.h"
 #include "api_rounds.h"
@@ -22,11 +26,11 @@ using namespace akv;
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kLoads = 8;                            // 16-byte pieces a thread
 constexpr int kChooseThreads = 512;
-constexpr int kPart = kThreads * kLoads * 4;         // logits a block
+constexpr int kPart = 4096;                          // logits a part
+constexpr int kPerBlock = 2;                         // parts a block of the first launch
 constexpr int kMostPlaces = 64;                      // rows a request
-constexpr int kMostParts = 64;
+constexpr int kMostParts = 64;                       // a lane each
 
 // What a part of a row leaves.
 struct Part {
@@ -69,35 +73,70 @@ __device__ __forceinline__ double exp_of(double z) {
   return ldexp(v, static_cast<int>(k));
 }
 
-// The same for what is done to whole rows: 2^(z / 32) of z rounded to a whole number k is one of 32 powers (`powers`: in LDS, a bank
-// pair each, so that lanes do not wait for each other), shifted; the rest, at most 1/64 of a power, a polynomial of degree 5 (off by
-// 2e-15).  Rounding is an addition of 1.5 * 2^52, whose lowest bits are k.  A logit is held above -690 t below the row's largest
-// (weights of 1e-299).
+// e^((x - offset) / t) for what is done to whole rows, in nine operations of 64 bits.  In units of 1/32 of a power of two the exponent is
+// x by + B, by = 32 log2(e) / t, B = -offset by.  B's whole part goes into the number that rounds: adding C = 1.5 * 2^52 + rint(B) to
+// x by leaves the whole number k in the sum's lowest bits, and x by - (that - C) is the rest f, |f| <= 1/2, exactly - a fused product
+// rounds once.  2^(k / 32) is one of 32 powers (`powers`: in LDS, a bank pair each, so that lanes do not wait for each other) with k's upper
+// bits added to its exponent; the entries' exponents have k's lower five bits subtracted, so that k is added whole.  2^(f / 32) is
+// a polynomial of degree 4, the series to the fifth with its last term spread over the others by the fifth Chebyshev polynomial (off by
+// 8e-14).  With an offset that makes B whole that is all; what another one leaves is a factor, `rest`.  A logit is held above 680 t
+// below the row's largest, rounded towards the largest (the next float may be half as far away: weights of 1e-147 and less, and whatever
+// is less than kLeast counts as nothing where an id is picked).  Where that is the largest itself, the next float below it
+// is more than 680 t away and only logits equal to it have any weight: `near` is false, and the logits are replaced
+// by 0, the largest, and minus infinity.
 constexpr int kPowers = 32;
+constexpr double kMagic = 6755399441055744.0;
+constexpr double kLeast = 1e-130;
+constexpr float kWarmest = 1e28f;        // temperatures above it are taken as it: 680 t stays below the steps of the largest floats
 struct Scale {
-  double by, top;      // 32 log2(e) / t; the (possibly none's) logit whose weight is 1
+  double by, shift, origin;
   float lowest;
+  bool near;
 };
-__device__ __forceinline__ Scale scale_of(float t, float top) {
-  return Scale{kPowers * 1.4426950408889634074 / static_cast<double>(t), static_cast<double>(top), fmaxf(top - 690.f * t, -3.4e38f)};
+// `inverse` = 1 / t, a division that a block does once.  The offset is the one next to the largest logit for which B is whole.
+__device__ __forceinline__ Scale scale_of(float t, double inverse, float top) {
+  Scale s{kPowers * 1.4426950408889634074 * inverse, kMagic, 0.0, 0.f, true};
+  const double deepest = static_cast<double>(top) - 680.0 * t;
+  s.lowest = static_cast<float>(deepest);
+  if (static_cast<double>(s.lowest) < deepest) s.lowest = nextafterf(s.lowest, INFINITY);
+  s.near = s.lowest < top;
+  if (s.near) s.origin = static_cast<double>(top);
+  else s.lowest = -680.f * t;
+  s.shift += rint(-s.origin * s.by);
+  return s;
 }
-__device__ __forceinline__ void fill_powers(double* powers) {
-  if (threadIdx.x < kPowers) powers[threadIdx.x] = exp2(threadIdx.x * (1.0 / kPowers));
+// The offset `above` beyond the largest logit.
+__device__ __forceinline__ Scale scale_of(float t, double inverse, float top, double above, double& rest) {
+  Scale s = scale_of(t, inverse, top);
+  const double offset = s.origin + above;
+  const double b = -offset * s.by, lost = fma(-offset, s.by, -b), whole = rint(b);
+  rest = exp2(((b - whole) + lost) * (1.0 / kPowers));
+  s.shift = kMagic + whole;
+  return s;
 }
-// `v` times 2^(a whole power / 32) is e^((x - top) / t)
+template <int COUNT> __device__ __forceinline__ void only_largest(float (&v)[COUNT], float top) {
+#pragma unroll
+  for (int e = 0; e < COUNT; ++e) v[e] = v[e] == top ? 0.f : -INFINITY;
+}
+// (by a block's first 32 threads; `factor`: every weight's)
+__device__ __forceinline__ void fill_powers(double* powers, double factor) {
+  if (threadIdx.x < kPowers) {
+    const double power = exp2(threadIdx.x * (1.0 / kPowers)) * factor;
+    powers[threadIdx.x] = __hiloint2double(__double2hiint(power) - (static_cast<int>(threadIdx.x) << 15), __double2loint(power));
+  }
+}
 __device__ __forceinline__ double split_exp(float x, const Scale& s, const double* powers, double& power) {
-  constexpr double kMagic = 6755399441055744.0, kStep = 0.69314718055994530942 / kPowers;
-  const double d = static_cast<double>(fmaxf(x, s.lowest)) - s.top;
-  const double rounded = fma(d, s.by, kMagic);
+  constexpr double kStep = 0.69314718055994530942 / kPowers, kReach = kStep / 2;
+  const double wide = static_cast<double>(fmaxf(x, s.lowest));
+  const double rounded = fma(wide, s.by, s.shift);
   const int k = __double2loint(rounded);
-  const double f = fma(d, s.by, -(rounded - kMagic));
-  double v = kStep * kStep * kStep * kStep * kStep / 120.0;
-  v = fma(v, f, kStep * kStep * kStep * kStep / 24.0);
-  v = fma(v, f, kStep * kStep * kStep / 6.0);
+  const double f = fma(wide, s.by, -(rounded - s.shift));
+  double v = kStep * kStep * kStep * kStep / 24.0;
+  v = fma(v, f, kStep * kStep * kStep * (1.0 / 6.0 + kReach * kReach * 20.0 / (16.0 * 120.0)));
   v = fma(v, f, kStep * kStep / 2.0);
-  v = fma(v, f, kStep);
+  v = fma(v, f, kStep * (1.0 - kReach * kReach * kReach * kReach * 5.0 / (16.0 * 120.0)));
   power = powers[k & (kPowers - 1)];
-  power = __hiloint2double(__double2hiint(power) + ((k >> 5) << 20), __double2loint(power));
+  power = __hiloint2double(__double2hiint(power) + (k << 15), __double2loint(power));
   return fma(v, f, 1.0);
 }
 __device__ __forceinline__ double add_exp(double sum, float x, const Scale& s, const double* powers) {
@@ -165,20 +204,20 @@ __device__ __forceinline__ int wave_lowest(int v) {
   return __builtin_amdgcn_readlane(v, kWave - 1);
 }
 
-// Part `part` of a row in a block's registers: piece u of a thread is x[part * kPart + 4 (u * threads + thread) ..], ids beyond the row minus
-// infinity.  `whole`: rows of whole 16-byte pieces on 16-byte boundaries.
-template <int THREADS>
-__device__ __forceinline__ void fetch_part(const float* x, int vocab, int part, bool whole, float (&v)[kPart / 4 / THREADS][4]) {
-  constexpr int kLoads = kPart / 4 / THREADS, kThreads = THREADS;
-  const int first = part * kPart + 4 * threadIdx.x;
+// IDS ids of a row from `begin` on in a block's registers: piece u of a thread is x[begin + 4 (u * threads + thread) ..], ids beyond the
+// row minus infinity.  `whole`: rows of whole 16-byte pieces on 16-byte boundaries.
+template <int THREADS, int IDS>
+__device__ __forceinline__ void fetch_run(const float* x, int vocab, int begin, bool whole, float (&v)[IDS / 4 / THREADS][4]) {
+  constexpr int kLoads = IDS / 4 / THREADS;
+  const int first = begin + 4 * threadIdx.x;
   if (whole) {
     float4 fetched[kLoads];
 #pragma unroll
-    for (int u = 0; u < kLoads; ++u) fetched[u] = *reinterpret_cast<const float4*>(x + min(first + u * kThreads * 4, vocab - 4));
+    for (int u = 0; u < kLoads; ++u) fetched[u] = *reinterpret_cast<const float4*>(x + min(first + u * THREADS * 4, vocab - 4));
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int u = 0; u < kLoads; ++u) {
-      const bool inside = first + u * kThreads * 4 < vocab;
+      const bool inside = first + u * THREADS * 4 < vocab;
       v[u][0] = inside ? fetched[u].x : -INFINITY;
       v[u][1] = inside ? fetched[u].y : -INFINITY;
       v[u][2] = inside ? fetched[u].z : -INFINITY;
@@ -188,13 +227,13 @@ __device__ __forceinline__ void fetch_part(const float* x, int vocab, int part, 
 #pragma unroll
     for (int u = 0; u < kLoads; ++u)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[u][j] = x[min(first + u * kThreads * 4 + j, vocab - 1)];
+      for (int j = 0; j < 4; ++j) v[u][j] = x[min(first + u * THREADS * 4 + j, vocab - 1)];
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int u = 0; u < kLoads; ++u)
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (first + u * kThreads * 4 + j >= vocab) v[u][j] = -INFINITY;
+        if (first + u * THREADS * 4 + j >= vocab) v[u][j] = -INFINITY;
   }
 }
 
@@ -210,78 +249,99 @@ __device__ __forceinline__ int rows_of(const Verify& a, int request, int& first)
   return max(0, min(end - first, a.places));
 }
 
-// grid (parts, 2 * places - 1, requests): rows 0 .. places - 1 are the target's, the others the draft's
+__device__ __forceinline__ float temperature_of(const Verify& a, int request) {
+  const float t = a.temperature[request];
+  return t > kWarmest ? kWarmest : t;
+}
+
+// grid (blocks a row, 2 * places - 1, requests): rows 0 .. places - 1 are the target's, the others the draft's.  A block takes
+// kPerBlock parts at once, and its waves do not wait for each other until the end.
 __global__ __launch_bounds__(kThreads) void parts_kernel(Verify a) {
-  const int part = blockIdx.x, request = blockIdx.z;
+  constexpr int kWaves = kThreads / kWave, kPieces = kPart / 4 / kThreads;        // 16-byte pieces of a part a thread
+  __shared__ Part of_waves[kPerBlock][kWaves];
+  __shared__ double offsets[kPerBlock][kWaves];
+  __shared__ double powers[kPowers];
+  const int request = blockIdx.z, lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   const bool target = static_cast<int>(blockIdx.y) < a.places;
   const int place = target ? blockIdx.y : blockIdx.y - a.places;
-  if (part == 0 && blockIdx.y == 0 && threadIdx.x == 0)
+  const int begin = blockIdx.x * kPerBlock;
+  if (begin == 0 && blockIdx.y == 0 && threadIdx.x == 0)
     __hip_atomic_store(a.arrivals + request, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);     // for the launch behind this one
   int first;
   const int rows = rows_of(a, request, first);
-  const float t = a.temperature[request];
+  const float t = temperature_of(a, request);
   const bool drawn = t > 0.f;
   if (place >= (target ? rows : rows - 1) || (!target && !drawn)) return;
   const float* x = target ? a.logits + static_cast<size_t>(first + place) * a.vocab
                           : a.draft + request * a.draft_request + place * a.draft_place;
-  float v[kLoads][4];
-  fetch_part<kThreads>(x, a.vocab, part, whole_pieces(a, x), v);
-  __shared__ Part of_waves[kThreads / kWave];
-  __shared__ double powers[kPowers];
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  if (drawn) fill_powers(powers);
+  float v[kPerBlock * kPieces][4];
+  fetch_run<kThreads, kPerBlock * kPart>(x, a.vocab, begin * kPart, whole_pieces(a, x), v);
+  if (drawn) fill_powers(powers, 1.0);
+  const double inverse = 1.0 / static_cast<double>(t);
   __syncthreads();
   float top = -INFINITY;
   bool nan = false;
 #pragma unroll
-  for (int u = 0; u < kLoads; ++u)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      nan |= v[u][j] != v[u][j];
-      top = fmaxf(top, v[u][j]);
-    }
+  for (int u = 0; u < kPerBlock * kPieces; ++u) {
+    nan |= __builtin_isunordered(v[u][0], v[u][1]) || __builtin_isunordered(v[u][2], v[u][3]);
+    top = fmaxf(fmaxf(fmaxf(top, v[u][0]), v[u][1]), fmaxf(v[u][2], v[u][3]));
+  }
   top = wave_top(top);
   nan = __any(nan);
+  double sums[kPerBlock] = {}, offset = static_cast<double>(top);
   int best = 0x7fffffff;
-  double sum = 0.0;
   if (!drawn) {
 #pragma unroll
-    for (int u = kLoads - 1; u >= 0; --u)
+    for (int u = kPerBlock * kPieces - 1; u >= 0; --u)
 #pragma unroll
       for (int j = 3; j >= 0; --j)
-        if (v[u][j] == top) best = part * kPart + u * kThreads * 4 + 4 * static_cast<int>(threadIdx.x) + j;
+        if (v[u][j] == top) best = begin * kPart + (u * kThreads + static_cast<int>(threadIdx.x)) * 4 + j;
     best = wave_lowest(best);
   } else if (top > -INFINITY && top < INFINITY && !nan) {
-    const Scale scale = scale_of(t, top);
-    double other = 0.0;                // (two sums: an addition does not wait for the one before it)
+    const Scale scale = scale_of(t, inverse, top);
+    if (scale.near) {
+      offset = -(scale.shift - kMagic) * (t * (0.69314718055994530942 / kPowers));
+    } else {
 #pragma unroll
-    for (int u = 0; u < kLoads; ++u) {
-      sum = add_exp(sum, v[u][0], scale, powers);
-      other = add_exp(other, v[u][1], scale, powers);
-      sum = add_exp(sum, v[u][2], scale, powers);
-      other = add_exp(other, v[u][3], scale, powers);
+      for (int u = 0; u < kPerBlock * kPieces; ++u) only_largest(v[u], top);
     }
-    sum = wave_sum64(sum + other);
+#pragma unroll
+    for (int i = 0; i < kPerBlock; ++i) {
+      double sum = 0.0, other = 0.0;     // (two sums: an addition does not wait for the one before it)
+#pragma unroll
+      for (int u = i * kPieces; u < (i + 1) * kPieces; ++u) {
+        sum = add_exp(sum, v[u][0], scale, powers);
+        other = add_exp(other, v[u][1], scale, powers);
+        sum = add_exp(sum, v[u][2], scale, powers);
+        other = add_exp(other, v[u][3], scale, powers);
+      }
+      sums[i] = wave_sum64(sum + other);
+    }
   }
-  if (lane == 0) of_waves[wave] = Part{sum, top, best, nan ? 1 : 0, 0};
+  if (lane == 0)
+#pragma unroll
+    for (int i = 0; i < kPerBlock; ++i) {
+      of_waves[i][wave] = Part{sums[i], top, best, nan ? 1 : 0, 0};
+      offsets[i][wave] = offset;
+    }
   __syncthreads();
-  if (threadIdx.x == 0) {
-    Part whole = of_waves[0];
+  const int mine = static_cast<int>(threadIdx.x);
+  if (mine < kPerBlock && begin + mine < a.part_count) {
+    Part joined = of_waves[mine][0];
 #pragma unroll
-    for (int w = 1; w < kThreads / kWave; ++w) {
-      const Part one = of_waves[w];
-      whole.nan |= one.nan;
-      if (one.top > whole.top || (one.top == whole.top && one.best < whole.best)) { whole.top = one.top; whole.best = one.best; }
+    for (int w = 1; w < kWaves; ++w) {
+      const Part one = of_waves[mine][w];
+      joined.nan |= one.nan;
+      if (one.top > joined.top || (one.top == joined.top && one.best < joined.best)) { joined.top = one.top; joined.best = one.best; }
     }
-    whole.sum = 0.0;
-    if (drawn && whole.top > -INFINITY && whole.top < INFINITY) {
-      const double inverse = 1.0 / static_cast<double>(t), highest = static_cast<double>(whole.top);
+    joined.sum = 0.0;
+    if (drawn && joined.top > -INFINITY && joined.top < INFINITY) {
 #pragma unroll
-      for (int w = 0; w < kThreads / kWave; ++w)
-        if (of_waves[w].top > -INFINITY)
-          whole.sum += of_waves[w].sum * exp_of((static_cast<double>(of_waves[w].top) - highest) * inverse);
+      for (int w = 0; w < kWaves; ++w)
+        if (of_waves[mine][w].top > -INFINITY)
+          joined.sum += of_waves[mine][w].sum * exp_of((offsets[mine][w] - static_cast<double>(joined.top)) * inverse);
     }
-    a.parts[(static_cast<size_t>(request) * (2 * a.places - 1) + blockIdx.y) * a.part_count + part] = whole;
+    a.parts[(static_cast<size_t>(request) * (2 * a.places - 1) + blockIdx.y) * a.part_count + begin + mine] = joined;
   }
 }
 
@@ -307,19 +367,18 @@ __global__ __launch_bounds__(kChooseThreads) void choose_kernel(Verify a) {
   constexpr int kThreads = kChooseThreads, kWaves = kThreads / kWave, kLoads = kPart / 4 / kThreads;
   __shared__ Row target[kMostPlaces], draft[kMostPlaces];
   __shared__ unsigned char fine[kMostPlaces];
-  __shared__ double sums[kWaves], powers[kPowers];
+  __shared__ double sums[kWaves], powers[kPowers], draft_powers[kPowers];
   __shared__ int of_waves[kWaves];
   __shared__ int is_last;
   const int block = blockIdx.x, request = blockIdx.y, tid = threadIdx.x;
   const int lane = tid & (kWave - 1), wave = tid / kWave;
   int first;
   const int rows = rows_of(a, request, first);
-  const float t = a.temperature[request];
+  const float t = temperature_of(a, request);
   const bool drawn = t > 0.f;
   const double inverse = drawn ? 1.0 / static_cast<double>(t) : 1.0;
   const Part* parts = a.parts + static_cast<size_t>(request) * (2 * a.places - 1) * a.part_count;
   const int drafts = a.draft != nullptr && drawn ? rows - 1 : 0;
-  if (drawn) fill_powers(powers);
   for (int i = wave; i < rows + drafts; i += kWaves) {
     Part part{0.0, -INFINITY, 0x7fffffff, 0, 0};
     if (lane < a.part_count) part = parts[static_cast<size_t>(i < rows ? i : a.places + i - rows) * a.part_count + lane];
@@ -368,23 +427,33 @@ __global__ __launch_bounds__(kChooseThreads) void choose_kernel(Verify a) {
   const float* x = a.logits + static_cast<size_t>(first + kept) * a.vocab;
   const float* y = from_draft ? a.draft + request * a.draft_request + kept * a.draft_place : nullptr;
   // (a logit of `top + t log(sum)` would have a probability of 1: probabilities come without a product)
-  Scale of_row = scale_of(t, static_cast<float>(row.top)), of_draft = of_row;
-  of_row.top += static_cast<double>(t) * log(row.sum);
-  if (from_draft) {
-    of_draft = scale_of(t, static_cast<float>(draft[kept].top));
-    of_draft.top += static_cast<double>(t) * log(draft[kept].sum);
-  }
-  // the weight of an id: p's, `plain`, or what q leaves of it (logits of minus infinity count 1e-299: no more than a rounding)
+  double rest, draft_rest = 1.0;
+  const float top = static_cast<float>(row.top), draft_top = from_draft ? static_cast<float>(draft[kept].top) : 0.f;
+  const Scale of_row = scale_of(t, inverse, top, t * log(row.sum), rest);
+  Scale of_draft{};
+  if (from_draft) of_draft = scale_of(t, inverse, draft_top, t * log(draft[kept].sum), draft_rest);
+  fill_powers(powers, rest);
+  if (from_draft) fill_powers(draft_powers, draft_rest);
+  __syncthreads();
+  // the weight of an id: p's, `plain`, or what q leaves of it (logits of minus infinity count next to nothing)
   auto weight_of = [&](float logit, float draft_logit, int id, bool plain) {
     const double p = just_exp(logit, of_row, powers);
-    if (from_draft && !plain) return fmax(difference(p, just_exp(draft_logit, of_draft, powers)), 0.0);
+    if (from_draft && !plain) return fmax(difference(p, just_exp(draft_logit, of_draft, draft_powers)), 0.0);
     return !plain && id == refused ? 0.0 : p;
   };
   // the sum of the weights of a part, the same in every thread
   auto sum_part = [&](int of_part, bool plain) {
     float v[kLoads][4], z[kLoads][4];
-    fetch_part<kThreads>(x, a.vocab, of_part, whole_pieces(a, x), v);
-    if (from_draft) fetch_part<kThreads>(y, a.vocab, of_part, whole_pieces(a, y), z);
+    fetch_run<kThreads, kPart>(x, a.vocab, of_part * kPart, whole_pieces(a, x), v);
+    if (from_draft) fetch_run<kThreads, kPart>(y, a.vocab, of_part * kPart, whole_pieces(a, y), z);
+    if (!of_row.near) {
+#pragma unroll
+      for (int u = 0; u < kLoads; ++u) only_largest(v[u], top);
+    }
+    if (from_draft && !of_draft.near) {
+#pragma unroll
+      for (int u = 0; u < kLoads; ++u) only_largest(z[u], draft_top);
+    }
     double sum = 0.0;
 #pragma unroll
     for (int u = 0; u < kLoads; ++u)
@@ -429,7 +498,7 @@ __global__ __launch_bounds__(kChooseThreads) void choose_kernel(Verify a) {
   }
   // by the request's last (or only) block: the part that the draw falls into
   double upto = sums_up_to(weight), total = of_lane(upto, kWave - 1);
-  if (!(total > 0.0)) {                // nothing is left of p: p itself
+  if (!(total > kLeast)) {              // nothing is left of p: p itself
     plain = true;
     weights_of_p();
     upto = sums_up_to(weight);
@@ -440,7 +509,7 @@ __global__ __launch_bounds__(kChooseThreads) void choose_kernel(Verify a) {
   const double goal = number < 1.f ? static_cast<double>(number) * total : INFINITY;
   // the first lane with weight whose sum lies beyond the goal, or the last lane with weight
   auto lane_of = [&](double value, double sum) {
-    const unsigned long long some = __ballot(value > 0.0), beyond = __ballot(value > 0.0 && sum > goal);
+    const unsigned long long some = __ballot(value > kLeast), beyond = __ballot(value > kLeast && sum > goal);
     return beyond != 0ull ? __builtin_ctzll(beyond) : some != 0ull ? kWave - 1 - __builtin_clzll(some) : -1;
   };
   const int at = max(0, lane_of(weight, upto));
@@ -451,7 +520,7 @@ __global__ __launch_bounds__(kChooseThreads) void choose_kernel(Verify a) {
   double w[kEach], own = 0.0;
   {
     float v[kEach], z[kEach];
-    auto fetch_run = [&](const float* from, float (&to)[kEach]) {
+    auto fetch_own = [&](const float* from, const Scale& scale, float largest, float (&to)[kEach]) {
       if (whole_pieces(a, from)) {
 #pragma unroll
         for (int u = 0; u < kLoads; ++u) {
@@ -462,12 +531,13 @@ __global__ __launch_bounds__(kChooseThreads) void choose_kernel(Verify a) {
 #pragma unroll
         for (int e = 0; e < kEach; ++e) to[e] = from[min(id0 + e, a.vocab - 1)];
       }
+      if (!scale.near) only_largest(to, largest);
     };
-    fetch_run(x, v);
-    if (from_draft) fetch_run(y, z);
+    fetch_own(x, of_row, top, v);
+    if (from_draft) fetch_own(y, of_draft, draft_top, z);
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
-      w[e] = id0 + e < a.vocab && v[e] > -INFINITY ? weight_of(v[e], z[e], id0 + e, plain) : 0.0;
+      w[e] = id0 + e < a.vocab ? weight_of(v[e], z[e], id0 + e, plain) : 0.0;
       own += w[e];
     }
   }
@@ -490,7 +560,7 @@ __global__ __launch_bounds__(kChooseThreads) void choose_kernel(Verify a) {
 #pragma unroll
   for (int e = 0; e < kEach; ++e) {
     sum += w[e];
-    if (w[e] > 0.0 && !done) {
+    if (w[e] > kLeast && !done) {
       last = id0 + e;
       done = sum > goal;
     }
@@ -522,6 +592,12 @@ extern "C" int akv_verify_drafts(const float* logits, int rows, int vocab, const
                                  const float* draft_logits, long draft_request_stride, long draft_place_stride, int* kept, int* chosen,
                                  void* workspace, hipStream_t stream) {
   if (!sizes_taken(requests, places, vocab) || rows < 0 || workspace == nullptr) return -2;
+  const long last_draft = (requests - 1) * draft_request_stride + (places - 2) * draft_place_stride + vocab;
+  const Span spans[] = {{kept, 4L * requests}, {chosen, 4L * requests * places}, {logits, 4L * rows * vocab}, {tokens, 4L * rows},
+                        {q_start, 4L * requests + 4}, {temperature, 4L * requests}, {uniforms, 4L * requests * places},
+                        {draft_logits, 4 * last_draft}};
+  const int shared = shared_spans(spans, 2, 8);
+  if (shared != 0) return shared;
   const int parts = part_count_of(vocab);
   char* room = static_cast<char*>(workspace);
   Verify a{};
@@ -533,7 +609,7 @@ extern "C" int akv_verify_drafts(const float* logits, int rows, int vocab, const
   a.draft_request = draft_request_stride; a.draft_place = draft_place_stride;
   a.rows = rows; a.vocab = vocab; a.requests = requests; a.places = places; a.part_count = parts;
   const int of_requests = draft_logits != nullptr ? 2 * places - 1 : places;
-  parts_kernel<<<dim3(parts, of_requests, requests), kThreads, 0, stream>>>(a);
+  parts_kernel<<<dim3((parts + kPerBlock - 1) / kPerBlock, of_requests, requests), kThreads, 0, stream>>>(a);
   const int first = AKV_LAUNCH_STATUS();
   if (first != 0) return first;
   // (as many blocks as the device holds at once, two a unit: every block decides for itself first, which takes it as long as two parts)

@@ -104,32 +104,19 @@ class RoundKernels:
         if not isinstance(t, torch.Tensor) or not t.is_cuda or t.get_device() != self.device.index:
             raise self._error(f"{name} must be a tensor on {self.device}, got {getattr(t, 'device', type(t))}")
 
-    def _vectors(self, spans: list, entries) -> list:
-        """Checks int32 vectors - (tensor, name, length, whether it is written) - and adds what memory they take to `spans`.  (One loop with
-        the comparisons in it: a call has fifteen of them and takes the device five microseconds.)"""
+    def _vectors(self, names, tensors, counts) -> None:
+        """Checks int32 vectors.  (One loop with the comparisons in it: a call has fifteen of them and takes the device five microseconds.)"""
         index, i32 = self.device.index, torch.int32
-        for t, name, count, out in entries:
+        for t, count in zip(tensors, counts):
             if t.dtype is not i32 or t.get_device() != index or t.dim() != 1 or t.numel() != count or not t.is_contiguous():
-                self._dense(t, name, i32, (count,))
-            low = t.data_ptr()
-            spans.append((low, low + 4 * count, out, name))
-        return spans
+                self._dense(t, names[[one is t for one in tensors].index(True)], i32, (count,))
 
-    def _apart(self, spans: list) -> None:
-        """Refuses outputs that lie in each other or in an input - `spans` of (begin, end, whether it is written, name) -: kernels of several
-        blocks read while others write."""
-        spans.sort()
-        end, of, of_out = 0, None, False
-        for low, high, out, name in spans:
-            if low < end and (out or of_out) and high > low:
-                raise self._error(f"{name} and {of} share memory")
-            if high > end or (out and high > low):
-                end, of, of_out = (high if high > end else end), name, out
-
-    @staticmethod
-    def _span(t, out: bool, name: str) -> tuple:
-        low = t.data_ptr()
-        return low, low + t.numel() * t.element_size(), out, name
+    def _check_spans(self, status: int, what: str, spans) -> None:
+        """`_check` of an entry that looks at what memory its operands share (csrc/common.h, `shared_spans`)."""
+        if status <= -1000:
+            first, second = divmod(-status - 1000, 64)
+            raise self._error(f"{what}: {spans[first]} and {spans[second]} share memory")
+        self._check(status, what)
 
     # ---- attention -----------------------------------------------------------------------------------------------------
     def attention_shared_prefix(self, q, k_pages, v_pages, block_table, q_start, seq_lens, shared, q_heads, kv_heads, head_dim, scale, out,
@@ -153,17 +140,12 @@ class RoundKernels:
         num_pages, page_size = self._pages(k_pages, v_pages, kv_heads, head_dim, q.dtype)
         if page_size < 8 or page_size & (page_size - 1):
             raise self._error(f"pages of {page_size} tokens: attention over a shared prompt takes 8 or more, a power of two")
-        spans = [self._span(out, True, "out"), self._span(q, False, "q"), self._span(k_pages, False, "k_pages"),
-                 self._span(v_pages, False, "v_pages")]
-        entries = [(q_start, "q_start", requests + 1, False), (seq_lens, "seq_lens", requests, False)]
+        self._vectors(("q_start", "seq_lens"), (q_start, seq_lens), (requests + 1, requests))
         if rows is not None:
-            entries.append((rows, "table rows", requests, False))
-        self._vectors(spans, entries)
+            self._dense(rows, "table rows", torch.int32, (requests,))
         self._dense(block_table, "block_table", torch.int32)
         if block_table.dim() != 2 or (rows is None and block_table.shape[0] != requests):
             raise self._error(f"block_table must be [{requests if rows is None else 'rows'}, pages], got {tuple(block_table.shape)}")
-        spans.append(self._span(block_table, False, "block_table"))
-        self._apart(spans)
         shared, max_seq_len, max_new_tokens = int(shared), int(max_seq_len), int(max_new_tokens)
         if shared < 0 or shared % page_size:
             raise self._error(f"a shared prompt of {shared} tokens is not whole pages of {page_size}")
@@ -190,11 +172,12 @@ class RoundKernels:
         # (from torch's pool: a recorded call then has room of its own, and calls on other streams do not meet in one)
         room = torch.empty(segments * tokens * q_heads * (head_dim + 2), dtype=torch.float32, device=self.device)
         sums = room.data_ptr()
-        self._check(self._shared_prefix_entry(head_dim)(
+        self._check_spans(self._shared_prefix_entry(head_dim)(
             q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), _DTYPE_CODE[q.dtype], sums,
             sums + 4 * segments * tokens * q_heads * head_dim, q_start.data_ptr(), seq_lens.data_ptr(), block_table.data_ptr(), _address(rows),
             block_table.shape[1], block_table.shape[0], requests, tokens, q_heads, kv_heads, page_size, num_pages, scale, shared, max_seq_len - shared, max_new_tokens,
-            prefix_segments, prefix_keys, own_segments, own_keys, int(wide), self._stream()), "attention_shared_prefix")
+            prefix_segments, prefix_keys, own_segments, own_keys, int(wide), self._stream()), "attention_shared_prefix",
+            ("out", "q", "k_pages", "v_pages", "block_table", "q_start", "seq_lens", "table rows"))
 
     # ---- drafted tokens ------------------------------------------------------------------------------------------------
     def verify_drafts(self, logits, tokens, q_start, temperature, uniforms, kept, chosen, draft_logits=None):
@@ -202,23 +185,22 @@ class RoundKernels:
         the target's own draws.  logits [rows, vocab] float32: the target's, for the rows q_start[r] .. q_start[r + 1] - 1 (int32) of
         request r; tokens [rows] int32: what was fed there, the request's last token and its drafts behind it.  uniforms [requests,
         places] float32 in [0, 1), places - 1 the most drafts of a request: number i for draft i, the last for the token that follows.
-        temperature [requests] float32; 0 (or less) keeps a draft where it is the largest logit (ties: the lowest id).
+        temperature [requests] float32, up to 1e28 (more is taken as that); 0 (or less) keeps a draft where it is the largest logit (ties: the
+        lowest id).
         draft_logits [requests, places - 1, vocab] float32: what the drafts were drawn from, at the same temperature - any strides, rows
         contiguous; None: drafts that were not drawn (looked up in a text), kept with the target's probability of them.
         kept [requests], chosen [requests, places] int32: the kept drafts, the token that follows, -1 behind it.
-        A request without rows, or with rows that are not among the logits, gets 0 and -1; rows beyond `places` are not looked at.  A row that has no next token - a NaN, nothing above minus infinity, or (where it is
-        drawn from) plus infinity, in the target's or the draft's - ends the walk with -1 as the token.  A draft that is no id of the
-        vocabulary is not kept."""
+        A request without rows, or with rows that are not among the logits, gets 0 and -1; rows beyond `places` are not looked at.  A row
+        that has no next token - a NaN, nothing above minus infinity, or (where it is drawn from) plus infinity, in the target's or the
+        draft's - ends the walk with -1 as the token.  A draft that is no id of the vocabulary is not kept."""
         if logits.dim() != 2 or uniforms.dim() != 2:
             raise self._error("logits and uniforms must be matrices")
         (count, vocab), (requests, places) = logits.shape, uniforms.shape
         self._dense(logits, "logits", torch.float32)
-        spans = self._vectors([], ((tokens, "tokens", count, False), (q_start, "q_start", requests + 1, False), (kept, "kept", requests, True)))
+        self._vectors(("tokens", "q_start", "kept"), (tokens, q_start, kept), (count, requests + 1, requests))
         self._dense(temperature, "temperature", torch.float32, (requests,))
         self._dense(uniforms, "uniforms", torch.float32)
         self._dense(chosen, "chosen", torch.int32, (requests, places))
-        spans += [self._span(chosen, True, "chosen"), self._span(logits, False, "logits"), self._span(temperature, False, "temperature"),
-                  self._span(uniforms, False, "uniforms")]
         strides = (0, 0)
         if draft_logits is not None and places > 1:
             self._placed(draft_logits, "draft_logits")
@@ -229,22 +211,20 @@ class RoundKernels:
             strides = draft_logits.stride()[:2]
         elif draft_logits is not None:
             draft_logits = None
-        if draft_logits is not None:      # (any strides: from its first element to its last)
-            low = draft_logits.data_ptr()
-            last = sum((n - 1) * stride for n, stride in zip(draft_logits.shape, draft_logits.stride())) if draft_logits.numel() else -1
-            spans.append((low, low + 4 * (last + 1), False, "draft_logits"))
-        self._apart(spans)
         if requests == 0:
             return
         lib = self._rounds()
         room = lib.akv_verify_workspace(requests, places, vocab)
         if room < 0:
-            raise self._error(f"verify_drafts: {requests} requests of up to {places} rows of {vocab} logits: at most 65,535, 64 and 524,288 are taken")
+            raise self._error(f"verify_drafts: {requests} requests of up to {places} rows of {vocab} logits: at most 65,535, 64 and 262,144 are taken")
         workspace = torch.empty(room, dtype=torch.uint8, device=self.device)
-        self._check(lib.akv_verify_drafts(
+        self._check_spans(lib.akv_verify_drafts(
             logits.data_ptr(), count, vocab, tokens.data_ptr(), q_start.data_ptr(), temperature.data_ptr(), uniforms.data_ptr(), requests, places,
             _address(draft_logits), strides[0], strides[1], kept.data_ptr(), chosen.data_ptr(), workspace.data_ptr(), self._stream()),
-            "verify_drafts")
+            "verify_drafts", ("kept", "chosen", "logits", "tokens", "q_start", "temperature", "uniforms", "draft_logits"))
+
+    _PLACED = ("lengths", "counts", "held", "free_pages", "cursor", "q_start", "seq_lens", "held_after", "cursor_after", "positions", "seq_of_token",
+               "slot_map", "status")
 
     # ---- a step's layout -----------------------------------------------------------------------------------------------
     def place_tokens(self, lengths, counts, held, free_pages, cursor, table, page_size, q_start, seq_lens, held_after, cursor_after, positions,
@@ -259,28 +239,26 @@ class RoundKernels:
         narrow or that two requests name, -3 more tokens than the maps have room for, -4 a negative number, or fewer pages than a length fills."""
         requests, tokens = lengths.shape[0], positions.shape[0]
         lib = self._rounds()
-        entries = [(lengths, "lengths", requests, False), (counts, "counts", requests, False), (held, "held", requests, False),
-                   (free_pages, "free_pages", free_pages.shape[0], False), (cursor, "cursor", 1, False), (q_start, "q_start", requests + 1, True),
-                   (seq_lens, "seq_lens", requests, True), (held_after, "held_after", requests, True), (cursor_after, "cursor_after", 1, True),
-                   (positions, "positions", tokens, True), (seq_of_token, "seq_of_token", tokens, True), (slot_map, "slot_map", tokens, True),
-                   (status, "status", 1, True)]
+        free = free_pages.shape[0]
+        self._vectors(self._PLACED, (lengths, counts, held, free_pages, cursor, q_start, seq_lens, held_after, cursor_after, positions, seq_of_token,
+                                     slot_map, status),
+                      (requests, requests, requests, free, 1, requests + 1, requests, requests, 1, tokens, tokens, tokens, 1))
         if rows is not None:
-            entries.append((rows, "table rows", requests, False))
+            self._dense(rows, "table rows", torch.int32, (requests,))
         if prefix_pages is not None:
-            entries.append((prefix_pages, "prefix_pages", prefix_pages.shape[0], False))
-        spans = self._vectors([], entries)
+            self._dense(prefix_pages, "prefix_pages", torch.int32, (prefix_pages.shape[0],))
         self._dense(table, "table", torch.int32)
         if table.dim() != 2 or (rows is None and table.shape[0] < requests):
             raise self._error(f"table must be a matrix with a row for each of {requests} requests, got {tuple(table.shape)}")
-        spans.append(self._span(table, True, "table"))
         if page_size < 1 or page_size != int(page_size):
             raise self._error(f"page_size {page_size} must be a positive number of tokens")
         if requests > self._place_most:
             raise self._error(f"{requests} requests in one step; at most {self._place_most} are taken")
-        self._apart(spans)
-        self._check(lib.akv_place_tokens(
-            lengths.data_ptr(), counts.data_ptr(), held.data_ptr(), free_pages.data_ptr(), free_pages.shape[0], cursor.data_ptr(),
+        self._check_spans(lib.akv_place_tokens(
+            lengths.data_ptr(), counts.data_ptr(), held.data_ptr(), free_pages.data_ptr(), free, cursor.data_ptr(),
             table.data_ptr(), _address(rows), table.shape[0], table.shape[1], int(page_size), _address(prefix_pages),
             prefix_pages.shape[0] if prefix_pages is not None else 0, requests, tokens, q_start.data_ptr(), seq_lens.data_ptr(),
             held_after.data_ptr(), cursor_after.data_ptr(), positions.data_ptr(), seq_of_token.data_ptr(), slot_map.data_ptr(),
-            status.data_ptr(), self._stream()), "place_tokens")
+            status.data_ptr(), self._stream()), "place_tokens",
+            ("q_start", "seq_lens", "held_after", "cursor_after", "positions", "seq_of_token", "slot_map", "status", "table", "lengths", "counts",
+             "held", "cursor", "free_pages", "table rows", "prefix_pages"))

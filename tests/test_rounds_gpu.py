@@ -5,6 +5,7 @@ import math
 import pytest
 import torch
 
+from ampere_kv_engine_amd.kernels.hip import KernelError
 from ampere_kv_engine_amd.kernels.hip_rounds import wide_tiles, wide_tiles_fit
 from plain import rounds_plain
 
@@ -332,6 +333,26 @@ def test_a_draft_model_that_leaves_nothing(kernels):
     assert kept.tolist() == [0, 0, 0] and bool((chosen[:, 0] >= 0).all())
 
 
+@pytest.mark.parametrize("with_draft", [True, False], ids=["drawn", "looked-up"])
+@pytest.mark.parametrize("t", [1e-45, 1e-30, 1e-20, 1e-12, 1e-8, 1e-4, 1e4, 1e20, 1e28])
+def test_temperatures_far_from_one(kernels, with_draft, t):
+    """Cold rows are all on their largest logits (equal ones share it), warm ones nearly even; in each, minus infinity has no weight."""
+    vocab, counts = 9001, (3, 2, 3, 3, 1)
+    logits, tokens, starts, temperature, uniforms, draft = drafted(vocab, counts, 3, with_draft, 21)
+    temperature = torch.full_like(temperature, t)
+    uniforms[:, -1] = torch.tensor([0.0, 0.3137, 0.5171, 0.7, 0.999])
+    logits[0, [5, 4100, 9000]] = logits[0].max()                  # one row's largest three times, in several parts
+    logits[starts[1]] = torch.finfo(torch.float32).min            # rows of nothing but the lowest value, and masks below it
+    logits[starts[1], 100:] = -math.inf
+    logits[starts[2], ::2] = -math.inf
+    logits[starts[3]] = -math.inf
+    logits[starts[3], 4097] = -3.4e38
+    if draft is not None:
+        draft[1, 0, 7:] = -math.inf
+        draft[2, 0] = logits[starts[2]]
+    verify_both(kernels, logits, tokens, starts, temperature, uniforms, draft)
+
+
 def test_ties_go_to_the_lowest_id(kernels):
     logits, tokens, starts, temperature, uniforms, _ = drafted(20000, (3, 3), 3, False, 6, temperatures=(0.0,))
     logits[:, [77, 9000, 19999]] = 50.0
@@ -576,3 +597,32 @@ def test_calls_on_two_streams_at_once(kernels):
     for (attention, verify), out, (kept, chosen) in zip(arguments, good, want):
         assert torch.equal(attention["out"], out)
         assert verify["kept"].tolist() == kept and verify["chosen"].tolist() == chosen
+
+
+@pytest.mark.parametrize("first,second", [("lengths", "seq_lens"), ("held", "held_after"), ("cursor", "cursor_after"), ("positions", "slot_map"),
+                                          ("free_pages", "status"), ("table", "status")])
+def test_layout_refuses_what_shares_memory(kernels, first, second):
+    vector = lambda n: torch.zeros(n, dtype=torch.int32, device=DEV)
+    arguments = dict(lengths=vector(3), counts=vector(3), held=vector(3), free_pages=vector(9), cursor=vector(1), table=vector(12).view(3, 4),
+                     page_size=16, q_start=vector(4), seq_lens=vector(3), held_after=vector(3), cursor_after=vector(1), positions=vector(5),
+                     seq_of_token=vector(5), slot_map=vector(5), status=vector(1))
+    arguments[second] = arguments[first].view(-1)[:len(arguments[second])]
+    with pytest.raises(KernelError, match="share memory"):
+        kernels.place_tokens(**arguments)
+
+
+def test_attention_and_verification_refuse_what_shares_memory(kernels):
+    case = batch(torch.bfloat16, 8, 2, 64, 16, 64, (3, 40), (2, 1), seed=50)
+    q = case["q"].to(DEV)
+    with pytest.raises(KernelError, match="out and q share memory"):
+        attend(kernels, case, q=q, out=q)
+    pages = case["k"].to(DEV)
+    with pytest.raises(KernelError, match="out and k_pages share memory"):
+        attend(kernels, case, k_pages=pages, out=pages.view(-1)[1024:1024 + 3 * 512].view(3, 512))
+    logits, tokens, starts, temperature, uniforms, draft = drafted(100, (3, 2, 3), 3, True, 51)
+    tokens, chosen = tokens.to(DEV), torch.zeros(3, 3, dtype=torch.int32, device=DEV)
+    arguments = dict(logits=logits.to(DEV), tokens=tokens, q_start=ints(starts), temperature=temperature.to(DEV), uniforms=uniforms.to(DEV),
+                     kept=ints([0, 0, 0]), chosen=chosen, draft_logits=draft.to(DEV))
+    for changes in (dict(kept=tokens[2:5]), dict(kept=chosen.view(-1)[6:9]), dict(tokens=chosen.view(-1)[:8])):
+        with pytest.raises(KernelError, match="share memory"):
+            kernels.verify_drafts(**{**arguments, **changes})

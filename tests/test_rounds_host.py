@@ -1,6 +1,7 @@
 """What the calls of a drafted round refuse, and how they cut their work, on the CPU: the kernel set with its device checks and its
 library replaced by recorders."""
 
+import ctypes
 import random
 
 import pytest
@@ -45,7 +46,7 @@ class Recorder(HipKernels):
 
         class Library:
             def akv_verify_workspace(self, requests, places, vocab):
-                return -1 if places > 64 or vocab > 524288 or requests > 65535 else 1024
+                return -1 if places > 64 or vocab > 262144 or requests > 65535 else 1024
 
             def akv_verify_drafts(self, *arguments):
                 recorder.calls.append(arguments)
@@ -93,14 +94,8 @@ def test_attention_refuses(changes):
     assert not kernels.calls
 
 
-def test_attention_refuses_an_output_in_an_input_and_odd_addresses():
+def test_attention_refuses_odd_addresses():
     kernels = Recorder()
-    q = torch.zeros(5, 512)
-    with pytest.raises(KernelError, match="share memory"):
-        kernels.attention_shared_prefix(**attention(q=q, out=q))
-    pages = torch.zeros(12, 2, 16, 64)
-    with pytest.raises(KernelError, match="share memory"):
-        kernels.attention_shared_prefix(**attention(k_pages=pages, out=pages.view(-1)[512:512 + 5 * 512].view(5, 512)))
     with pytest.raises(KernelError, match="16-byte"):
         kernels.attention_shared_prefix(**attention(q=torch.zeros(5 * 512 + 1)[1:].view(5, 512)))
 
@@ -143,16 +138,6 @@ def test_verification_refuses(changes):
     with pytest.raises(KernelError):
         kernels.verify_drafts(**verification(**changes))
     assert not kernels.calls
-
-
-def test_verification_refuses_outputs_in_inputs():
-    kernels = Recorder()
-    tokens = torch.zeros(7, dtype=I32)
-    with pytest.raises(KernelError, match="share memory"):
-        kernels.verify_drafts(**verification(tokens=tokens, kept=tokens[:3]))
-    chosen = torch.zeros(3, 4, dtype=I32)
-    with pytest.raises(KernelError, match="share memory"):
-        kernels.verify_drafts(**verification(chosen=chosen, kept=chosen.view(-1)[2:5]))
 
 
 def layout(**changes):
@@ -205,19 +190,31 @@ def test_layout_refuses_more_requests_than_it_takes():
                                       q_start=torch.zeros(n + 1, dtype=I32), table=torch.zeros(n, 1, dtype=I32)))
 
 
-@pytest.mark.parametrize("first,second", [("lengths", "seq_lens"), ("held", "held_after"), ("cursor", "cursor_after"), ("positions", "slot_map"),
-                                          ("free_pages", "status")])
-def test_layout_refuses_what_shares_memory(first, second):
+def test_spans_that_overlap():
+    """The entries' check of what memory their operands share, by itself."""
+    lib = ctypes.CDLL(build.ensure_rounds())
+
+    def shared(written, *spans):
+        begins = (ctypes.c_void_p * len(spans))(*(begin or None for begin, _ in spans))
+        sizes = (ctypes.c_long * len(spans))(*(size for _, size in spans))
+        return lib.akv_shared_spans(begins, sizes, written, len(spans))
+
+    assert shared(1, (100, 20), (120, 4), (96, 4), (300, 0)) == 0
+    assert shared(1, (100, 20), (119, 4)) == -(1000 + 1)
+    assert shared(1, (100, 20), (200, 8), (90, 11)) == -(1000 + 2)
+    assert shared(1, (100, 20), (50, 500)) == -(1000 + 1)
+    assert shared(2, (100, 20), (200, 20), (300, 4), (210, 1)) == -(1000 + 64 + 3)
+    assert shared(1, (100, 20), (200, 40), (210, 40)) == 0           # (what is only read may overlap)
+    assert shared(1, (100, 0), (100, 0)) == 0 and shared(1, (100, 20), (110, 0)) == 0 and shared(1, (100, 20), (0, 500)) == 0
+
+
+def test_what_shares_memory_is_named():
     kernels = Recorder()
-    arguments = layout()
-    n = len(arguments[second])
-    arguments[second] = arguments[first].view(-1)[:n]
-    with pytest.raises(KernelError, match="share memory"):
-        kernels.place_tokens(**arguments)
-    arguments = layout()
-    arguments["status"] = arguments["table"].view(-1)[5:6]
-    with pytest.raises(KernelError, match="share memory"):
-        kernels.place_tokens(**arguments)
+    kernels._shared_prefix_entry = lambda head_dim: lambda *arguments: -(1000 + 2)
+    with pytest.raises(KernelError, match="out and k_pages share memory"):
+        kernels.attention_shared_prefix(**attention())
+    with pytest.raises(KernelError, match="dtype not supported"):
+        kernels._check_spans(-1, "this", ())
 
 
 def test_segments_cover_the_keys():
