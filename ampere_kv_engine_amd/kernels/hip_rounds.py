@@ -36,20 +36,21 @@ def wide_tiles(rows: int, kv_heads: int, shared: int, units: int) -> bool:
 
 
 def cut_own(requests: int, rows: int, kv_heads: int, most: int, units: int) -> tuple[int, int]:
-    """(segments, keys of one) of up to `most` keys that a request of up to `rows` rows a kv head holds behind the prompt.  Six blocks a unit:
-    a unit holds two, and what a block waits for at its start and end is a good part of its time; but a long request's keys are not to
-    outlast the others'.  Segments of 128 keys - a step for each of a block's waves - at least.  (64 requests of up to 2,053 keys, 8 kv
-    heads, whole calls, us: segments of 256 keys 84, 512 82, 768 83, 1,024 83; 27 of 2,005: 69, 68, 70, 69, and of 384 65; 64 of 517 with 40
-    rows each: 158, 148, 139, 138.)"""
+    """(segments, keys of one) of up to `most` keys that a request of up to `rows` rows a kv head holds behind the prompt.  Four blocks a unit,
+    of which it holds two: what a block waits for at its start and end is a good part of its time; but a long request's keys are not to
+    outlast the others', so no segment has more than about a thousand; and 128 keys - a step for each of a block's waves - at least.
+    (Whole calls, us, with two, three, four and six blocks a unit, 8 kv heads: 64 requests of 517 keys 112, 111, 115, 124; 27 of up to
+    2,005 72, 71, 69, 69; 64 of up to 512 40, 40, 38, 38; 40 of up to 700 29, 29, 28, 28.)"""
     blocks = requests * kv_heads * ((rows + 31) // 32)
-    segments = max(1, min((most + 127) // 128, 6 * units // blocks, 256))
+    segments = max(1, min((most + 127) // 128, max(4 * units // blocks, (most + 1023) // 1024), 256))
     keys = ((most + segments - 1) // segments + 127) // 128 * 128
     return (most + keys - 1) // keys, keys
 
 
 def cut_prefix(columns: int, rows: int, kv_heads: int, shared: int, units: int, own_blocks: int) -> tuple[int, int]:
     """The same of a shared prompt, whose blocks take `columns` rows each: as many as the device holds at once, one a unit of
-    256 columns or two of 32, segments of 128 keys at least.  Tiles of 32 columns wait for reads, and leave room for up to half as many blocks of the requests' own keys beside them."""
+    256 columns or two of 32, segments of 128 keys at least.  Tiles of 32 columns wait for reads, and leave room for up to half as many
+    blocks of the requests' own keys beside them."""
     if shared == 0:
         return 0, 32
     blocks = kv_heads * ((rows + columns - 1) // columns)
@@ -130,7 +131,8 @@ class RoundKernels:
         thousands of tokens are `attention`'s).
         float32 or bfloat16; head sizes as `check_attention_sizes` has them; pages of 8 tokens or more, a power of two.
         A token gets NaN where its request's table (or the first one's, of the prompt) names a page outside the pool or is no row of
-        block_table, where its request exceeds the bounds, or where it stands within the prompt.  Rows of `out` behind the last request's are left as they are."""
+        block_table, where its request exceeds the bounds, or where it stands within the
+        prompt.  Rows of `out` behind the last request's are left as they are."""
         tokens, requests = q.shape[0], seq_lens.shape[0]
         self.check_attention_sizes(q_heads, kv_heads, head_dim, 1)
         if q.dtype not in _DTYPE_CODE:
