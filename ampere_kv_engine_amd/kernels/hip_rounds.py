@@ -234,7 +234,8 @@ class RoundKernels:
         """A step's layout from lengths on the device (all int32).  lengths, counts, held [requests]: the tokens a request holds, those it
         brings, and its pages.  It takes the pages it lacks from free_pages[cursor ...], in the requests' order; they are entered into its
         row of `table` (row r, or rows[r]), and held_after [requests] and cursor_after [1] say what is held and taken then.  A request
-        that holds no page starts on `prefix_pages`, if they are given: they are entered too, and `lengths` counts their tokens.
+        that holds no page starts on `prefix_pages`, if they are given: they are entered too, and `lengths` counts their tokens
+        (all of them: what a request brings within shared pages would be written into them).
         q_start [requests + 1], seq_lens [requests] (the tokens held after the step); positions, seq_of_token and slot_map [tokens]: of
         every token, request by request; tokens are all that the requests bring, or more: entries behind the last are left as they are.
         status [1]: the pages taken, or, with nothing else written, -1 too few free pages, -2 a row that the table does not have, that is too

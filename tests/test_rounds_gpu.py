@@ -231,6 +231,42 @@ def test_a_request_gives_the_same_whatever_stands_beside_it(tiled):
     assert torch.equal(out[1::2], good[1::2]) and bool(out[::2].isnan().all())
 
 
+def test_attention_in_a_pool_of_many_gigabytes(tiled):
+    """Pages whose places lie beyond 2^31 elements and 2^32 bytes."""
+    case = batch(torch.bfloat16, 16, 4, 128, 16, 512, (20, 300, 5), (2, 1, 3), seed=61)
+    pages, far = len(case["k"]), 300_000
+    pools = {}
+    for name in ("k", "v"):
+        pool = torch.empty((far + pages, *case[name].shape[1:]), dtype=torch.bfloat16, device=DEV)
+        pool[far:] = case[name].to(DEV)
+        pools[name + "_pages"] = pool
+    assert pools["k_pages"].numel() > 2 ** 31
+    table = torch.where(case["table"] >= 0, case["table"] + far, case["table"])
+    near = attend(tiled, case)
+    within(tiled, case, near)
+    assert torch.equal(attend(tiled, case, block_table=table.to(DEV), **pools), near)
+
+
+def test_attention_recorded(tiled):
+    """A recorded call, replayed over changed queries and lengths with eager calls in between, gives what the eager call does."""
+    case = batch(torch.bfloat16, 16, 4, 128, 16, 512, (20, 300, 5), (2, 1, 3), seed=62)
+    q, lengths, out = case["q"].to(DEV), ints(case["lengths"]), torch.empty_like(case["q"], device=DEV)
+    pages = dict(k_pages=case["k"].to(DEV), v_pages=case["v"].to(DEV), block_table=case["table"].to(DEV), q_start=ints(case["starts"]))
+    run = lambda to: attend(tiled, case, q=q, seq_lens=lengths, out=to, **pages)
+    run(out)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        tiled.attention_shared_prefix(q, seq_lens=lengths, shared=512, q_heads=16, kv_heads=4, head_dim=128, scale=case["scale"], out=out,
+                                      max_seq_len=max(case["lengths"]), max_new_tokens=3, **pages)
+    for turn in range(3):
+        q.mul_(-0.9)
+        lengths.sub_(ints([1, 2, 0]))
+        want = run(torch.empty_like(out))
+        out.zero_()
+        graph.replay()
+        assert torch.equal(out, want)
+
+
 def test_attention_agrees_with_the_engines_own(kernels):
     """The same requests through `HipKernels.attention`."""
     from types import SimpleNamespace
@@ -375,6 +411,21 @@ def test_rows_without_a_next_token(kernels, value, place):
         verify_both(kernels, logits, tokens, starts, temperature, uniforms, draft)
 
 
+def test_logits_of_many_gigabytes(kernels):
+    """Rows beyond 2^31 logits, and requests that do not begin at the first row."""
+    vocab, before = 151936, 14200
+    logits, tokens, starts, temperature, uniforms, draft = drafted(vocab, (2, 3), 3, True, 63)
+    all_logits = torch.empty((before + len(logits), vocab), device=DEV)
+    all_logits[before:] = logits.to(DEV)
+    assert before * vocab > 2 ** 31
+    all_tokens = torch.cat([torch.zeros(before, dtype=torch.int32), tokens])
+    kept, chosen = ints([9, 9]), torch.zeros(2, 3, dtype=torch.int32, device=DEV)
+    kernels.verify_drafts(all_logits, all_tokens.to(DEV), ints([s + before for s in starts]), temperature.to(DEV), uniforms.to(DEV), kept, chosen,
+                          draft_logits=draft.to(DEV))
+    want = rounds_plain.verify(logits, tokens, starts, temperature, uniforms, draft)
+    assert kept.tolist() == want[0] and chosen.tolist() == want[1]
+
+
 def test_drafts_that_are_no_ids(kernels):
     logits, tokens, starts, temperature, uniforms, draft = drafted(600, (3, 3, 3), 3, True, 8)
     tokens[1], tokens[4], tokens[8] = -1, 600, 2 ** 31 - 1
@@ -488,8 +539,8 @@ def test_layout_without_requests(kernels):
 
 @pytest.mark.parametrize("every", [3, 1])
 def test_rounds_follow_each_other_on_the_device(kernels, every):
-    """(Every `every`-th token is the best one behind the token before it: a draft that a greedy request keeps.)  Three rounds with nothing read back in between - place, write keys and values, attend, verify -, eagerly and recorded, against
-    the same on the host."""
+    """(Every `every`-th token is the best one behind the token before it: a draft that a greedy request keeps.)  Three rounds with nothing
+    read back in between - place, write keys and values, attend, verify -, eagerly and recorded, against the same on the host."""
     heads, kv_heads, dim, page, vocab, requests, places = 8, 2, 64, 16, 500, 5, 4
     generator = torch.Generator().manual_seed(21)
     shared, pool = 64, 64
