@@ -172,14 +172,16 @@ __device__ __forceinline__ float sum_over_halves(float v) {
   return __uint_as_float(swapped[0]) + __uint_as_float(swapped[1]);
 }
 
-// One tile of 32 columns over the keys first_key .. end_key - 1, by the block's waves in turn, 32 keys a step.
+// One tile of 32 columns over the keys first_key .. end_key - 1, by WAVES waves in turn, 32 keys a step: the block's, or one of its
+// TEAMS, which take a tile each (none: `columns` and keys of 0).
 // `row0`: the tile's first row of the kv head's, `columns` how many of the 32 are there.  A column sees the keys below `visible`
 // (its lane's), `all_see` the least of them over the tile.  `wanted`: a bit for each column whose results are written.
-template <typename T, int WAVES>
+template <typename T, int WAVES, int TEAMS = 1>
 __device__ __forceinline__ void walk(const Args& a, const int* table, int head, long row0, int columns, int first_key, int end_key,
                                      int visible, int all_see, int segment, float* lds, uint32_t wanted = 0xffffffffu) {
   constexpr int kBuffers = WAVES / 2;
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave % WAVES, thread = threadIdx.x % (WAVES * kWave);
+  if (TEAMS > 1) lds += __builtin_amdgcn_readfirstlane(threadIdx.x / (WAVES * kWave)) * (narrow_lds<T>(WAVES) / sizeof(float));
   const int r = lane & 31, half = lane >> 5;
   const int group = static_cast<int>(a.group.by), segments = a.prefix_segments + a.own_segments;
   const int page_mask = (1 << a.page_shift) - 1;
@@ -205,14 +207,14 @@ __device__ __forceinline__ void walk(const Args& a, const int* table, int head, 
   };
   const int first_base = first_key + 32 * wave;
   if (first_base < end_key) lookup(first_base);
-  for (int c = wave; c < KC; c += WAVES) {
+  for (int c = wave; c < KC && (TEAMS == 1 || columns > 0); c += WAVES) {
     const long row = row0 + min(r, columns - 1);
     const long token = group == 1 ? row : row / group;
     const T* q = static_cast<const T*>(a.q) + (token * a.q_heads + static_cast<long>(head) * group + (row - token * group)) * D + 8 * half;
     queries[c * kWave + lane] = load_piece<T>(q + 16 * c);
   }
   if (wave == 0 && half == 0) seen[r] = visible;
-  if (threadIdx.x == 0) seen[32] = 0;
+  if (thread == 0) seen[32] = 0;
   Piece<T> kf[KC], vf[2][DT];
   auto fetch_keys = [&](int base, int page) {
     const int key = min(base + key_at, end_key - 1);
@@ -350,7 +352,7 @@ __device__ __forceinline__ void walk(const Args& a, const int* table, int head, 
   }
   float* sums = a.sums + ((static_cast<size_t>(head) * segments + segment) * a.rows + row0) * D;
   const bool any_odd = seen[32] != 0;
-  for (int i = threadIdx.x; i < columns * (D / 4); i += WAVES * kWave) {
+  for (int i = thread; i < columns * (D / 4); i += WAVES * kWave) {
     const int column = i / (D / 4), at = i % (D / 4) * 4;
     if (((wanted >> column) & 1u) == 0u) continue;
     floatx4 sum = *reinterpret_cast<const floatx4*>(lds + column * kRow + at);
@@ -668,8 +670,8 @@ __global__ __launch_bounds__(kWideWaves * kWave, 2) void wide_prefix_kernel(Args
   }
 }
 
-// Blocks 0 .. prefix_blocks - 1 take (segment and head, tile) of the prefix, the others (request, head, tile, segment) of the requests'
-// own keys.
+// Blocks 0 .. prefix_blocks - 1 take (segment and head, tile) of the prefix, the others (request, head, two tiles, segment) of the
+// requests' own keys.
 template <typename T>
 __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 || D > 128 ? 1 : 2)) void shared_prefix_kernel(Args a) {
   extern __shared__ float lds[];
@@ -687,7 +689,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 || D > 128 ? 1 : 2)) void
     visible = all_see = end = min(a.shared, first + a.prefix_keys);
   } else {
     block -= a.prefix_blocks;
-    tile_of(block, static_cast<long>(a.requests) * a.kv_heads * a.own_segments, a.own_tiles, item, tile);
+    tile_of(block, static_cast<long>(a.requests) * a.kv_heads * a.own_segments, (a.own_tiles + 1) / 2, item, tile);
     // (segments last: with them first, every eighth block - one XCD's - would be of the segments that short requests do not have)
     head = static_cast<int>(item % a.kv_heads);
     item /= a.kv_heads;
@@ -695,16 +697,28 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 || D > 128 ? 1 : 2)) void
     segment = static_cast<int>(item / a.requests);
     const int begin = a.q_start[request], count = a.q_start[request + 1] - begin, length = a.seq_lens[request], before = length - count;
     if (!within_bounds(a, begin, count, length)) return;
-    const int group = static_cast<int>(a.group.by);
-    columns = min(32, count * group - 32 * tile);
-    if (columns <= 0) return;
+    const int group = static_cast<int>(a.group.by), left = count * group - 64 * tile;
+    if (left <= 0) return;
+    // two tiles, where a request brings them, for half of the waves each: what one reads the other finds in the unit's cache (64 requests
+    // of 40 rows a head, calls with equal lengths of 517 139 -> 134 us, with lengths up to that 93 -> 89)
+    const bool pair = left > 32;
+    const int column0 = 64 * tile + (pair ? 32 * __builtin_amdgcn_readfirstlane(threadIdx.x / (kThreads / 2)) : 0);
+    columns = min(32, count * group - column0);
     first = a.shared + segment * a.own_keys;
-    end = min(before + a.group.quotient(32 * tile + columns - 1) + 1, first + a.own_keys);     // (what the tile's last token sees)
-    if (first >= end) return;
-    visible = before + a.group.quotient(32 * tile + min(r, columns - 1)) + 1;
-    all_see = before + a.group.quotient(32 * tile) + 1;
-    row0 = static_cast<long>(begin) * group + 32 * tile;
+    end = min(before + a.group.quotient(column0 + columns - 1) + 1, first + a.own_keys);       // (what the tile's last token sees)
+    if (first >= end) {
+      if (!pair) return;
+      columns = 0;
+    }
+    visible = before + a.group.quotient(column0 + min(r, max(columns, 1) - 1)) + 1;
+    all_see = before + a.group.quotient(column0) + 1;
+    row0 = static_cast<long>(begin) * group + column0;
     segment += a.prefix_segments;
+    if (pair) {
+      const int* table = table_of(a, request);
+      if (table != nullptr) walk<T, kWaves / 2, 2>(a, table, head, row0, columns, first, end, visible, all_see, segment, lds);
+      return;
+    }
   }
   const int* table = table_of(a, request);
   if (table == nullptr) return;
@@ -812,7 +826,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Args a) {
 }
 
 template <typename K> int room_for(K kernel, size_t lds) {
-  static_assert(kWideLds <= 160 * 1024 && kWideNarrowLds <= 160 * 1024, "LDS of a compute unit");
+  static_assert(kWideLds <= 160 * 1024 && kWideNarrowLds <= 160 * 1024 && 2 * narrow_lds<float>(kWaves / 2) <= 160 * 1024, "LDS of a compute unit");
   if (lds <= 64 * 1024) return 0;
   return static_cast<int>(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
 }
@@ -820,8 +834,8 @@ template <typename K> int room_for(K kernel, size_t lds) {
 // `wide`: the prefix goes to `wide_prefix_kernel`, and the requests' own keys alone to the other one, which holds twice as many blocks a
 // unit.
 template <typename T> int run(const Args& all, bool wide, hipStream_t stream) {
-  constexpr size_t lds = narrow_lds<T>(kWaves);
   Args a = all;
+  const size_t lds = a.own_tiles > 1 ? 2 * narrow_lds<T>(kWaves / 2) : narrow_lds<T>(kWaves);       // (the former is the larger)
   int status = 0;
   if constexpr (kWideFits && sizeof(T) == 2)
     if (wide && a.prefix_blocks > 0) {
@@ -832,7 +846,7 @@ template <typename T> int run(const Args& all, bool wide, hipStream_t stream) {
       if ((status = AKV_LAUNCH_STATUS()) != 0) return status;
       a.prefix_blocks = 0;
     }
-  const long blocks = a.prefix_blocks + static_cast<long>(a.requests) * a.kv_heads * a.own_tiles * a.own_segments;
+  const long blocks = a.prefix_blocks + static_cast<long>(a.requests) * a.kv_heads * ((a.own_tiles + 1) / 2) * a.own_segments;
   if (blocks > 0x7fffffffL || a.q_heads > 65535) return -2;
   if ((status = room_for(shared_prefix_kernel<T>, lds)) != 0) return status;
   shared_prefix_kernel<T><<<static_cast<unsigned>(blocks), kThreads, lds, stream>>>(a);

@@ -36,13 +36,17 @@ def wide_tiles(rows: int, kv_heads: int, shared: int, units: int) -> bool:
 
 
 def cut_own(requests: int, rows: int, kv_heads: int, most: int, units: int) -> tuple[int, int]:
-    """(segments, keys of one) of up to `most` keys that a request of up to `rows` rows a kv head holds behind the prompt.  Four blocks a unit,
-    of which it holds two: what a block waits for at its start and end is a good part of its time; but a long request's keys are not to
-    outlast the others', so no segment has more than about a thousand; and 128 keys - a step for each of a block's waves - at least.
-    (Whole calls, us, with two, three, four and six blocks a unit, 8 kv heads: 64 requests of 517 keys 112, 111, 115, 124; 27 of up to
-    2,005 72, 71, 69, 69; 64 of up to 512 40, 40, 38, 38; 40 of up to 700 29, 29, 28, 28.)"""
-    blocks = requests * kv_heads * ((rows + 31) // 32)
-    segments = max(1, min((most + 127) // 128, max(4 * units // blocks, (most + 1023) // 1024), 256))
+    """(segments, keys of one) of up to `most` keys that a request of up to `rows` rows a kv head holds behind the prompt.  What a block waits
+    for at its start and end is a good part of its time, but a long request's keys are not to outlast the others': four blocks a unit,
+    of which it holds two, or six where not even those two are there without a cut; no segment of more than about a thousand keys, nor of
+    fewer than 128, a step for each of a block's waves.  (Whole calls, us, with two, three, four and six blocks a unit, 8 kv heads: 64
+    requests of 517 keys 112, 111, 115, 124; 64 of up to 512 40, 40, 38, 38; 64 of 2,053 128, 127, 127, 132; 27 of up to 2,005 72, 71,
+    73, 69; 5 of up to 2,005 14.5, 14.2, 14.3, 13.9.)  Blocks of two tiles, where a request has more than 32 rows, take twice as
+    long: three a unit.  (64 requests of 40 rows and 517 keys, in segments of 256, 384 and 640 keys: 148, 141, 134; of up to 517: 90, 89,
+    92; 16 of up to 2,005: 31, 30, 30.)"""
+    blocks = requests * kv_heads * ((rows + 63) // 64)
+    of_unit = 3 if rows > 32 else 4 if blocks >= 2 * units else 6
+    segments = max(1, min((most + 127) // 128, max(of_unit * units // blocks, (most + 1023) // 1024), 256))
     keys = ((most + segments - 1) // segments + 127) // 128 * 128
     return (most + keys - 1) // keys, keys
 

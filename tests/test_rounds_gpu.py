@@ -131,6 +131,8 @@ SHAPES = [
     (32, 2, 64, 128, 1024, (0, 260, 11), (1, 70, 33)),   # more rows of a request than a tile holds
     (34, 1, 64, 16, 96, (2, 3), (1, 2)),                 # a group wider than a tile
     (16, 4, 128, 16, 1600, tuple(3 + 5 * i for i in range(40)), (1,) * 40),
+    (2, 2, 64, 16, 160, (70,), (64,)),                   # the first tile sees nothing of the last segment, the second does
+    (16, 2, 256, 16, 128, (9, 40), (5, 6)),
 ]
 
 
