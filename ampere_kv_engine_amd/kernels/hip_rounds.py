@@ -28,38 +28,44 @@ def wide_tiles_fit(head_dim: int, page_size: int, dtype) -> bool:
 
 def wide_tiles(rows: int, kv_heads: int, shared: int, units: int) -> bool:
     """Whether the prompt's keys are multiplied in tiles of 256 columns that share them through LDS (`wide_prefix_kernel`, a launch of its
-    own) rather than of 32 beside the requests' own keys.  The shared ones cost 8 to 10 us more at their start and end and half as much a
-    column and key.  Whole calls, narrow / wide us, 256 units: 32 heads over 8 of 128, 128 own keys, 8,192 shared, 128 rows 26 / 36, 256
-    44 / 50; 32,768 shared, 64 rows 36 / 50, 128 58 / 56, 192 84 / 64, 256 100 / 71; 16 over 4 of 64, 32,768 shared, 128 rows 26 / 30, 192
-    35 / 32, 256 41 / 34."""
-    return rows * kv_heads * shared >= 110_000 * units
+    own) rather than of 32 beside the requests' own keys.  The shared ones cost 8 to 10 us more at their start and end and less a column
+    and key.  Whole calls, narrow / wide us, 256 units, 64 own keys: 32 heads over 8 of 128, 32,768 shared, 64 rows 38 / 52, 96 49 / 51, 112
+    57 / 53; 16,000 shared, 160 rows 42 / 43, 192 49 / 45, 256 57 / 49; 8,192 shared, 256 rows 35 / 42, 320 42 / 42; 2,048 shared, 960 rows
+    36 / 43, 1,280 53 / 46; 16 over 4 of 64, 32,768 shared, 128 rows 24 / 29, 192 33 / 31, 256 40 / 33."""
+    return rows * kv_heads * shared >= 85_000 * units
 
 
-def cut_own(requests: int, rows: int, kv_heads: int, most: int, units: int) -> tuple[int, int]:
+def cut_own(requests: int, rows: int, kv_heads: int, most: int, units: int, alone: bool) -> tuple[int, int]:
     """(segments, keys of one) of up to `most` keys that a request of up to `rows` rows a kv head holds behind the prompt.  What a block waits
-    for at its start and end is a good part of its time, but a long request's keys are not to outlast the others': four blocks a unit,
-    of which it holds two, or six where not even those two are there without a cut; no segment of more than about a thousand keys, nor of
-    fewer than 128, a step for each of a block's waves.  (Whole calls, us, with two, three, four and six blocks a unit, 8 kv heads: 64
-    requests of 517 keys 112, 111, 115, 124; 64 of up to 512 40, 40, 38, 38; 64 of 2,053 128, 127, 127, 132; 27 of up to 2,005 72, 71,
-    73, 69; 5 of up to 2,005 14.5, 14.2, 14.3, 13.9.)  Blocks of two tiles, where a request has more than 32 rows, take twice as
-    long: three a unit.  (64 requests of 40 rows and 517 keys, in segments of 256, 384 and 640 keys: 148, 141, 134; of up to 517: 90, 89,
-    92; 16 of up to 2,005: 31, 30, 30.)"""
+    for at its start and end is a good part of its time, but a long request's keys are not to outlast the others': no segment of more than
+    about a thousand keys, nor of fewer than 128, a step for each of a block's waves.  Beside the prompt's blocks, of which a unit has
+    one, one more a unit.  (8 kv heads, whole calls, us, equal lengths / up to that: 8 requests of 1,000 keys, 128, 256 and 512 blocks 23 /
+    22, 21 / 19, 25 / 24; 16 of 600, 256, 384, 640 blocks 20 / 19, 23 / 18, 25 / 21; 27 of 2,000, 432, 864, 1,728 blocks 47 / 30, 50 /
+    32, 53 / 30; 64 of 517, 512, 1,024, 1,536 blocks 47 / 40, 50 / 38, 55 / 38.)
+    `alone`, in a launch of their own: four a unit, which holds two, or six where not even those two are there without a cut.  (Two,
+    three, four and six a unit: 64 requests of 517 keys 112, 111, 115, 124; 64 of 2,053 128, 127, 127, 132; 27 of up to 2,005 72, 71,
+    73, 69.)  Blocks of two tiles, where a request has more than 32 rows, take twice as long: three a unit.  (64 requests of 40 rows and 517
+    keys, in segments of 256, 384 and 640 keys: 148, 141, 134; of up to 517: 90, 89, 92; 16 of up to 2,005: 31, 30, 30.)"""
     blocks = requests * kv_heads * ((rows + 63) // 64)
-    of_unit = 3 if rows > 32 else 4 if blocks >= 2 * units else 6
+    of_unit = 1 if not alone else 3 if rows > 32 else 4 if blocks >= 2 * units else 6
     segments = max(1, min((most + 127) // 128, max(of_unit * units // blocks, (most + 1023) // 1024), 256))
     keys = ((most + segments - 1) // segments + 127) // 128 * 128
     return (most + keys - 1) // keys, keys
 
 
-def cut_prefix(columns: int, rows: int, kv_heads: int, shared: int, units: int, own_blocks: int) -> tuple[int, int]:
-    """The same of a shared prompt, whose blocks take `columns` rows each: as many as the device holds at once, one a unit of
-    256 columns or two of 32, segments of 128 keys at least.  Tiles of 32 columns wait for reads, and leave room for up to half as many
-    blocks of the requests' own keys beside them."""
+def cut_prefix(columns: int, rows: int, kv_heads: int, shared: int, units: int, exact: bool) -> tuple[int, int]:
+    """The same of a shared prompt, whose blocks take `columns` rows each, 256 or 32: one a unit, whatever else runs beside them - with more
+    some units have two, and the others wait for those -, segments of 256 keys at least, or of 128 of less than 1,024 that are shared
+    and in float32 (`exact`), whose steps take four times as long.
+    (Tiles of 32 columns, 8 kv heads, whole calls, us: 32,768 shared, 48 rows, 128, 256, 320, 416 and 512 blocks 54, 35, 45, 38, 36; 96
+    rows, 240, 312, 480 48, 62, 46; 8,192 shared, 64 rows, 128, 256, 352, 512 22, 18, 20, 23; 2,048 shared, 64 rows, segments of 128,
+    256, 384 keys 15.7, 13.6, 14.4; of 4 kv heads 512 shared, 8 rows, 11.0, 11.5, 11.5; float32, 2,000
+    shared, segments of 128 and 256 keys 16, 22.)"""
     if shared == 0:
         return 0, 32
     blocks = kv_heads * ((rows + columns - 1) // columns)
-    room = 2 * units - min(own_blocks, units) if columns == 32 else units
-    segments = max(1, min(room // blocks, (shared + 127) // 128, 128))
+    least = 256 if shared >= 1024 and not exact else 128
+    segments = max(1, min(units // blocks, (shared + least - 1) // least, 128))
     keys = ((shared + segments - 1) // segments + 127) // 128 * 128
     return (shared + keys - 1) // keys, keys
 
@@ -171,9 +177,9 @@ class RoundKernels:
         max_new_tokens = min(max_new_tokens, tokens)
         wide = wide_tiles_fit(head_dim, page_size, q.dtype) and (
             self.wide_prefix_tiles if self.wide_prefix_tiles is not None else wide_tiles(tokens * group, kv_heads, shared, self.compute_units))
-        own_segments, own_keys = cut_own(requests, max_new_tokens * group, kv_heads, max_seq_len - shared, self.compute_units)
-        own_blocks = requests * kv_heads * own_segments
-        prefix_segments, prefix_keys = cut_prefix(256 if wide else 32, tokens * group, kv_heads, shared, self.compute_units, own_blocks)
+        own_segments, own_keys = cut_own(requests, max_new_tokens * group, kv_heads, max_seq_len - shared, self.compute_units,
+                                         alone=wide or shared == 0)
+        prefix_segments, prefix_keys = cut_prefix(256 if wide else 32, tokens * group, kv_heads, shared, self.compute_units, q.dtype == torch.float32)
         segments = prefix_segments + own_segments
         # (from torch's pool: a recorded call then has room of its own, and calls on other streams do not meet in one)
         room = torch.empty(segments * tokens * q_heads * (head_dim + 2), dtype=torch.float32, device=self.device)
