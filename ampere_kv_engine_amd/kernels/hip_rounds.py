@@ -31,8 +31,9 @@ def wide_tiles(rows: int, kv_heads: int, shared: int, units: int) -> bool:
     own) rather than of 32 beside the requests' own keys.  The shared ones cost 8 to 10 us more at their start and end and less a column
     and key.  Whole calls, narrow / wide us, 256 units, 64 own keys: 32 heads over 8 of 128, 32,768 shared, 64 rows 38 / 52, 96 49 / 51, 112
     57 / 53; 16,000 shared, 160 rows 42 / 43, 192 49 / 45, 256 57 / 49; 8,192 shared, 256 rows 35 / 42, 320 42 / 42; 2,048 shared, 960 rows
-    36 / 43, 1,280 53 / 46; 16 over 4 of 64, 32,768 shared, 128 rows 24 / 29, 192 33 / 31, 256 40 / 33."""
-    return rows * kv_heads * shared >= 85_000 * units
+    36 / 43, 1,280 53 / 46; 16 over 4 of 64, 32,768 shared, 128 rows 24 / 29, 192 33 / 31, 256 40 / 33.  Two tiles of 32 wait
+    for reads however long the prompt: 131,072 shared, 64 rows 139 / 148, 80 186 / 155."""
+    return rows > 64 and rows * kv_heads * shared >= 85_000 * units
 
 
 def cut_own(requests: int, rows: int, kv_heads: int, most: int, units: int, alone: bool) -> tuple[int, int]:
@@ -65,7 +66,7 @@ def cut_prefix(columns: int, rows: int, kv_heads: int, shared: int, units: int, 
         return 0, 32
     blocks = kv_heads * ((rows + columns - 1) // columns)
     least = 256 if shared >= 1024 and not exact else 128
-    segments = max(1, min(units // blocks, (shared + least - 1) // least, 128))
+    segments = max(1, min(units // blocks, (shared + least - 1) // least, 256))
     keys = ((shared + segments - 1) // segments + 127) // 128 * 128
     return (shared + keys - 1) // keys, keys
 

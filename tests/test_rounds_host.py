@@ -231,7 +231,7 @@ def test_segments_cover_the_keys():
 
 
 def test_wide_tiles_are_for_many_columns_of_long_prompts():
-    assert not hip_rounds.wide_tiles(32, 8, 8192, 256) and hip_rounds.wide_tiles(256, 8, 32768, 256)
+    assert not hip_rounds.wide_tiles(32, 8, 8192, 256) and hip_rounds.wide_tiles(256, 8, 32768, 256) and not hip_rounds.wide_tiles(64, 8, 1 << 20, 256)
     assert hip_rounds.wide_tiles_fit(128, 16, torch.bfloat16) and not hip_rounds.wide_tiles_fit(128, 8, torch.bfloat16)
     assert not hip_rounds.wide_tiles_fit(128, 16, torch.float32) and not hip_rounds.wide_tiles_fit(96, 16, torch.bfloat16)
 
