@@ -176,11 +176,11 @@ __device__ __forceinline__ float sum_over_halves(float v) {
 // TEAMS, which take a tile each (none: `columns` and keys of 0).
 // `row0`: the tile's first row of the kv head's, `columns` how many of the 32 are there.  A column sees the keys below `visible`
 // (its lane's), `all_see` the least of them over the tile.  `wanted`: a bit for each column whose results are written.
-// Reads are what bounds it where there are few columns, each 16 KB of a step asked for a step ahead: own keys of 64 requests, 269 MB, at
-// the card's rate (46 us from memory, 29 where the last-level cache has them); 8 requests behind 8,192 shared tokens, 42 MB in all,
-// 13.6 us, of which 8 are the way to the first keys - launch, page, read - and the results' way back.  With a wave a vector unit and many
-// tiles a step takes 1.4 us: 0.35 of matrix instructions, as much of exponentials, the rest waits for operands whose rows' 32-byte pieces
-// are fetched line by line (`walk_wide` has them in LDS).
+// Reads and their latency are what bounds it where there are few columns, 16 KB a step asked for a step ahead: own keys of 64 requests of
+// 328 each, 86 MB, 19 us (4.5 TB/s), of 4 to 2,048 26 us; 8 requests behind 8,192 shared tokens, 42 MB in all, 13.6 us, of which 8 are the
+// way to the first keys - launch, page, read - and the results' way back.  A block alone on its unit takes 2.8 us a step of its four
+// waves.  With a wave a vector unit and many tiles a step takes 1.4 us: 0.35 of matrix instructions, as much of exponentials, the rest
+// waits for operands whose rows' 32-byte pieces are fetched line by line (`walk_wide` has them in LDS).
 template <typename T, int WAVES, int TEAMS = 1>
 __device__ __forceinline__ void walk(const Args& a, const int* table, int head, long row0, int columns, int first_key, int end_key,
                                      int visible, int all_see, int segment, float* lds, uint32_t wanted = 0xffffffffu) {
@@ -678,6 +678,50 @@ __global__ __launch_bounds__(kWideWaves * kWave, 2) void wide_prefix_kernel(Args
   }
 }
 
+// Sums over the lanes up to each, inside the vector unit: four shifts within rows of 16 lanes, two broadcasts of a row's last lane.
+template <int CTRL, int ROWS> __device__ __forceinline__ int moved(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false); }
+__device__ __forceinline__ int sums_up_to(int v) {
+  v += moved<0x111, 0xf>(v);
+  v += moved<0x112, 0xf>(v);
+  v += moved<0x114, 0xf>(v);
+  v += moved<0x118, 0xf>(v);
+  v += moved<0x142, 0xa>(v);
+  v += moved<0x143, 0xc>(v);
+  return v;
+}
+
+// The `number`-th of the segments that the requests' own keys fill, request by request: the grid has blocks for as many as the longest
+// request may fill in each, and those that are not there come last - between the others they would keep the units from work for a
+// microsecond each (64 requests of 4 to 2,048 keys in segments of 256: 33 -> 27 us; 27 of up to 2,000: 20 -> 15).  False behind the last.
+__device__ __forceinline__ bool own_item(const Args& a, long number, int& request, int& segment, int& begin, int& count, int& length) {
+  const int lane = threadIdx.x & (kWave - 1);
+  if (a.own_segments == 1) {
+    request = static_cast<int>(number);
+    segment = 0;
+    begin = a.q_start[request];
+    count = a.q_start[request + 1] - begin;
+    length = a.seq_lens[request];
+    return within_bounds(a, begin, count, length);
+  }
+  for (int r0 = 0; r0 < a.requests; r0 += kWave) {
+    const int r = min(r0 + lane, a.requests - 1);
+    const int from = a.q_start[r], brings = a.q_start[r + 1] - from, holds = a.seq_lens[r];
+    const int filled = r0 + lane < a.requests && within_bounds(a, from, brings, holds) ? (holds - a.shared + a.own_keys - 1) / a.own_keys : 0;
+    const int upto = sums_up_to(filled), all = __builtin_amdgcn_readlane(upto, kWave - 1);
+    if (number < all) {
+      const int at = __builtin_ctzll(__ballot(upto > number));
+      request = r0 + at;
+      segment = static_cast<int>(number) - __builtin_amdgcn_readlane(upto - filled, at);
+      begin = __builtin_amdgcn_readlane(from, at);
+      count = __builtin_amdgcn_readlane(brings, at);
+      length = __builtin_amdgcn_readlane(holds, at);
+      return true;
+    }
+    number -= all;
+  }
+  return false;
+}
+
 // Blocks 0 .. prefix_blocks - 1 take (segment and head, tile) of the prefix, the others (request, head, two tiles, segment) of the
 // requests' own keys.
 template <typename T>
@@ -698,13 +742,10 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 || D > 128 ? 1 : 2)) void
   } else {
     block -= a.prefix_blocks;
     tile_of(block, static_cast<long>(a.requests) * a.kv_heads * a.own_segments, (a.own_tiles + 1) / 2, item, tile);
-    // (segments last: with them first, every eighth block - one XCD's - would be of the segments that short requests do not have)
     head = static_cast<int>(item % a.kv_heads);
-    item /= a.kv_heads;
-    request = static_cast<int>(item % a.requests);
-    segment = static_cast<int>(item / a.requests);
-    const int begin = a.q_start[request], count = a.q_start[request + 1] - begin, length = a.seq_lens[request], before = length - count;
-    if (!within_bounds(a, begin, count, length)) return;
+    int begin, count, length;
+    if (!own_item(a, item / a.kv_heads, request, segment, begin, count, length)) return;
+    const int before = length - count;
     const int group = static_cast<int>(a.group.by), left = count * group - 64 * tile;
     if (left <= 0) return;
     // two tiles, where a request brings them, for half of the waves each: what one reads the other finds in the unit's cache (64 requests

@@ -36,21 +36,18 @@ def wide_tiles(rows: int, kv_heads: int, shared: int, units: int) -> bool:
     return rows > 64 and rows * kv_heads * shared >= 85_000 * units
 
 
-def cut_own(requests: int, rows: int, kv_heads: int, most: int, units: int, alone: bool) -> tuple[int, int]:
+def cut_own(requests: int, rows: int, kv_heads: int, most: int, units: int) -> tuple[int, int]:
     """(segments, keys of one) of up to `most` keys that a request of up to `rows` rows a kv head holds behind the prompt.  What a block waits
-    for at its start and end is a good part of its time, but a long request's keys are not to outlast the others': no segment of more than
-    about a thousand keys, nor of fewer than 128, a step for each of a block's waves.  Beside the prompt's blocks, of which a unit has
-    one, one more a unit.  (8 kv heads, whole calls, us, equal lengths / up to that: 8 requests of 1,000 keys, 128, 256 and 512 blocks 23 /
-    22, 21 / 19, 25 / 24; 16 of 600, 256, 384, 640 blocks 20 / 19, 23 / 18, 25 / 21; 27 of 2,000, 432, 864, 1,728 blocks 47 / 30, 50 /
-    32, 53 / 30; 64 of 517, 512, 1,024, 1,536 blocks 47 / 40, 50 / 38, 55 / 38.)
-    `alone`, in a launch of their own: four a unit, which holds two, or six where not even those two are there without a cut.  (Two,
-    three, four and six a unit: 64 requests of 517 keys 112, 111, 115, 124; 64 of 2,053 128, 127, 127, 132; 27 of up to 2,005 72, 71,
-    73, 69.)  Blocks of two tiles, where a request has more than 32 rows, take twice as long: three a unit.  (64 requests of 40 rows and 517
-    keys, in segments of 256, 384 and 640 keys: 148, 141, 134; of up to 517: 90, 89, 92; 16 of up to 2,005: 31, 30, 30.)"""
+    for at its start and end is a good part of its time, but a long request's keys are not to outlast the others': segments of 128 keys, a
+    step for each of a block's waves, while they find a unit each, of 256 while those do, of 384 beyond, and the whole up to half as
+    much again.  (8 kv heads, whole calls, us, equal lengths / up to that, segments of 128, 256, 384, 512 and about 1,000 keys: 8 requests of
+    256 keys 17.3 / 16.8, 18.5 / 18.2, 20.5 / 19.7; 8 of 1,000 26 / 18, 21 / 19, 21 / 20, 22 / 22, 27 / 27; 16 of 600 25 / 18, 24 / 18,
+    20 / 19, 21 / 20; 64 of 1,000 87 / 37, 66 / 32, 62 / 33, 64 / 34, 58 / 39; in a launch of their own 64 of 2,048 213 / 94, 187 / 81,
+    179 / 79, 179 / 82, 179 / 89; 27 of 2,000 with up to 25 rows 145 / 68, 124 / 63, 124 / 64, 117 / 63, 111 / 67; of one segment 64 of
+    500, 512 keys 39 / 30 and 384 40 / 29; with 40 rows 133 / 92 and 145 / 85.)"""
     blocks = requests * kv_heads * ((rows + 63) // 64)
-    of_unit = 1 if not alone else 3 if rows > 32 else 4 if blocks >= 2 * units else 6
-    segments = max(1, min((most + 127) // 128, max(of_unit * units // blocks, (most + 1023) // 1024), 256))
-    keys = ((most + segments - 1) // segments + 127) // 128 * 128
+    keys = 128 if blocks * ((most + 127) // 128) <= units else 256 if blocks * ((most + 255) // 256) <= units else 384 if most > 576 else most
+    keys = (max(keys, (most + 255) // 256) + 127) // 128 * 128
     return (most + keys - 1) // keys, keys
 
 
@@ -178,8 +175,7 @@ class RoundKernels:
         max_new_tokens = min(max_new_tokens, tokens)
         wide = wide_tiles_fit(head_dim, page_size, q.dtype) and (
             self.wide_prefix_tiles if self.wide_prefix_tiles is not None else wide_tiles(tokens * group, kv_heads, shared, self.compute_units))
-        own_segments, own_keys = cut_own(requests, max_new_tokens * group, kv_heads, max_seq_len - shared, self.compute_units,
-                                         alone=wide or shared == 0)
+        own_segments, own_keys = cut_own(requests, max_new_tokens * group, kv_heads, max_seq_len - shared, self.compute_units)
         prefix_segments, prefix_keys = cut_prefix(256 if wide else 32, tokens * group, kv_heads, shared, self.compute_units, q.dtype == torch.float32)
         segments = prefix_segments + own_segments
         # (from torch's pool: a recorded call then has room of its own, and calls on other streams do not meet in one)

@@ -133,6 +133,8 @@ SHAPES = [
     (16, 4, 128, 16, 1600, tuple(3 + 5 * i for i in range(40)), (1,) * 40),
     (2, 2, 64, 16, 160, (70,), (64,)),                   # the first tile sees nothing of the last segment, the second does
     (16, 2, 256, 16, 128, (9, 40), (5, 6)),
+    # several segments of more requests than lanes, some that bring nothing
+    (2, 1, 16, 8, 64, tuple(0 if i % 3 else 5 * i for i in range(150)), tuple((2 * i) % 3 for i in range(150))),
 ]
 
 

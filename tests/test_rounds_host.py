@@ -222,8 +222,8 @@ def test_segments_cover_the_keys():
     for _ in range(3000):
         requests, kv_heads, rows = rng.choice((1, 2, 7, 64, 500)), rng.choice((1, 2, 8, 32)), rng.choice((1, 4, 40, 900, 20000))
         most, shared = rng.choice((1, 5, 127, 128, 129, 2000, 131072)), rng.choice((0, 8, 16, 512, 8192, 131072))
-        own_segments, own_keys = hip_rounds.cut_own(requests, min(rows, 600), kv_heads, most, 256, rng.random() < 0.5)
-        assert own_keys % 32 == 0 and (own_segments - 1) * own_keys < most <= own_segments * own_keys
+        own_segments, own_keys = hip_rounds.cut_own(requests, min(rows, 600), kv_heads, most, 256)
+        assert own_segments <= 256 and own_keys % 32 == 0 and (own_segments - 1) * own_keys < most <= own_segments * own_keys
         for columns in (32, 256):
             segments, keys = hip_rounds.cut_prefix(columns, rows, kv_heads, shared, 256, rng.random() < 0.5)
             assert keys % 32 == 0 and segments * keys >= shared and (segments == 0 if shared == 0 else (segments - 1) * keys < shared)
