@@ -777,7 +777,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 || D > 128 ? 1 : 2)) void
 // A row - (token, query head) - a wave, four of a token a block, or, SHARE, where there are too few rows to fill the device, a block: its
 // waves then take the segments in turn.  What a row waits for is a chain of reads - whose the token is, what it sees -, so many
 // short waves run beside each other, and the segments that a row is sure to have are on their way meanwhile (20,480 rows of four segments
-// 13.9 -> 12.2 us, 43 MB read and 5 written; 2,048 rows of up to 41: 9.2 us for 43 MB).
+// 13.9 -> 12.2 us, 43 MB read and 5 written; 2,048 rows of 33 to 38: 8.8 us for 36 MB).
 template <typename T, bool SHARE>
 __global__ __launch_bounds__(kThreads) void join_kernel(Args a) {
   constexpr int kEach = (D + kWave - 1) / kWave;                // dims of a lane, kEach in a row (the last lanes may have none)
