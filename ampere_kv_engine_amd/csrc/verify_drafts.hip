@@ -379,30 +379,46 @@ __global__ __launch_bounds__(kChooseThreads) void choose_kernel(Verify a) {
   const double inverse = drawn ? 1.0 / static_cast<double>(t) : 1.0;
   const Part* parts = a.parts + static_cast<size_t>(request) * (2 * a.places - 1) * a.part_count;
   const int drafts = a.draft != nullptr && drawn ? rows - 1 : 0;
-  for (int i = wave; i < rows + drafts; i += kWaves) {
+  auto part_of = [&](int i) {
     Part part{0.0, -INFINITY, 0x7fffffff, 0, 0};
-    if (lane < a.part_count) part = parts[static_cast<size_t>(i < rows ? i : a.places + i - rows) * a.part_count + lane];
+    if (i < rows + drafts && lane < a.part_count) part = parts[static_cast<size_t>(i < rows ? i : a.places + i - rows) * a.part_count + lane];
+    return part;
+  };
+  // (what place `tid`'s draft is decided by, and the rows' parts, are on their way together)
+  const float last_number = a.uniforms[static_cast<size_t>(request) * a.places + a.places - 1];
+  Part ahead = part_of(wave);
+  int drafted = -1;
+  float its_logit = 0.f, its_draft_logit = 0.f, its_number = 0.f;
+  if (tid < rows - 1) {
+    drafted = a.tokens[first + tid + 1];
+    if (drawn && drafted >= 0 && drafted < a.vocab) {
+      its_number = a.uniforms[static_cast<size_t>(request) * a.places + tid];
+      its_logit = a.logits[static_cast<size_t>(first + tid) * a.vocab + drafted];
+      if (a.draft != nullptr) its_draft_logit = a.draft[request * a.draft_request + tid * a.draft_place + drafted];
+    }
+  }
+  for (int i = wave; i < rows + drafts; i += kWaves) {
+    const Part part = ahead;
+    ahead = part_of(i + kWaves);
     const Row row = gather_row(part, inverse, drawn);
     if (lane == 0) (i < rows ? target[i] : draft[i - rows]) = row;
   }
   __syncthreads();
   if (tid < rows - 1) {                                   // place `tid`'s draft: kept if all before it are
-    const int id = a.tokens[first + tid + 1];
     const Row row = target[tid];
     bool keep = false;
-    if (row.fine && id >= 0 && id < a.vocab) {
+    if (row.fine && drafted >= 0 && drafted < a.vocab) {
       if (!drawn) {
-        keep = row.best == id;
+        keep = row.best == drafted;
       } else {
-        const double p = exp_of((static_cast<double>(a.logits[static_cast<size_t>(first + tid) * a.vocab + id]) - row.top) * inverse) / row.sum;
+        const double p = exp_of((static_cast<double>(its_logit) - row.top) * inverse) / row.sum;
         double q = 1.0;
         bool known = true;
         if (a.draft != nullptr) {
           known = draft[tid].fine;
-          const float x = a.draft[request * a.draft_request + tid * a.draft_place + id];
-          q = exp_of((static_cast<double>(x) - draft[tid].top) * inverse) / draft[tid].sum;
+          q = exp_of((static_cast<double>(its_draft_logit) - draft[tid].top) * inverse) / draft[tid].sum;
         }
-        keep = known && static_cast<double>(a.uniforms[static_cast<size_t>(request) * a.places + tid]) * q < p;
+        keep = known && static_cast<double>(its_number) * q < p;
       }
     }
     fine[tid] = keep;
@@ -505,8 +521,7 @@ __global__ __launch_bounds__(kChooseThreads) void choose_kernel(Verify a) {
     total = of_lane(upto, kWave - 1);
   }
   // (a number of 1 or more is the end of the line whatever the sums' last bits say)
-  const float number = a.uniforms[static_cast<size_t>(request) * a.places + a.places - 1];
-  const double goal = number < 1.f ? static_cast<double>(number) * total : INFINITY;
+  const double goal = last_number < 1.f ? static_cast<double>(last_number) * total : INFINITY;
   // the first lane with weight whose sum lies beyond the goal, or the last lane with weight
   auto lane_of = [&](double value, double sum) {
     const unsigned long long some = __ballot(value > kLeast), beyond = __ballot(value > kLeast && sum > goal);
