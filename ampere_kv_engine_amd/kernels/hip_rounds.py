@@ -71,7 +71,8 @@ def cut_prefix(columns: int, rows: int, kv_heads: int, shared: int, units: int, 
 class RoundKernels:
     """Mixed into `HipKernels` (which provides `_dense`, `_check`, `_pages`, `_stream`, `device`)."""
 
-    wide_prefix_tiles = None        # a shared prompt's keys for tiles of 256 columns, where heads and pages allow it: None = by the sizes
+    # a shared prompt's keys for tiles of 256 columns, whose weights are rounded once, where heads and pages allow it: None = by the sizes
+    wide_prefix_tiles = None
     _rounds_lib = None
 
     def _rounds(self):
@@ -129,7 +130,7 @@ class RoundKernels:
 
     # ---- attention -----------------------------------------------------------------------------------------------------
     def attention_shared_prefix(self, q, k_pages, v_pages, block_table, q_start, seq_lens, shared, q_heads, kv_heads, head_dim, scale, out,
-                                max_seq_len, max_new_tokens, rows=None):
+                                max_seq_len, max_new_tokens, rows=None, two_part_weights=False):
         """Attention of requests whose first `shared` tokens (a multiple of the page size; 0: none) lie in the same pages: those
         are read once for all of them, so that many requests cost little more than one.  q, out [tokens, q_heads * head_dim]:
         encoded queries, request by request, whose keys and values are in the pages already.  q_start [requests + 1]: a request's
@@ -138,6 +139,11 @@ class RoundKernels:
         more than `max_seq_len` tokens or brings more than `max_new_tokens` (0 is fine, and any number from there on; prompts of
         thousands of tokens are `attention`'s).
         float32 or bfloat16; head sizes as `check_attention_sizes` has them; pages of 8 tokens or more, a power of two.
+        bfloat16: softmax weights are multiplied in two bfloat16 parts, the rounded one and what the rounding left, as `attention` does -
+        but the weights of a prompt whose keys go in tiles of 256 columns (heads of 64 and 128, pages of 16 and more, from
+        the rows and keys on that `wide_tiles` says) are rounded once, by up to 2^-8 of each: what a request gets there is off by 0.0023 of the
+        output's largest in place of 0.0017, of which 0.0016 is the output's own rounding, and which of both it is depends on the batch.
+        `two_part_weights`: in two parts whatever the batch, in tiles of 32 columns.
         A token gets NaN where its request's table (or the first one's, of the prompt) names a page outside the pool or is no row of
         block_table, where its request exceeds the bounds, or where it stands within the
         prompt.  Rows of `out` behind the last request's are left as they are."""
@@ -173,7 +179,7 @@ class RoundKernels:
             raise self._error("there are no pages")
         group = q_heads // kv_heads
         max_new_tokens = min(max_new_tokens, tokens)
-        wide = wide_tiles_fit(head_dim, page_size, q.dtype) and (
+        wide = not two_part_weights and wide_tiles_fit(head_dim, page_size, q.dtype) and (
             self.wide_prefix_tiles if self.wide_prefix_tiles is not None else wide_tiles(tokens * group, kv_heads, shared, self.compute_units))
         own_segments, own_keys = cut_own(requests, max_new_tokens * group, kv_heads, max_seq_len - shared, self.compute_units)
         prefix_segments, prefix_keys = cut_prefix(256 if wide else 32, tokens * group, kv_heads, shared, self.compute_units, q.dtype == torch.float32)
