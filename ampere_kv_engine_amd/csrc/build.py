@@ -35,6 +35,7 @@ ROUNDS_LIBRARY = "libakv_rounds.so"
 SHARED_PREFIX_SOURCE = "shared_prefix.hip"     # compiled once per head size as well
 ATTENTION_SOURCE = "attention_mfma.hip"        # compiled once per head size, into its own small library
 DEFAULT_HEAD_DIMS = (16, 32, 48, 64, 80, 96, 128, 192, 256)
+SHARED_PREFIX_HEAD_DIMS = (16, 32, 48, 64, 80, 96, 128, 160, 176, 192, 256)
 ARCH = "gfx950"
 # packed-fp32 instructions are switched off for all device code of this library
 FLAGS = ("-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-Xclang", "-target-feature", "-Xclang",
@@ -297,12 +298,12 @@ def ensure_shared_prefix(head_dim: int, verbose: bool = True) -> str:
     return shared_prefix_library_path(head_dim) or build_shared_prefix(head_dim, verbose)
 
 
-def build_all(head_dims=DEFAULT_HEAD_DIMS, verbose: bool = True) -> list[str]:
+def build_all(head_dims=DEFAULT_HEAD_DIMS, verbose: bool = True, shared_prefix_head_dims=SHARED_PREFIX_HEAD_DIMS) -> list[str]:
     """The kernel libraries and the attention libraries of the usual head sizes."""
     paths = [build(verbose), build_parts(verbose), build_rounds(verbose)]
     with ThreadPoolExecutor(max_workers=4) as pool:
         paths += list(pool.map(lambda d: build_attention(d, verbose), head_dims))
-        paths += list(pool.map(lambda d: build_shared_prefix(d, verbose), head_dims))
+        paths += list(pool.map(lambda d: build_shared_prefix(d, verbose), shared_prefix_head_dims))
     return paths
 
 

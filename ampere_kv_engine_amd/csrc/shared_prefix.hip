@@ -780,7 +780,8 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 || D > 128 ? 1 : 2)) void
 // 13.9 -> 12.2 us, 43 MB read and 5 written; 2,048 rows of 33 to 38: 8.8 us for 36 MB).
 template <typename T, bool SHARE>
 __global__ __launch_bounds__(kThreads) void join_kernel(Args a) {
-  constexpr int kEach = (D + kWave - 1) / kWave;                // dims of a lane, kEach in a row (the last lanes may have none)
+  constexpr int kEach = D <= kWave ? 1 : D <= 2 * kWave ? 2 : 4;    // dims of a lane, kEach in a row (the last lanes may have none)
+  static_assert(D % kEach == 0 && D / kEach <= kWave, "a lane's dims lie in its head, all of them or none");   // (three would not: 160, 176)
   constexpr int kStride = SHARE ? kWaves : 1;
   __shared__ float shares[SHARE ? kWaves : 1][kEach * kWave];
   const int token = blockIdx.x, lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;

@@ -1,7 +1,12 @@
 """What the calls of a drafted round promise at their limits, on the CPU: the library replaced by a recorder."""
 
+import os
+import subprocess
+from concurrent.futures import ThreadPoolExecutor
+
 import torch
 
+from ampere_kv_engine_amd.csrc import build
 from test_rounds_host import Recorder, attention
 
 
@@ -18,3 +23,16 @@ def test_the_caller_says_whether_weights_are_rounded_once():
     kernels.wide_prefix_tiles = True
     kernels.attention_shared_prefix(**arguments, two_part_weights=True)
     assert kernels.calls[-1][-2] == 0
+
+
+def test_every_head_size_compiles():
+    """What is asserted of a head size when it is compiled (that a lane's dims of the join lie in one head) holds for all that are taken."""
+    source = os.path.join(build.HERE, build.SHARED_PREFIX_SOURCE)
+
+    def compiled(dim):
+        return subprocess.run([build._hipcc(), *build.FLAGS, f"-DAKV_HEAD_DIM={dim}", "--cuda-host-only", "-fsyntax-only", source],
+                              capture_output=True, text=True)
+
+    with ThreadPoolExecutor(max_workers=8) as pool:
+        for result in pool.map(compiled, range(16, 257, 16)):
+            assert result.returncode == 0, result.stderr
