@@ -66,11 +66,16 @@ __global__ __launch_bounds__(kThreads) void place_kernel(Place p) {
   if (p.rows != nullptr)
     for (int i = tid; i < p.hash_places; i += kThreads) rows_seen[i] = -1;
   __syncthreads();
+  // Whether a request brings places of the prompt's own pages.  That is how a prompt is written - by requests of a batch none of which
+  // has it yet, a place by one of them at most; beside a request that has pages or starts behind the prompt (8) it would be written over.
+  const long prompt_end = static_cast<long>(p.prefix_count) * p.page_size;
+  auto writes_prompt = [&](bool fresh, int length, int brings) { return fresh && brings > 0 && length < prompt_end; };
   long tokens_before = 0, pages_before = 0;
   for (int r0 = 0; r0 < n; r0 += kThreads) {
     const int r = r0 + tid;
     long count = 0, taken = 0;
-    int fault = 0;           // 1 a length or count that cannot be, 2 a table row that is too narrow, not there or named twice
+    // 1 a length or count that cannot be, 2 a table row that is too narrow, not there or named twice; 4 and 8: see `writes_prompt`
+    int fault = 0;
     if (r < n) {
       const int length = p.lengths[r], held = p.held[r], brings = p.counts[r];
       const int row = p.rows != nullptr ? p.rows[r] : r;
@@ -85,6 +90,8 @@ __global__ __launch_bounds__(kThreads) void place_kernel(Place p) {
         if (had < old + (p.page.rest(length, old) != 0 ? 1 : 0)) fault = 1;
         count = brings;
         taken = max(0, need - had);
+        if (writes_prompt(held == 0, length, brings)) fault |= 4;
+        else if (held != 0 || brings != 0) fault |= 8;
         if (row < 0 || row >= p.table_rows || had + taken > p.table_width) {
           fault |= 2;
         } else if (p.rows != nullptr) {
@@ -117,9 +124,24 @@ __global__ __launch_bounds__(kThreads) void place_kernel(Place p) {
     __syncthreads();
   }
   int verdict = pages_before > 0x7fffffffL ? -1 : static_cast<int>(pages_before);
-  if ((wrong & 1) != 0) verdict = -4;
+  const int faults = wrong;
+  bool meet = (faults & 12) == 12;
+  if ((faults & 13) == 4 && tokens_before <= p.tokens) {     // (a request's tokens lie in LDS as a difference)
+    if (tid == 0) first_token[n] = static_cast<int>(tokens_before);
+    __syncthreads();
+    for (int r = tid; r < n && !meet; r += kThreads) {
+      const int brings = first_token[r + 1] - first_token[r], from = length_of[r];
+      if (!writes_prompt(had_of[r] < 0, from, brings)) continue;
+      for (int other = 0; other < r && !meet; ++other) {
+        const int its = first_token[other + 1] - first_token[other], at = length_of[other];
+        meet = writes_prompt(had_of[other] < 0, at, its) && max(from, at) < min(prompt_end, min(from + static_cast<long>(brings), at + static_cast<long>(its)));
+      }
+    }
+    meet = __syncthreads_or(meet);
+  }
+  if ((faults & 1) != 0 || meet) verdict = -4;
   else if (tokens_before > p.tokens) verdict = -3;
-  else if ((wrong & 2) != 0) verdict = -2;
+  else if ((faults & 2) != 0) verdict = -2;
   else if (cursor < 0 || cursor + pages_before > p.free_count) verdict = -1;
   if (blockIdx.x == 0 && tid == 0) {
     p.status[0] = verdict;
@@ -179,7 +201,8 @@ extern "C" int akv_place_most_requests() { return kMost; }
 
 // `status` [1]: the pages taken, or why nothing but `status` was written: -1 too few free pages, -2 a request's row is not in the
 // table, too narrow for its pages or another request's too, -3 more tokens than the maps have room for, -4 a negative length, count or
-// number of pages, or a request that holds fewer pages than its length fills.  No output may lie in an input but `table`, whose entries below a request's
+// number of pages, a request that holds fewer pages than its length fills, or one that would write into a prompt that another one of the batch has
+// or writes as well.  No output may lie in an input but `table`, whose entries below a request's
 // pages are read and never written.
 extern "C" int akv_place_tokens(const int* lengths, const int* counts, const int* held, const int* free_pages, long free_count,
                                 const int* cursor, int* table, const int* rows, int table_rows, int table_width, int page_size,

@@ -247,12 +247,16 @@ class RoundKernels:
         """A step's layout from lengths on the device (all int32).  lengths, counts, held [requests]: the tokens a request holds, those it
         brings, and its pages.  It takes the pages it lacks from free_pages[cursor ...], in the requests' order; they are entered into its
         row of `table` (row r, or rows[r]), and held_after [requests] and cursor_after [1] say what is held and taken then.  A request
-        that holds no page starts on `prefix_pages`, if they are given: they are entered too, and `lengths` counts their tokens
-        (all of them: what a request brings within shared pages would be written into them).
+        that holds no page starts on `prefix_pages`, if they are given: they are entered too, and `lengths` counts their tokens.  What it
+        brings at places within them is written into them: so a prompt is filled, by a batch none of whose requests has it yet, a place
+        by one request at most - other batches are refused (-4), those outside the batch nobody sees.  (A request that is to have no
+        part of the prompt goes into a call without prefix_pages.)
         q_start [requests + 1], seq_lens [requests] (the tokens held after the step); positions, seq_of_token and slot_map [tokens]: of
         every token, request by request; tokens are all that the requests bring, or more: entries behind the last are left as they are.
         status [1]: the pages taken, or, with nothing else written, -1 too few free pages, -2 a row that the table does not have, that is too
-        narrow or that two requests name, -3 more tokens than the maps have room for, -4 a negative number, or fewer pages than a length fills."""
+        narrow or that two requests name, -3 more tokens than the maps have room for, -4 a negative number, fewer pages than a length
+        fills, or a request that brings places of the prompt's pages beside one that has pages, starts behind the prompt or brings the same
+        places."""
         requests, tokens = lengths.shape[0], positions.shape[0]
         lib = self._rounds()
         free = free_pages.shape[0]

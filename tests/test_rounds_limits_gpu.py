@@ -5,7 +5,7 @@ from types import SimpleNamespace
 import pytest
 import torch
 
-from test_rounds_gpu import attend, batch, kernel_set, kernels, tiled, within  # noqa: F401  (fixtures among them)
+from test_rounds_gpu import attend, batch, kernel_set, kernels, place_both, tiled, within  # noqa: F401  (fixtures among them)
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -36,3 +36,29 @@ def test_heads_of_every_width_stay_in_their_places(kernels, dtype, dim, rows):
     counts = (2, 1, 2) if rows == 5 else (4,) * 75
     case = batch(dtype, 8 if rows == 5 else 16, 2 if rows == 5 else 8, dim, 16, 64, tuple(3 * i % 40 for i in range(len(counts))), counts, seed=71)
     within_surroundings(kernels, case)
+
+
+# ---- a step's layout --------------------------------------------------------------------------------------------------------
+
+PROMPT = [7, 901, 33]           # three pages of sixteen tokens
+
+
+@pytest.mark.parametrize("lengths,counts,held", [
+    ((48, 0), (1, 3), (0, 0)), ((0, 48), (3, 1), (0, 0)),       # a request without tokens beside one that starts behind the prompt
+    ((70, 0), (1, 3), (5, 0)), ((47, 70), (1, 0), (0, 5)),      # the same beside one that holds pages
+    ((0, 0), (3, 2), (0, 0)), ((0, 2), (3, 2), (0, 0)), ((5, 0), (1, 60), (0, 0)),      # two that bring the same places
+])
+def test_nobody_writes_into_a_prompt_that_others_have(kernels, lengths, counts, held):
+    assert place_both(kernels, lengths, counts, held, 16, prefix=PROMPT) == -4
+    assert place_both(kernels, lengths, counts, held, 16, prefix=PROMPT, rows=[4, 1], table_rows=5) == -4
+
+
+def test_a_prompt_is_written_where_nobody_has_it_yet(kernels):
+    assert place_both(kernels, [0], [60], [0], 16, prefix=PROMPT) == 1
+    assert place_both(kernels, [0, 3, 40], [3, 30, 8], [0, 0, 0], 16, prefix=PROMPT) == 0
+    assert place_both(kernels, [48, 0, 70], [1, 0, 2], [0, 0, 5], 16, prefix=PROMPT) == 1        # one that brings nothing
+    prompt = list(range(50, 175))
+    lengths = torch.randperm(2000, generator=torch.Generator().manual_seed(3))[:1500].tolist()
+    assert place_both(kernels, lengths, [1] * 1500, [0] * 1500, 16, prefix=prompt) == 0
+    lengths[1400] = lengths[3]
+    assert place_both(kernels, lengths, [1] * 1500, [0] * 1500, 16, prefix=prompt) == -4
