@@ -192,7 +192,8 @@ __device__ __forceinline__ void walk(const Args& a, const int* table, int head, 
   const int page_mask = (1 << a.page_shift) - 1;
   // in LDS: half the waves' results, a row a column; every wave's maxima and sums; what a column sees; the queries, as operands
   float* shares = lds + kBuffers * 32 * kRow;         // [waves][32][2]
-  int* seen = reinterpret_cast<int*>(shares + WAVES * 32 * 2);      // [32], and whether a masked value was not finite
+  // [32], whether a masked value was not finite, a bit for each column without a result (its sum of weights is NaN)
+  int* seen = reinterpret_cast<int*>(shares + WAVES * 32 * 2);
   Piece<T>* queries = reinterpret_cast<Piece<T>*>(seen + 64);       // [KC][lane]
   // the key of a step that this lane's row of A holds
   const int key_at = 16 * (r >> 4) + 8 * ((r >> 2) & 1) + 4 * ((r >> 3) & 1) + (r & 3);
@@ -329,8 +330,12 @@ __device__ __forceinline__ void walk(const Args& a, const int* table, int head, 
 #pragma unroll
   for (int w = 0; w < WAVES; ++w) top = fmaxf(top, shares[(w * 32 + r) * 2]);
   const float reference = top == -INFINITY ? 0.f : top;
+  if (wave == 0) {      // (which hands on nothing in the first turn below)
 #pragma unroll
-  for (int w = 0; w < WAVES; ++w) whole += shares[(w * 32 + r) * 2 + 1] * __builtin_amdgcn_exp2f(shares[(w * 32 + r) * 2] - reference);
+    for (int w = 0; w < WAVES; ++w) whole += shares[(w * 32 + r) * 2 + 1] * __builtin_amdgcn_exp2f(shares[(w * 32 + r) * 2] - reference);
+    const unsigned long long lost = __ballot(whole != whole);
+    if (lane == 0) seen[33] = static_cast<int>(lost);
+  }
   const float by = __builtin_amdgcn_exp2f(m - reference);
   float* mine = lds + ((wave % kBuffers) * 32 + r) * kRow;
 #pragma unroll
@@ -363,15 +368,26 @@ __device__ __forceinline__ void walk(const Args& a, const int* table, int head, 
     floatx4 sum = *reinterpret_cast<const floatx4*>(lds + column * kRow + at);
 #pragma unroll
     for (int w = 1; w < kBuffers; ++w) sum += *reinterpret_cast<const floatx4*>(lds + (w * 32 + column) * kRow + at);
-    if (any_odd)      // (any weight times such a value is the same; only keys that some column does not see were looked at)
-      for (int j = first_key + (max(0, all_see - first_key) & ~31); j < min(end_key, seen[column]); ++j) {
+    // A value that is not finite makes the sum what it is itself, however small its weight.  The product does not: 0 times it is NaN, where the
+    // weight is less than 32 bits hold or its second part is nothing, and so is what a negative second part takes from infinity.  So where a
+    // sum is not finite such values are looked for among all keys, and else among those that were left out of the product.
+    bool finite = true;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) finite = finite && fabsf(sum[e]) < INFINITY;
+    if ((any_odd || !finite) && ((seen[33] >> column) & 1) == 0) {
+      floatx4 odd = {0.f, 0.f, 0.f, 0.f};
+      for (int j = finite ? first_key + (max(0, all_see - first_key) & ~31) : first_key; j < min(end_key, seen[column]); ++j) {
         const size_t place = place_of(table[j >> a.page_shift]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float v = to_float(static_cast<const T*>(a.v_pages)[((place * D + at + e) << a.page_shift) + (j & page_mask)]);
-          if (!(fabsf(v) < INFINITY)) sum[e] += v;
+          if (!(fabsf(v) < INFINITY)) odd[e] += v;
         }
       }
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (odd[e] != 0.f) sum[e] = odd[e];
+    }
     *reinterpret_cast<floatx4*>(sums + static_cast<size_t>(column) * D + at) = sum;
   }
 }
@@ -384,8 +400,8 @@ __device__ __forceinline__ void walk(const Args& a, const int* table, int head, 
 // A turn multiplies the scores of step u + 1 (32 keys), turns those of step u into weights and adds the values of step u - 1: the three
 // do not wait for each other, and nothing in it depends on what the scores are.  A column's weights are taken below a fixed point,
 // the maximum of the segment's first step, and may grow: bfloat16 and float32 reach to 2^127, and a sum that is divided by another of the
-// same scale loses nothing.  Where a column's weights pass 2^40, or there is no such point (nothing but minus infinity, a NaN), the column
-// is done again by `walk`, which keeps a running maximum: what a column gets hangs on nothing beside it.  (A branch that moves the point in
+// same scale loses nothing.  Where a column's weights pass 2^40, its sums are not finite, or there is no such point (nothing but minus
+// infinity, a NaN), the column is done again by `walk`, which keeps a running maximum: what a column gets hangs on nothing beside it.  (A branch that moves the point in
 // the loop costs it half as much again: the compiler then keeps the sums in two sets of registers.)
 // The weights are rounded to bfloat16, once: a second part would cost half the matrix instructions again, and the sum that they are
 // divided by is the sum of the rounded ones, so that what is left is the error of an average over the keys.
@@ -628,6 +644,13 @@ __device__ __forceinline__ void walk_wide(const Args& a, const int* table, int h
   over |= !(sum <= kLimit);
   l += sum;
   add_values(stage, second_step, weights[0], there < 32 ? 1 : 2);
+  // (a column whose sums are not finite is done again too: its weights may be above one, and values may be infinite)
+  float nothing = 0.f;
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) nothing = fmaf(o[t][i], 0.f, nothing);
+  over |= nothing != 0.f;
   l = sum_over_halves(l);
   const unsigned long long passed = __ballot(over && my_row < rows);
   const uint32_t mask = static_cast<uint32_t>(passed) | static_cast<uint32_t>(passed >> 32);
@@ -783,6 +806,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Args a) {
   constexpr int kEach = D <= kWave ? 1 : D <= 2 * kWave ? 2 : 4;    // dims of a lane, kEach in a row (the last lanes may have none)
   static_assert(D % kEach == 0 && D / kEach <= kWave, "a lane's dims lie in its head, all of them or none");   // (three would not: 160, 176)
   constexpr int kStride = SHARE ? kWaves : 1;
+  constexpr float kLittle = 0x1p-126f;      // (a segment that is worth less is taken as that: its sum may be infinite, and 0 times it a NaN)
   __shared__ float shares[SHARE ? kWaves : 1][kEach * kWave];
   const int token = blockIdx.x, lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   const int q_head = SHARE ? blockIdx.y : blockIdx.y * kWaves + wave;
@@ -831,7 +855,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Args a) {
       if (i0 + lane >= used) one = float2{-INFINITY, 0.f};
       const float m = fmaxf(top, wave_max(one.x)), reference = m == -INFINITY ? 0.f : m;
       if (i0 != 0) {                                            // (more segments than lanes: what is there already goes along)
-        const float by = __builtin_amdgcn_exp2f(top - reference);
+        const float by = fmaxf(__builtin_amdgcn_exp2f(top - reference), kLittle);
         total *= by;
 #pragma unroll
         for (int e = 0; e < kEach; ++e) sum[e] *= by;
@@ -843,7 +867,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Args a) {
       auto add = [&](int from, int end) {
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-          const float by = __shfl(weight, min(from + u * kStride, end - 1) - i0, kWave);
+          const float by = fmaxf(__shfl(weight, min(from + u * kStride, end - 1) - i0, kWave), kLittle);
           if (from + u * kStride < end) {
 #pragma unroll
             for (int e = 0; e < kEach; ++e) sum[e] = fmaf(by, fetched[u][e], sum[e]);

@@ -1,5 +1,6 @@
 """The operators of a drafted round at their limits, on the GPU."""
 
+import math
 from types import SimpleNamespace
 
 import pytest
@@ -36,6 +37,56 @@ def test_heads_of_every_width_stay_in_their_places(kernels, dtype, dim, rows):
     counts = (2, 1, 2) if rows == 5 else (4,) * 75
     case = batch(dtype, 8 if rows == 5 else 16, 2 if rows == 5 else 8, dim, 16, 64, tuple(3 * i % 40 for i in range(len(counts))), counts, seed=71)
     within_surroundings(kernels, case)
+
+
+def put_value(case, request, position, kv_head, dim, value):
+    """At one dim of a token's value; position counts from the request's first token, the prompt's among them."""
+    page = case["page"]
+    case["v"][int(case["table"][request, position // page]), kv_head, dim, position % page] = value
+
+
+def expect_reached(case, got, finite, reached, values):
+    """Elements that see a value that is not finite are that value (or NaN, of two), whatever its weight; the others are as without it."""
+    got, finite = got.view_as(reached).float(), finite.view_as(reached).float()
+    assert bool((got[~reached].isfinite()).all())
+    assert float((got[~reached] - finite[~reached]).abs().max()) <= float(torch.finfo(case["q"].dtype).eps) * float(finite.abs().max())
+    want = values[reached]
+    assert torch.equal(got[reached].nan_to_num(nan=12345.0), want.nan_to_num(nan=12345.0))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("scale", [None, 2.0], ids=["mild", "far"])
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+def test_values_that_are_not_finite_in_places_that_all_see(tiled, dtype, scale, value):
+    """In the prompt and among own keys, of a token each and of drafts: everybody who sees the place gets what the formula gives - its
+    weight, however small, is no nought.  (`far`: scores some hundred apart, whose weights are less than 32 bits hold.)"""
+    heads, kv_heads, dim, shared = 8, 2, 128, 1104
+    counts = (1, 3, 1)
+    case = batch(dtype, heads, kv_heads, dim, 16, shared, (300, 7, 60), counts, seed=72, scale=scale)
+    finite = attend(tiled, case)
+    put_value(case, 0, 700, 0, 5, value)                       # of the prompt, seen by all
+    put_value(case, 0, shared + 200, 1, 9, value)              # among the first request's own
+    put_value(case, 1, shared + 3, 1, 77, value)               # among the second's, seen by its three tokens
+    put_value(case, 2, shared + 59, 1, 100, -value)            # of the third's
+    put_value(case, 2, 4, 1, 100, value)                       # which the prompt has there too: of both signs is NaN
+    case_values = torch.zeros(5, heads, dim, device=DEV)
+    reached = torch.zeros(5, heads, dim, dtype=torch.bool, device=DEV)
+    for tokens, of_heads, d, v in ((slice(0, 5), slice(0, 4), 5, value), (slice(0, 1), slice(4, 8), 9, value), (slice(1, 4), slice(4, 8), 77, value),
+                                   (slice(0, 5), slice(4, 8), 100, value), (slice(4, 5), slice(4, 8), 100, math.nan)):
+        reached[tokens, of_heads, d] = True
+        case_values[tokens, of_heads, d] = v
+    expect_reached(case, attend(tiled, case), finite, reached, case_values)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+def test_values_near_the_largest(tiled, dtype):
+    """A segment's first keys of scores far below the others': weights above one times values of 2^100 stay in range."""
+    case = batch(dtype, 8, 2, 64, 16, 2048, (20, 40), (2, 1), seed=73)
+    case["q"] = torch.ones_like(case["q"])
+    case["k"].fill_(0.0)
+    case["k"][case["table"][0, 60:].clamp(min=0).long()] = 3.0         # scores of 24, weights of 2^34 beside those of the first keys
+    case["v"] *= 2.0 ** 100
+    within(tiled, case, attend(tiled, case))
 
 
 # ---- a step's layout --------------------------------------------------------------------------------------------------------
