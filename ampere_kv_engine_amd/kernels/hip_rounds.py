@@ -36,7 +36,10 @@ def wide_tiles(rows: int, kv_heads: int, shared: int, units: int) -> bool:
     return rows > 64 and rows * kv_heads * shared >= 85_000 * units
 
 
-def cut_own(requests: int, rows: int, kv_heads: int, most: int, units: int) -> tuple[int, int]:
+OWN_ROOM = 512 << 20        # bytes of own keys' partial sums
+
+
+def cut_own(requests: int, rows: int, kv_heads: int, most: int, units: int, segment_bytes: int = 0) -> tuple[int, int]:
     """(segments, keys of one) of up to `most` keys that a request of up to `rows` rows a kv head holds behind the prompt.  What a block waits
     for at its start and end is a good part of its time, but a long request's keys are not to outlast the others': segments of 128 keys, a
     step for each of a block's waves, while they find a unit each, of 256 while those do, of 384 beyond, and the whole up to half as
@@ -44,10 +47,14 @@ def cut_own(requests: int, rows: int, kv_heads: int, most: int, units: int) -> t
     256 keys 17.3 / 16.8, 18.5 / 18.2, 20.5 / 19.7; 8 of 1,000 26 / 18, 21 / 19, 21 / 20, 22 / 22, 27 / 27; 16 of 600 25 / 18, 24 / 18,
     20 / 19, 21 / 20; 64 of 1,000 87 / 37, 66 / 32, 62 / 33, 64 / 34, 58 / 39; in a launch of their own 64 of 2,048 213 / 94, 187 / 81,
     179 / 79, 179 / 82, 179 / 89; 27 of 2,000 with up to 25 rows 145 / 68, 124 / 63, 124 / 64, 117 / 63, 111 / 67; of one segment 64 of
-    500, 512 keys 39 / 30 and 384 40 / 29; with 40 rows 133 / 92 and 145 / 85.)"""
+    500, 512 keys 39 / 30 and 384 40 / 29; with 40 rows 133 / 92 and 145 / 85.)
+    The bound is the caller's, and a recorded call's the longest it may meet: a segment leaves `segment_bytes` of partial sums, as many of them as
+    `OWN_ROOM` holds, but eight at least (64 requests of 5 rows, 64 heads of 128, a bound of 131,072 keys: 256 segments of 512 keys would be 2.7
+    GB, 49 of 2,688 are)."""
     blocks = requests * kv_heads * ((rows + 63) // 64)
     keys = 128 if blocks * ((most + 127) // 128) <= units else 256 if blocks * ((most + 255) // 256) <= units else 384 if most > 576 else most
-    keys = (max(keys, (most + 255) // 256) + 127) // 128 * 128
+    segments = max(8, min(256, OWN_ROOM // segment_bytes)) if segment_bytes else 256
+    keys = (max(keys, (most + segments - 1) // segments) + 127) // 128 * 128
     return (most + keys - 1) // keys, keys
 
 
@@ -144,6 +151,9 @@ class RoundKernels:
         the rows and keys on that `wide_tiles` says) are rounded once, by up to 2^-8 of each: what a request gets there is off by 0.0023 of the
         output's largest in place of 0.0017, of which 0.0016 is the output's own rounding, and which of both it is depends on the batch.
         `two_part_weights`: in two parts whatever the batch, in tiles of 32 columns.
+        Both bounds cost time and memory where they are far above the lengths: the launch has a block for every segment of keys that each
+        request might hold, and partial sums lie in 4 * tokens * q_heads * (head_dim + 2) bytes a segment (`cut_own`, `cut_prefix`) - some
+        tens of MB where bounds are tight, 600 MB at most, or eight segments of very large batches.
         A token gets NaN where its request's table (or the first one's, of the prompt) names a page outside the pool or is no row of
         block_table, where its request exceeds the bounds, or where it stands within the
         prompt.  Rows of `out` behind the last request's are left as they are."""
@@ -181,11 +191,12 @@ class RoundKernels:
         max_new_tokens = min(max_new_tokens, tokens)
         wide = not two_part_weights and wide_tiles_fit(head_dim, page_size, q.dtype) and (
             self.wide_prefix_tiles if self.wide_prefix_tiles is not None else wide_tiles(tokens * group, kv_heads, shared, self.compute_units))
-        own_segments, own_keys = cut_own(requests, max_new_tokens * group, kv_heads, max_seq_len - shared, self.compute_units)
+        of_segment = 4 * tokens * q_heads * (head_dim + 2)
+        own_segments, own_keys = cut_own(requests, max_new_tokens * group, kv_heads, max_seq_len - shared, self.compute_units, of_segment)
         prefix_segments, prefix_keys = cut_prefix(256 if wide else 32, tokens * group, kv_heads, shared, self.compute_units, q.dtype == torch.float32)
         segments = prefix_segments + own_segments
         # (from torch's pool: a recorded call then has room of its own, and calls on other streams do not meet in one)
-        room = torch.empty(segments * tokens * q_heads * (head_dim + 2), dtype=torch.float32, device=self.device)
+        room = torch.empty(segments * of_segment // 4, dtype=torch.float32, device=self.device)
         sums = room.data_ptr()
         self._check_spans(self._shared_prefix_entry(head_dim)(
             q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), _DTYPE_CODE[q.dtype], sums,

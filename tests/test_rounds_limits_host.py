@@ -7,6 +7,7 @@ from concurrent.futures import ThreadPoolExecutor
 import torch
 
 from ampere_kv_engine_amd.csrc import build
+from ampere_kv_engine_amd.kernels import hip_rounds
 from test_rounds_host import Recorder, attention
 
 
@@ -36,3 +37,30 @@ def test_every_head_size_compiles():
     with ThreadPoolExecutor(max_workers=8) as pool:
         for result in pool.map(compiled, range(16, 257, 16)):
             assert result.returncode == 0, result.stderr
+
+
+def test_partial_sums_stay_within_their_room_whatever_the_bound():
+    """A call over a long table, as it is recorded, brings its bound and not its lengths."""
+    for requests, new, heads, dim in ((64, 5, 64, 128), (64, 1, 32, 128), (500, 1, 32, 128), (500, 5, 64, 256), (1, 1, 16, 64)):
+        tokens = requests * new
+        of_segment = 4 * tokens * heads * (dim + 2)
+        for most in (1, 500, 2048, 32768, 131072, 1 << 20):
+            segments, keys = hip_rounds.cut_own(requests, new * heads // 8, 8, most, 256, of_segment)
+            assert segments * of_segment <= max(hip_rounds.OWN_ROOM, 8 * of_segment) and segments <= 256
+            assert keys % 128 == 0 and (segments - 1) * keys < most <= segments * keys
+            if most <= 2048:      # (bounds that are near the lengths: cut by what the blocks do)
+                assert (segments, keys) == hip_rounds.cut_own(requests, new * heads // 8, 8, most, 256)
+
+
+def test_the_call_takes_its_room_into_account():
+    q = torch.zeros(320, 64 * 16)
+    kernels = Recorder()
+    arguments = attention(q=q, out=torch.zeros_like(q), q_heads=64, kv_heads=8, head_dim=16, k_pages=torch.zeros(2, 8, 16, 16), v_pages=torch.zeros(2, 8, 16, 16),
+                          block_table=torch.zeros(3, 1 << 16, dtype=torch.int32), max_seq_len=1 << 20, max_new_tokens=5, shared=0)
+    hip_rounds_room, hip_rounds.OWN_ROOM = hip_rounds.OWN_ROOM, 64 << 20
+    try:
+        kernels.attention_shared_prefix(**arguments)
+    finally:
+        hip_rounds.OWN_ROOM = hip_rounds_room
+    own_segments = kernels.calls[0][-4]
+    assert own_segments * 4 * 320 * 64 * 18 <= 64 << 20 and own_segments >= 40
