@@ -366,7 +366,7 @@ __device__ __forceinline__ Row gather_row(const Part& part, double inverse, bool
 __global__ __launch_bounds__(kChooseThreads) void choose_kernel(Verify a) {
   constexpr int kThreads = kChooseThreads, kWaves = kThreads / kWave, kLoads = kPart / 4 / kThreads;
   __shared__ Row target[kMostPlaces], draft[kMostPlaces];
-  __shared__ unsigned char fine[kMostPlaces];
+  __shared__ unsigned char fine[kMostPlaces];                // 1: the place's draft is kept if all before it are; 2: its number is NaN
   __shared__ double sums[kWaves], powers[kPowers], draft_powers[kPowers];
   __shared__ int of_waves[kWaves];
   __shared__ int is_last;
@@ -407,7 +407,7 @@ __global__ __launch_bounds__(kChooseThreads) void choose_kernel(Verify a) {
   if (tid < rows - 1) {                                   // place `tid`'s draft: kept if all before it are
     const Row row = target[tid];
     bool keep = false;
-    if (row.fine && drafted >= 0 && drafted < a.vocab) {
+    if (row.fine && t == t && drafted >= 0 && drafted < a.vocab) {
       if (!drawn) {
         keep = row.best == drafted;
       } else {
@@ -421,11 +421,11 @@ __global__ __launch_bounds__(kChooseThreads) void choose_kernel(Verify a) {
         keep = known && static_cast<double>(its_number) * q < p;
       }
     }
-    fine[tid] = keep;
+    fine[tid] = keep ? 1 : its_number != its_number ? 2 : 0;
   }
   __syncthreads();
   int kept = 0;
-  while (kept < rows - 1 && fine[kept] != 0) ++kept;
+  while (kept < rows - 1 && fine[kept] == 1) ++kept;
   int* chosen = a.chosen + static_cast<size_t>(request) * a.places;
   if (block == 0)
     for (int i = tid; i < a.places; i += kThreads)
@@ -435,8 +435,9 @@ __global__ __launch_bounds__(kChooseThreads) void choose_kernel(Verify a) {
   const Row row = target[kept];
   const bool rejected = kept < rows - 1;
   const bool from_draft = rejected && a.draft != nullptr;
-  if (!row.fine || !drawn || (from_draft && !draft[kept].fine)) {
-    if (block == 0 && tid == 0) chosen[kept] = row.fine && !drawn ? row.best : -1;
+  const bool no_number = last_number != last_number || (rejected && fine[kept] == 2);
+  if (!row.fine || !drawn || (from_draft && !draft[kept].fine) || no_number) {
+    if (block == 0 && tid == 0) chosen[kept] = row.fine && !drawn && t == t ? row.best : -1;
     return;
   }
   const int refused = rejected && a.draft == nullptr ? a.tokens[first + kept + 1] : -1;    // (all of q lies on it)

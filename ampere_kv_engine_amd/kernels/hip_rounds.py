@@ -218,7 +218,8 @@ class RoundKernels:
         kept [requests], chosen [requests, places] int32: the kept drafts, the token that follows, -1 behind it.
         A request without rows, or with rows that are not among the logits, gets 0 and -1; rows beyond `places` are not looked at.  A row
         that has no next token - a NaN, nothing above minus infinity, or (where it is drawn from) plus infinity, in the target's or the
-        draft's - ends the walk with -1 as the token.  A draft that is no id of the vocabulary is not kept."""
+        draft's - ends the walk with -1 as the token.  So does a number that is NaN where the walk looks at it (a draft's that it comes to, the
+        last one where a token is drawn), and a temperature that is NaN at its first row.  A draft that is no id of the vocabulary is not kept."""
         if logits.dim() != 2 or uniforms.dim() != 2:
             raise self._error("logits and uniforms must be matrices")
         (count, vocab), (requests, places) = logits.shape, uniforms.shape

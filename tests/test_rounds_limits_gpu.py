@@ -6,7 +6,7 @@ from types import SimpleNamespace
 import pytest
 import torch
 
-from test_rounds_gpu import attend, batch, kernel_set, kernels, place_both, tiled, within  # noqa: F401  (fixtures among them)
+from test_rounds_gpu import attend, batch, drafted, ints, kernel_set, kernels, place_both, tiled, within  # noqa: F401  (fixtures among them)
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -87,6 +87,52 @@ def test_values_near_the_largest(tiled, dtype):
     case["k"][case["table"][0, 60:].clamp(min=0).long()] = 3.0         # scores of 24, weights of 2^34 beside those of the first keys
     case["v"] *= 2.0 ** 100
     within(tiled, case, attend(tiled, case))
+
+
+# ---- drafted tokens ---------------------------------------------------------------------------------------------------------
+
+def verified(kernels, logits, tokens, starts, temperature, uniforms, draft):
+    requests, places = uniforms.shape
+    kept, chosen = ints([99] * requests), torch.full((requests, places), 99, dtype=torch.int32, device=DEV)
+    kernels.verify_drafts(logits.to(DEV), tokens.to(DEV), ints(starts), temperature.to(DEV), uniforms.to(DEV), kept, chosen,
+                          draft_logits=draft.to(DEV) if draft is not None else None)
+    return kept.tolist(), chosen.tolist()
+
+
+@pytest.mark.parametrize("with_draft", [True, False], ids=["drawn", "looked-up"])
+def test_a_temperature_that_is_no_number_has_no_next_token(kernels, with_draft):
+    """Nothing is kept and nothing chosen; the requests beside it get what they get."""
+    logits, tokens, starts, temperature, uniforms, draft = drafted(5000, (3, 3, 1, 0, 3), 3, with_draft, 80, temperatures=(1.0, 0.0))
+    kept, chosen = verified(kernels, logits, tokens, starts, temperature, uniforms, draft)
+    temperature[[0, 2, 3]] = math.nan
+    now_kept, now_chosen = verified(kernels, logits, tokens, starts, temperature, uniforms, draft)
+    for r in range(5):
+        if r in (0, 2, 3):
+            assert now_kept[r] == 0 and now_chosen[r] == [-1, -1, -1]
+        else:
+            assert now_kept[r] == kept[r] and now_chosen[r] == chosen[r]
+
+
+@pytest.mark.parametrize("with_draft", [True, False], ids=["drawn", "looked-up"])
+@pytest.mark.parametrize("place", [0, 1, 2])
+def test_a_random_number_that_is_none_ends_the_walk(kernels, with_draft, place):
+    """The walk ends without a next token at a draft whose number is NaN, and where the token would be drawn with one.  Numbers that
+    nobody looks at - of places behind the walk's end, of greedy requests - change nothing."""
+    for seed in range(8):
+        logits, tokens, starts, temperature, uniforms, draft = drafted(700, (3, 2, 3, 3, 1), 3, with_draft, 90 + seed, temperatures=(1.0, 0.7, 0.0))
+        if seed % 2 and not with_draft:                     # (the best token as the draft, and numbers that keep it)
+            uniforms[:, :2] = 0.0
+        kept, chosen = verified(kernels, logits, tokens, starts, temperature, uniforms, draft)
+        numbers = uniforms.clone()
+        numbers[:, place] = math.nan
+        now_kept, now_chosen = verified(kernels, logits, tokens, starts, temperature, numbers, draft)
+        for r, rows in enumerate((3, 2, 3, 3, 1)):
+            if float(temperature[r]) == 0 or place < 2 and (place > kept[r] or place >= rows - 1):
+                assert now_kept[r] == kept[r] and now_chosen[r] == chosen[r]
+            elif place == 2:                                # the number for the token
+                assert now_kept[r] == kept[r] and now_chosen[r] == chosen[r][:kept[r]] + [-1] * (3 - kept[r])
+            else:                                           # a draft's
+                assert now_kept[r] == place and now_chosen[r] == chosen[r][:place] + [-1] * (3 - place)
 
 
 # ---- a step's layout --------------------------------------------------------------------------------------------------------
