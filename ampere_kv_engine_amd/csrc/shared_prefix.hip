@@ -63,6 +63,7 @@ struct Args {
   int own_segments, own_keys;          // the same of a request's own keys
   int prefix_tiles, own_tiles;         // tiles of columns: of all rows, of the most rows a request brings
   long prefix_blocks;
+  const int* prefix_pages;    // the prompt's pages, or null: they are read from the first request's row
 };
 
 // What the host could not see of a request: whether its tokens lie within q, its lengths within the bounds and behind the prompt.  The
@@ -746,15 +747,16 @@ __device__ __forceinline__ bool own_item(const Args& a, long number, int& reques
 }
 
 // Blocks 0 .. prefix_blocks - 1 take (segment and head, tile) of the prefix, the others (request, head, two tiles, segment) of the
-// requests' own keys.
-template <typename T>
+// requests' own keys.  GIVEN: the prompt's pages are `prefix_pages` (a kernel of its own: the choice costs registers and half a microsecond).
+template <typename T, bool GIVEN>
 __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 || D > 128 ? 1 : 2)) void shared_prefix_kernel(Args a) {
   extern __shared__ float lds[];
   long block = blockIdx.x;
   const int lane = threadIdx.x & (kWave - 1), r = lane & 31;
   int head, segment, request = 0, columns, first, end, visible, all_see, tile;
   long row0, item;
-  if (block < a.prefix_blocks) {
+  const bool of_prefix = block < a.prefix_blocks;
+  if (of_prefix) {
     tile_of(block, static_cast<long>(a.prefix_segments) * a.kv_heads, a.prefix_tiles, item, tile);
     head = static_cast<int>(item % a.kv_heads);
     segment = static_cast<int>(item / a.kv_heads);
@@ -792,7 +794,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 || D > 128 ? 1 : 2)) void
       return;
     }
   }
-  const int* table = table_of(a, request);
+  const int* table = GIVEN && of_prefix ? a.prefix_pages : table_of(a, request);
   if (table == nullptr) return;
   walk<T, kWaves>(a, table, head, row0, columns, first, end, visible, all_see, segment, lds);
 }
@@ -845,7 +847,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Args a) {
 #pragma unroll
   for (int e = 0; e < kEach; ++e) sum[e] = 0.f;
   if (!within_bounds(a, begin, count, length) || token - begin >= count || table_of(a, request) == nullptr ||
-      (a.shared > 0 && table_of(a, 0) == nullptr)) {
+      (a.shared > 0 && a.prefix_pages == nullptr && table_of(a, 0) == nullptr)) {
     total = NAN;
   } else {
     const int used = a.prefix_segments + (seen - a.shared + a.own_keys - 1) / a.own_keys;
@@ -916,14 +918,21 @@ template <typename T> int run(const Args& all, bool wide, hipStream_t stream) {
       constexpr size_t wide_lds = kWideLds > kWideNarrowLds ? kWideLds : kWideNarrowLds;
       if (a.prefix_blocks > 0x7fffffffL) return -2;
       if ((status = room_for(wide_prefix_kernel, wide_lds)) != 0) return status;
-      wide_prefix_kernel<<<static_cast<unsigned>(a.prefix_blocks), kWideWaves * kWave, wide_lds, stream>>>(a);
+      Args of_prompt = a;
+      if (a.prefix_pages != nullptr) {      // (a table whose only row they are)
+        of_prompt.block_table = a.prefix_pages;
+        of_prompt.table_rows = nullptr;
+        of_prompt.table_count = 1;
+      }
+      wide_prefix_kernel<<<static_cast<unsigned>(a.prefix_blocks), kWideWaves * kWave, wide_lds, stream>>>(of_prompt);
       if ((status = AKV_LAUNCH_STATUS()) != 0) return status;
       a.prefix_blocks = 0;
     }
   const long blocks = a.prefix_blocks + static_cast<long>(a.requests) * a.kv_heads * ((a.own_tiles + 1) / 2) * a.own_segments;
   if (blocks > 0x7fffffffL || a.q_heads > 65535) return -2;
-  if ((status = room_for(shared_prefix_kernel<T>, lds)) != 0) return status;
-  shared_prefix_kernel<T><<<static_cast<unsigned>(blocks), kThreads, lds, stream>>>(a);
+  const auto kernel = a.prefix_pages != nullptr && a.prefix_blocks > 0 ? shared_prefix_kernel<T, true> : shared_prefix_kernel<T, false>;
+  if ((status = room_for(kernel, lds)) != 0) return status;
+  kernel<<<static_cast<unsigned>(blocks), kThreads, lds, stream>>>(a);
   if ((status = AKV_LAUNCH_STATUS()) != 0) return status;
   // (a wave a row where they are 2,048 and more, eight of a unit's thirty-two)
   if (a.tokens * a.q_heads >= 8L * device_facts().compute_units)
@@ -942,8 +951,8 @@ template <typename T> int run(const Args& all, bool wide, hipStream_t stream) {
 // floats; segments: prefix_segments of prefix_keys (multiples of 32) cover `shared`, own_segments of own_keys `max_own` keys of a
 // request behind it, at most 512 together.  `wide`: the prompt's columns go in tiles of 256 (`walk_wide`).  Operands lie on 16-byte boundaries.
 extern "C" int AKV_NAME(AKV_HEAD_DIM)(const void* q, const void* k_pages, const void* v_pages, void* out, int dtype, float* sums, float* stats,
-                                      const int* q_start, const int* seq_lens, const int* block_table, const int* table_rows, int table_width, int table_count,
-                                      int requests, long tokens, int q_heads, int kv_heads, int page_size, long num_pages, float scale,
+                                      const int* q_start, const int* seq_lens, const int* block_table, const int* table_rows, const int* prefix_pages, int table_width,
+                                      int table_count, int requests, long tokens, int q_heads, int kv_heads, int page_size, long num_pages, float scale,
                                       int shared, int max_own, int max_new, int prefix_segments, int prefix_keys, int own_segments,
                                       int own_keys, int wide, hipStream_t stream) {
   if (requests <= 0 || tokens <= 0) return 0;
@@ -954,13 +963,13 @@ extern "C" int AKV_NAME(AKV_HEAD_DIM)(const void* q, const void* k_pages, const 
     return -2;
   const long size = dtype == kF32 ? 4 : 2, of_q = tokens * q_heads * D * size, of_pages = num_pages * kv_heads * page_size * D * size;
   const Span spans[] = {{out, of_q}, {q, of_q}, {k_pages, of_pages}, {v_pages, of_pages}, {block_table, 4L * table_width * table_count},
-                        {q_start, 4L * requests + 4}, {seq_lens, 4L * requests}, {table_rows, 4L * requests}};
-  const int overlap = shared_spans(spans, 1, 8);
+                        {q_start, 4L * requests + 4}, {seq_lens, 4L * requests}, {table_rows, 4L * requests}, {prefix_pages, 4L * (shared / page_size)}};
+  const int overlap = shared_spans(spans, 1, 9);
   if (overlap != 0) return overlap;
   Args a{};
   const int group = q_heads / kv_heads;
   a.q = q; a.k_pages = k_pages; a.v_pages = v_pages; a.out = out; a.sums = sums; a.stats = stats;
-  a.q_start = q_start; a.seq_lens = seq_lens; a.block_table = block_table; a.table_rows = table_rows;
+  a.q_start = q_start; a.seq_lens = seq_lens; a.block_table = block_table; a.table_rows = table_rows; a.prefix_pages = prefix_pages;
   a.table_width = table_width; a.table_count = table_count; a.requests = requests; a.tokens = tokens; a.rows = tokens * group;
   a.q_heads = q_heads; a.kv_heads = kv_heads; a.shared = shared; a.max_own = max_own; a.max_new = max_new;
   a.num_pages = num_pages; a.scale_log2 = scale * kLog2e; a.group = Divider::of(group);

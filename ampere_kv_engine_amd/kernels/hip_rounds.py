@@ -113,7 +113,7 @@ class RoundKernels:
             entry = getattr(self._load(ensure_shared_prefix(head_dim)), f"akv_attention_shared_prefix_d{head_dim}")
             p, i, n = ctypes.c_void_p, ctypes.c_int, ctypes.c_long
             entry.restype = i
-            entry.argtypes = (p, p, p, p, i, p, p, p, p, p, p, i, i, i, n, i, i, i, n, ctypes.c_float, i, i, i, i, i, i, i, i, p)
+            entry.argtypes = (p, p, p, p, i, p, p, p, p, p, p, p, i, i, i, n, i, i, i, n, ctypes.c_float, i, i, i, i, i, i, i, i, p)
             entries[head_dim] = entry
         return entries[head_dim]
 
@@ -137,14 +137,15 @@ class RoundKernels:
 
     # ---- attention -----------------------------------------------------------------------------------------------------
     def attention_shared_prefix(self, q, k_pages, v_pages, block_table, q_start, seq_lens, shared, q_heads, kv_heads, head_dim, scale, out,
-                                max_seq_len, max_new_tokens, rows=None, two_part_weights=False):
+                                max_seq_len, max_new_tokens, rows=None, prefix_pages=None, two_part_weights=False):
         """Attention of requests whose first `shared` tokens (a multiple of the page size; 0: none) lie in the same pages: those
         are read once for all of them, so that many requests cost little more than one.  q, out [tokens, q_heads * head_dim]:
         encoded queries, request by request, whose keys and values are in the pages already.  q_start [requests + 1]: a request's
         first row; seq_lens [requests]: the tokens it holds, its new ones among them; both int32 on the device.  block_table: row r,
-        or rows[r] where `rows` is given, holds request r's pages; the first request's row is read for the prompt.  No request holds
-        more than `max_seq_len` tokens or brings more than `max_new_tokens` (0 is fine, and any number from there on; prompts of
-        thousands of tokens are `attention`'s).
+        or rows[r] where `rows` is given, holds request r's pages.  The prompt's are read from `prefix_pages` (its first shared / page
+        size entries, as `place_tokens` takes them), or, where that is not given, from the first request's row, which must then stand
+        although that request brings nothing any more.  No request holds more than `max_seq_len` tokens or brings more than
+        `max_new_tokens` (0 is fine, and any number from there on; prompts of thousands of tokens are `attention`'s).
         float32 or bfloat16; head sizes as `check_attention_sizes` has them; pages of 8 tokens or more, a power of two.
         bfloat16: softmax weights are multiplied in two bfloat16 parts, the rounded one and what the rounding left, as `attention` does -
         but the weights of a prompt whose keys go in tiles of 256 columns (heads of 64 and 128, pages of 16 and more, from
@@ -154,7 +155,7 @@ class RoundKernels:
         Both bounds cost time and memory where they are far above the lengths: the launch has a block for every segment of keys that each
         request might hold, and partial sums lie in 4 * tokens * q_heads * (head_dim + 2) bytes a segment (`cut_own`, `cut_prefix`) - some
         tens of MB where bounds are tight, 600 MB at most, or eight segments of very large batches.
-        A token gets NaN where its request's table (or the first one's, of the prompt) names a page outside the pool or is no row of
+        A token gets NaN where its request's table (or, of the prompt, what it is read from) names a page outside the pool or is no row of
         block_table, where its request exceeds the bounds, or where it stands within the
         prompt.  Rows of `out` behind the last request's are left as they are."""
         tokens, requests = q.shape[0], seq_lens.shape[0]
@@ -169,6 +170,10 @@ class RoundKernels:
         self._vectors(("q_start", "seq_lens"), (q_start, seq_lens), (requests + 1, requests))
         if rows is not None:
             self._dense(rows, "table rows", torch.int32, (requests,))
+        if prefix_pages is not None:
+            self._dense(prefix_pages, "prefix_pages", torch.int32)
+            if prefix_pages.dim() != 1 or prefix_pages.shape[0] * page_size < shared:
+                raise self._error(f"prefix_pages must be a vector of the pages of {shared} tokens, got {tuple(prefix_pages.shape)}")
         self._dense(block_table, "block_table", torch.int32)
         if block_table.dim() != 2 or (rows is None and block_table.shape[0] != requests):
             raise self._error(f"block_table must be [{requests if rows is None else 'rows'}, pages], got {tuple(block_table.shape)}")
@@ -200,10 +205,10 @@ class RoundKernels:
         sums = room.data_ptr()
         self._check_spans(self._shared_prefix_entry(head_dim)(
             q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), _DTYPE_CODE[q.dtype], sums,
-            sums + 4 * segments * tokens * q_heads * head_dim, q_start.data_ptr(), seq_lens.data_ptr(), block_table.data_ptr(), _address(rows),
+            sums + 4 * segments * tokens * q_heads * head_dim, q_start.data_ptr(), seq_lens.data_ptr(), block_table.data_ptr(), _address(rows), _address(prefix_pages),
             block_table.shape[1], block_table.shape[0], requests, tokens, q_heads, kv_heads, page_size, num_pages, scale, shared, max_seq_len - shared, max_new_tokens,
             prefix_segments, prefix_keys, own_segments, own_keys, int(wide), self._stream()), "attention_shared_prefix",
-            ("out", "q", "k_pages", "v_pages", "block_table", "q_start", "seq_lens", "table rows"))
+            ("out", "q", "k_pages", "v_pages", "block_table", "q_start", "seq_lens", "table rows", "prefix_pages"))
 
     # ---- drafted tokens ------------------------------------------------------------------------------------------------
     def verify_drafts(self, logits, tokens, q_start, temperature, uniforms, kept, chosen, draft_logits=None):

@@ -6,6 +6,7 @@ from types import SimpleNamespace
 import pytest
 import torch
 
+from ampere_kv_engine_amd.kernels.hip import KernelError
 from test_rounds_gpu import attend, batch, drafted, ints, kernel_set, kernels, place_both, tiled, within  # noqa: F401  (fixtures among them)
 
 pytestmark = pytest.mark.gpu
@@ -87,6 +88,25 @@ def test_values_near_the_largest(tiled, dtype):
     case["k"][case["table"][0, 60:].clamp(min=0).long()] = 3.0         # scores of 24, weights of 2^34 beside those of the first keys
     case["v"] *= 2.0 ** 100
     within(tiled, case, attend(tiled, case))
+
+
+def test_the_prompt_is_found_without_the_first_request(tiled):
+    """The first request has ended and its row is cleared, or is none any more: the prompt's pages are given by themselves."""
+    case = batch(torch.bfloat16, 8, 2, 64, 16, 1104, (3, 40, 9, 5), (0, 1, 2, 1), seed=74)
+    good = attend(tiled, case)
+    within(tiled, case, good)
+    pages = case["table"][0, :1104 // 16].to(DEV)
+    table = case["table"].clone()
+    table[0] = -1
+    assert bool(attend(tiled, case, block_table=table.to(DEV)).isnan().all())
+    for changes in (dict(), dict(rows=ints([-1, 1, 2, 3])), dict(rows=ints([0, 1, 2, 3]), prefix_pages=torch.cat((pages, ints([-5, 7]))))):
+        assert torch.equal(attend(tiled, case, **{**dict(block_table=table.to(DEV), prefix_pages=pages), **changes}), good)
+    wrong = pages.clone()
+    wrong[30] = case["k"].shape[0]
+    assert bool(attend(tiled, case, prefix_pages=wrong).isnan().all())
+    out = torch.empty(4, 512, dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(KernelError, match="out and prefix_pages share memory"):
+        attend(tiled, case, prefix_pages=out.view(torch.int32).view(-1)[:69], out=out)
 
 
 # ---- drafted tokens ---------------------------------------------------------------------------------------------------------

@@ -4,10 +4,12 @@ import os
 import subprocess
 from concurrent.futures import ThreadPoolExecutor
 
+import pytest
 import torch
 
 from ampere_kv_engine_amd.csrc import build
 from ampere_kv_engine_amd.kernels import hip_rounds
+from ampere_kv_engine_amd.kernels.hip import KernelError
 from test_rounds_host import Recorder, attention
 
 
@@ -64,3 +66,16 @@ def test_the_call_takes_its_room_into_account():
         hip_rounds.OWN_ROOM = hip_rounds_room
     own_segments = kernels.calls[0][-4]
     assert own_segments * 4 * 320 * 64 * 18 <= 64 << 20 and own_segments >= 40
+
+
+def test_attention_refuses_pages_of_a_prompt_that_are_too_few():
+    ints = lambda *shape, dtype=torch.int32: torch.zeros(*shape, dtype=dtype)
+    kernels = Recorder()
+    kernels.attention_shared_prefix(**attention(prefix_pages=ints(2)))          # 32 shared tokens, pages of 16
+    kernels.attention_shared_prefix(**attention(prefix_pages=ints(5)))
+    kernels.attention_shared_prefix(**attention(prefix_pages=ints(0), shared=0))
+    assert len(kernels.calls) == 3
+    for pages in (ints(1), ints(2, dtype=torch.int64), ints(2, 1), ints(4)[::2]):
+        with pytest.raises(KernelError):
+            kernels.attention_shared_prefix(**attention(prefix_pages=pages))
+    assert len(kernels.calls) == 3
