@@ -18,7 +18,7 @@ int akv_place_tokens(const int* lengths, const int* counts, const int* held, con
                      const int* cursor, int* table, const int* rows, int table_rows, int table_width, int page_size,
                      const int* prefix_pages, int prefix_count, int requests, int tokens, int* q_start, int* seq_lens,
                      int* held_after, int* cursor_after, int* positions, int* seq_of_token, int* slot_map, int* status,
-                     hipStream_t stream);
+                     int clear_rest, hipStream_t stream);
 
 // Bytes of `workspace` (on a 16-byte boundary) for `requests` requests of up to `places` rows; -1 for sizes not taken.
 long akv_verify_workspace(int requests, int places, int vocab);

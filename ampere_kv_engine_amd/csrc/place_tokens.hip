@@ -9,7 +9,8 @@
 // own or a wait between blocks), keeps what it has read of them in LDS, and then takes its share of the tokens and of the table's
 // entries.  A token's page is computed, not read back from the table entries that another block may be writing: an entry below `had` was
 // there before the call (or is the prompt's), one from `had` on follows from the free list.  So no block reads what another writes.
-// Nothing but `status` is written where the step cannot be laid out: every block finds that out before it writes.
+// Nothing but `status` is written where the step cannot be laid out - or, `clear_rest`, a layout in which nobody brings anything: every
+// block finds that out before it writes.
 // What bounds it is latency: a launch (2.8 us), the lengths' reads, the scan's barriers, one dependent read (free list or table) a token:
 // 8 requests 4.2 us, 500 of up to 5 tokens 6.4, 64 prompts of 115,000 tokens together 6.0; a call takes the host 9.
 
@@ -28,6 +29,7 @@ struct Place {
   int *table, *q_start, *seq_lens, *held_after, *cursor_after, *positions, *seq_of_token, *slot_map, *status;
   long free_count;
   int table_rows, table_width, page_size, prefix_count, requests, tokens;
+  int clear_rest;                 // whether slots behind the last token, and what a step that cannot be laid out leaves, are written too
   int hash_places;                // a power of two, at least twice the requests
   Divider page;
 };
@@ -147,11 +149,24 @@ __global__ __launch_bounds__(kThreads) void place_kernel(Place p) {
     p.status[0] = verdict;
     if (verdict >= 0) p.cursor_after[0] = cursor + verdict;
   }
-  if (verdict < 0) return;
+  const int begin = blockIdx.x * kThreads + tid, stride = gridDim.x * kThreads;
+  if (verdict < 0) {
+    if (p.clear_rest == 0) return;
+    for (int i = begin; i < p.tokens; i += stride) p.slot_map[i] = -1;
+    for (int r = begin; r < n; r += stride) {
+      p.q_start[r] = 0;
+      p.seq_lens[r] = p.lengths[r];
+      p.held_after[r] = p.held[r];
+    }
+    if (begin == 0) {
+      p.q_start[n] = 0;
+      p.cursor_after[0] = cursor;
+    }
+    return;
+  }
   const int tokens = static_cast<int>(tokens_before), pages = static_cast<int>(pages_before);
   if (tid == 0) { first_token[n] = tokens; first_page[n] = pages; }
   __syncthreads();
-  const int begin = blockIdx.x * kThreads + tid, stride = gridDim.x * kThreads;
   auto pages_had = [&](int r) { return had_of[r] < 0 ? -1 - had_of[r] : had_of[r]; };
   // the last request whose first number is <= i (requests that bring nothing are stepped over)
   auto owner = [&](const int* first, int i) {
@@ -172,6 +187,8 @@ __global__ __launch_bounds__(kThreads) void place_kernel(Place p) {
     p.seq_of_token[i] = r;
     p.slot_map[i] = id < 0 ? -1 : id * p.page_size + inside;
   }
+  if (p.clear_rest != 0)
+    for (int i = tokens + begin; i < p.tokens; i += stride) p.slot_map[i] = -1;
   for (int i = begin; i < pages; i += stride) {
     const int r = owner(first_page, i);
     p.table[static_cast<size_t>(row_of[r]) * p.table_width + pages_had(r) + i - first_page[r]] = p.free_pages[cursor + i];
@@ -202,13 +219,14 @@ extern "C" int akv_place_most_requests() { return kMost; }
 // `status` [1]: the pages taken, or why nothing but `status` was written: -1 too few free pages, -2 a request's row is not in the
 // table, too narrow for its pages or another request's too, -3 more tokens than the maps have room for, -4 a negative length, count or
 // number of pages, a request that holds fewer pages than its length fills, or one that would write into a prompt that another one of the batch has
-// or writes as well.  No output may lie in an input but `table`, whose entries below a request's
+// or writes as well.  `clear_rest` not 0: slot_map is -1 behind the last token, and where the step cannot be laid out everywhere, with q_start
+// all 0 and the lengths, pages and cursor as before.  No output may lie in an input but `table`, whose entries below a request's
 // pages are read and never written.
 extern "C" int akv_place_tokens(const int* lengths, const int* counts, const int* held, const int* free_pages, long free_count,
                                 const int* cursor, int* table, const int* rows, int table_rows, int table_width, int page_size,
                                 const int* prefix_pages, int prefix_count, int requests, int tokens, int* q_start, int* seq_lens,
                                 int* held_after, int* cursor_after, int* positions, int* seq_of_token, int* slot_map, int* status,
-                                hipStream_t stream) {
+                                int clear_rest, hipStream_t stream) {
   if (requests < 0 || requests > kMost || tokens < 0 || page_size <= 0 || table_width < 0 || table_rows < 0 || prefix_count < 0) return -2;
   const long of_requests = 4L * requests, of_tokens = 4L * tokens;
   const Span spans[] = {{q_start, of_requests + 4}, {seq_lens, of_requests}, {held_after, of_requests}, {cursor_after, 4}, {positions, of_tokens},
@@ -221,7 +239,7 @@ extern "C" int akv_place_tokens(const int* lengths, const int* counts, const int
   while (places < 2 * requests) places *= 2;
   const Place p{lengths, counts, held, free_pages, cursor, rows, prefix_pages, table, q_start, seq_lens, held_after, cursor_after,
                 positions, seq_of_token, slot_map, status, free_count, table_rows, table_width, page_size, prefix_count, requests,
-                tokens, places, Divider::of(page_size)};
+                tokens, clear_rest, places, Divider::of(page_size)};
   // (a wave takes a forked request's entries, some hundred reads and writes of the prompt's pages: with blocks enough for all of them)
   const long entries = max(static_cast<long>(max(tokens, requests)), static_cast<long>(requests) * min(prefix_count, kWave));
   const int blocks = static_cast<int>(max(1L, min(256L, (entries + kThreads - 1) / kThreads)));

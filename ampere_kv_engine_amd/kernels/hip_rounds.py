@@ -88,7 +88,7 @@ class RoundKernels:
             p, i, n = ctypes.c_void_p, ctypes.c_int, ctypes.c_long      # (with the types known, addresses are handed over as they are)
             for name, result, types in (
                     ("akv_place_most_requests", i, ()),
-                    ("akv_place_tokens", i, (p, p, p, p, n, p, p, p, i, i, i, p, i, i, i, p, p, p, p, p, p, p, p, p)),
+                    ("akv_place_tokens", i, (p, p, p, p, n, p, p, p, i, i, i, p, i, i, i, p, p, p, p, p, p, p, p, i, p)),
                     ("akv_verify_workspace", n, (i, i, i)),
                     ("akv_verify_drafts", i, (p, i, i, p, p, p, p, i, i, p, n, n, p, p, p, p))):
                 getattr(lib, name).restype, getattr(lib, name).argtypes = result, types
@@ -260,7 +260,7 @@ class RoundKernels:
 
     # ---- a step's layout -----------------------------------------------------------------------------------------------
     def place_tokens(self, lengths, counts, held, free_pages, cursor, table, page_size, q_start, seq_lens, held_after, cursor_after, positions,
-                     seq_of_token, slot_map, status, rows=None, prefix_pages=None):
+                     seq_of_token, slot_map, status, rows=None, prefix_pages=None, clear_rest=False):
         """A step's layout from lengths on the device (all int32).  lengths, counts, held [requests]: the tokens a request holds, those it
         brings, and its pages.  It takes the pages it lacks from free_pages[cursor ...], in the requests' order; they are entered into its
         row of `table` (row r, or rows[r]), and held_after [requests] and cursor_after [1] say what is held and taken then.  A request
@@ -273,7 +273,11 @@ class RoundKernels:
         status [1]: the pages taken, or, with nothing else written, -1 too few free pages, -2 a row that the table does not have, that is too
         narrow or that two requests name, -3 more tokens than the maps have room for, -4 a negative number, fewer pages than a length
         fills, or a request that brings places of the prompt's pages beside one that has pages, starts behind the prompt or brings the same
-        places."""
+        places.
+        What is left as it is names the layout before: a cache write over the whole of `slot_map` would follow it.  `clear_rest`, for rounds in
+        which no host looks at counts and status: slot_map is -1 behind the last token (`kv_write` leaves such rows alone), and where the step
+        cannot be laid out nobody brings anything - slot_map all -1, q_start all 0, seq_lens the lengths, held_after and cursor_after as
+        held and cursor are -, so that attention writes nothing and `verify_drafts` answers 0 kept and -1."""
         requests, tokens = lengths.shape[0], positions.shape[0]
         lib = self._rounds()
         free = free_pages.shape[0]
@@ -296,6 +300,6 @@ class RoundKernels:
             table.data_ptr(), _address(rows), table.shape[0], table.shape[1], int(page_size), _address(prefix_pages),
             prefix_pages.shape[0] if prefix_pages is not None else 0, requests, tokens, q_start.data_ptr(), seq_lens.data_ptr(),
             held_after.data_ptr(), cursor_after.data_ptr(), positions.data_ptr(), seq_of_token.data_ptr(), slot_map.data_ptr(),
-            status.data_ptr(), self._stream()), "place_tokens",
+            status.data_ptr(), int(bool(clear_rest)), self._stream()), "place_tokens",
             ("q_start", "seq_lens", "held_after", "cursor_after", "positions", "seq_of_token", "slot_map", "status", "table", "lengths", "counts",
              "held", "cursor", "free_pages", "table rows", "prefix_pages"))

@@ -7,6 +7,7 @@ import pytest
 import torch
 
 from ampere_kv_engine_amd.kernels.hip import KernelError
+from plain import rounds_plain
 from test_rounds_gpu import attend, batch, drafted, ints, kernel_set, kernels, place_both, tiled, within  # noqa: F401  (fixtures among them)
 
 pytestmark = pytest.mark.gpu
@@ -179,3 +180,123 @@ def test_a_prompt_is_written_where_nobody_has_it_yet(kernels):
     assert place_both(kernels, lengths, [1] * 1500, [0] * 1500, 16, prefix=prompt) == 0
     lengths[1400] = lengths[3]
     assert place_both(kernels, lengths, [1] * 1500, [0] * 1500, 16, prefix=prompt) == -4
+
+
+def place_cleared(kernels, lengths, counts, held, page, tokens, free, cursor=0, prefix=None):
+    requests = len(lengths)
+    outs = {name: torch.full((n,), -99, dtype=torch.int32, device=DEV) for name, n in dict(
+        q_start=requests + 1, seq_lens=requests, held_after=requests, cursor_after=1, positions=tokens, seq_of_token=tokens, slot_map=tokens, status=1).items()}
+    table = torch.full((max(requests, 1), 9), -1, dtype=torch.int32, device=DEV)
+    kernels.place_tokens(ints(lengths), ints(counts), ints(held), ints(free), ints([cursor]), table, page, *outs.values(),
+                         prefix_pages=ints(prefix) if prefix else None, clear_rest=True)
+    return {name: t.tolist() for name, t in outs.items()}, table.tolist()
+
+
+@pytest.mark.parametrize("tokens", [5, 6, 3000])
+def test_slots_behind_the_last_token_are_cleared(kernels, tokens):
+    outs, _ = place_cleared(kernels, [16, 3], [2, 3], [1, 1], 16, tokens, [8, 9], prefix=None)
+    assert outs["status"] == [1] and outs["q_start"] == [0, 2, 5] and outs["slot_map"][:2] == [128, 129]
+    assert outs["slot_map"][5:] == [-1] * (tokens - 5) and outs["positions"][5:] == [-99] * (tokens - 5)
+
+
+@pytest.mark.parametrize("why,changes", [(-1, dict(free=[])), (-1, dict(cursor=5)), (-2, dict(lengths=[16, 200], held=[1, 13])), (-3, dict(tokens=4)),
+                                         (-4, dict(lengths=[16, -3])), (-4, dict(lengths=[0, 48], held=[0, 3], prefix=[1, 2, 3]))])
+def test_a_step_that_cannot_be_laid_out_brings_nothing(kernels, why, changes):
+    arguments = dict(lengths=[16, 3], counts=[2, 3], held=[1, 1], page=16, tokens=2500, free=[8, 9], cursor=0)
+    arguments.update(changes)
+    outs, table = place_cleared(kernels, **arguments)
+    assert outs["status"] == [why] and outs["q_start"] == [0, 0, 0] and outs["slot_map"] == [-1] * arguments["tokens"]
+    assert outs["seq_lens"] == arguments["lengths"] and outs["held_after"] == arguments["held"] and outs["cursor_after"] == [arguments["cursor"]]
+    assert table == [[-1] * 9] * 2
+
+
+def test_cleared_layouts_of_nobody(kernels):
+    outs, _ = place_cleared(kernels, [], [], [], 16, 4, [8, 9])
+    assert outs["status"] == [0] and outs["q_start"] == [0] and outs["slot_map"] == [-1] * 4
+    outs, _ = place_cleared(kernels, [], [], [], 16, 4, [8, 9], cursor=3)
+    assert outs["status"] == [-1] and outs["q_start"] == [0] and outs["slot_map"] == [-1] * 4 and outs["cursor_after"] == [3]
+
+
+def test_rounds_of_changing_counts(kernels):
+    """Rounds whose counts change and one that brings more than there is room for, nothing read back, eagerly and recorded: the pages hold
+    what the host puts there, and the refused round leaves pages, output and lengths alone."""
+    heads, kv_heads, dim, page, requests, places, shared, vocab = 4, 2, 64, 16, 4, 4, 32, 300
+    generator = torch.Generator().manual_seed(31)
+    normal = lambda *shape: torch.randn(shape, generator=generator)
+    pool, tokens = 14, requests * places
+    pages = normal(pool, kv_heads, page, dim), normal(pool, kv_heads, dim, page)
+    counts = [[4, 4, 4, 4], [1, 3, 0, 4], [4, 1, 4, 0], [60, 60, 60, 60], [0, 2, 1, 3], [0, 0, 0, 0], [2, 1, 4, 1]]      # (the fourth has no room)
+    rounds = [dict(q=2 * normal(tokens, heads * dim), k=normal(tokens, kv_heads, dim), v=normal(tokens, kv_heads, dim),
+                   logits=normal(tokens, vocab), fed=torch.randint(0, vocab, (tokens,), generator=generator, dtype=torch.int32),
+                   counts=torch.tensor(c, dtype=torch.int32)) for c in counts]
+    start = dict(lengths=ints([shared] * requests), held=ints([0] * requests), cursor=ints([0]), table=torch.full((requests, 8), -1, dtype=torch.int32, device=DEV),
+                 k_pages=pages[0].to(DEV), v_pages=pages[1].to(DEV))
+    at = {name: t.clone() for name, t in start.items()}
+    inputs = {name: t.to(DEV) for name, t in rounds[0].items()}
+    free, prompt, heat = ints(list(range(2, pool))), ints([0, 1]), torch.zeros(requests, device=DEV)
+    empty = lambda n: torch.zeros(n, dtype=torch.int32, device=DEV)
+    made = dict(q_start=empty(requests + 1), seq_lens=empty(requests), held_after=empty(requests), cursor_after=empty(1), positions=empty(tokens),
+                seq_of_token=empty(tokens), slot_map=empty(tokens), status=empty(1))
+    out, kept, chosen = torch.zeros_like(inputs["q"]), empty(requests), torch.zeros(requests, places, dtype=torch.int32, device=DEV)
+    numbers = torch.rand(requests, places, generator=generator).to(DEV)
+
+    def one_round():
+        kernels.place_tokens(at["lengths"], inputs["counts"], at["held"], free, at["cursor"], at["table"], page, *made.values(), prefix_pages=prompt, clear_rest=True)
+        kernels.kv_write(inputs["k"], inputs["v"], made["slot_map"], at["k_pages"], at["v_pages"])
+        kernels.attention_shared_prefix(inputs["q"], at["k_pages"], at["v_pages"], at["table"], made["q_start"], made["seq_lens"], shared, heads, kv_heads, dim,
+                                        dim ** -0.5, out, max_seq_len=8 * page, max_new_tokens=places, prefix_pages=prompt)
+        kernels.verify_drafts(inputs["logits"], inputs["fed"], made["q_start"], heat, numbers, kept, chosen)
+        at["lengths"].copy_(made["seq_lens"])
+        at["held"].copy_(made["held_after"])
+        at["cursor"].copy_(made["cursor_after"])
+
+    def run(step):
+        for name, t in start.items():
+            at[name].copy_(t)
+        for t in (out, kept, chosen):
+            t.fill_(7)
+        results = []
+        for one in rounds:
+            for name, t in one.items():
+                inputs[name].copy_(t)
+            out.fill_(7)
+            step()
+            results.append({name: t.clone() for name, t in dict(at, out=out, kept=kept, chosen=chosen, **made).items()})
+        return results
+
+    eager = run(one_round)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        one_round()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        one_round()
+    for _ in range(2):
+        for a, b in zip(eager, run(graph.replay)):
+            for name in a:
+                if name not in ("positions", "seq_of_token"):      # (behind the last token they are those of earlier rounds)
+                    assert torch.equal(a[name], b[name]), name
+
+    lengths, held, cursor, table = [shared] * requests, [0] * requests, 0, [[-1] * 8 for _ in range(requests)]
+    k, v = pages[0].clone(), pages[1].clone()
+    for number, (one, brings, got) in enumerate(zip(rounds, counts, eager)):
+        if number == 3:
+            assert int(got["status"]) < 0 and bool((got["out"] == 7).all())
+            assert got["kept"].tolist() == [0] * requests and bool((got["chosen"] == -1).all())
+        else:
+            placed = rounds_plain.place(lengths, brings, held, list(range(2, pool)), cursor, table, page, list(range(requests)), [0, 1])
+            lengths, held, cursor = placed["seq_lens"], placed["held_after"], placed["cursor_after"][0]
+            for n, slot in enumerate(placed["slot_map"]):
+                k[slot // page, :, slot % page] = one["k"][n]
+                v[slot // page, :, :, slot % page] = one["v"][n]
+            brought = sum(brings)
+            assert got["slot_map"].tolist() == placed["slot_map"] + [-1] * (tokens - brought)
+            assert bool((got["out"][brought:] == 7).all()) and bool(got["out"][:brought].isfinite().all())
+            case = dict(q=one["q"][:brought], k=k, v=v, table=torch.tensor(table, dtype=torch.int32), starts=placed["q_start"], lengths=lengths,
+                        heads=heads, kv_heads=kv_heads, dim=dim, page=page, shared=shared, scale=dim ** -0.5)
+            if brought:
+                within(kernels, case, got["out"][:brought])
+        assert torch.equal(got["k_pages"].cpu(), k) and torch.equal(got["v_pages"].cpu(), v)
+        assert got["lengths"].tolist() == lengths and got["held"].tolist() == held and got["cursor"].tolist() == [cursor]
