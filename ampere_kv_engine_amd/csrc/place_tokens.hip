@@ -185,7 +185,8 @@ __global__ __launch_bounds__(kThreads) void place_kernel(Place p) {
                    : had_of[r] < 0 ? p.prefix_pages[at] : p.table[static_cast<size_t>(row_of[r]) * p.table_width + at];
     p.positions[i] = position;
     p.seq_of_token[i] = r;
-    p.slot_map[i] = id < 0 ? -1 : id * p.page_size + inside;
+    const long slot = static_cast<long>(id) * p.page_size + inside;      // (beyond 31 bits it would be another page's)
+    p.slot_map[i] = id < 0 || slot > 0x7fffffffL ? -1 : static_cast<int>(slot);
   }
   if (p.clear_rest != 0)
     for (int i = tokens + begin; i < p.tokens; i += stride) p.slot_map[i] = -1;

@@ -269,7 +269,8 @@ class RoundKernels:
         by one request at most - other batches are refused (-4), those outside the batch nobody sees.  (A request that is to have no
         part of the prompt goes into a call without prefix_pages.)
         q_start [requests + 1], seq_lens [requests] (the tokens held after the step); positions, seq_of_token and slot_map [tokens]: of
-        every token, request by request; tokens are all that the requests bring, or more: entries behind the last are left as they are.
+        every token, request by request; tokens are all that the requests bring, or more: entries behind the last are left as they are.  A
+        token whose page is negative, or so far that its slot does not fit 31 bits, has slot -1.
         status [1]: the pages taken, or, with nothing else written, -1 too few free pages, -2 a row that the table does not have, that is too
         narrow or that two requests name, -3 more tokens than the maps have room for, -4 a negative number, fewer pages than a length
         fills, or a request that brings places of the prompt's pages beside one that has pages, starts behind the prompt or brings the same

@@ -300,3 +300,12 @@ def test_rounds_of_changing_counts(kernels):
                 within(kernels, case, got["out"][:brought])
         assert torch.equal(got["k_pages"].cpu(), k) and torch.equal(got["v_pages"].cpu(), v)
         assert got["lengths"].tolist() == lengths and got["held"].tolist() == held and got["cursor"].tolist() == [cursor]
+
+
+def test_slots_that_do_not_fit_are_none(kernels):
+    """The last slot of 31 bits, the first behind it, and pages whose slots would come round to others' again."""
+    fits = 2 ** 31 // 16 - 1
+    outs, _ = place_cleared(kernels, [15, 0, 0, 0], [2, 16, 1, 1], [1, 0, 0, 0], 16, 20, [fits, fits, 2 ** 28, 2 ** 31 - 1])
+    assert outs["status"] == [4]
+    assert outs["slot_map"] == [-1, 16 * fits] + list(range(16 * fits, 16 * fits + 16)) + [-1, -1]
+    assert max(outs["slot_map"]) == 2 ** 31 - 1
