@@ -7,6 +7,7 @@ import pytest
 import torch
 
 from ampere_kv_engine_amd.kernels.hip import KernelError
+from ampere_kv_engine_amd.kernels.hip_rounds import cut_own, cut_prefix
 from plain import rounds_plain
 from test_rounds_gpu import attend, batch, drafted, ints, kernel_set, kernels, place_both, tiled, within  # noqa: F401  (fixtures among them)
 
@@ -89,6 +90,49 @@ def test_values_near_the_largest(tiled, dtype):
     case["k"][case["table"][0, 60:].clamp(min=0).long()] = 3.0         # scores of 24, weights of 2^34 beside those of the first keys
     case["v"] *= 2.0 ** 100
     within(tiled, case, attend(tiled, case))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads,kv_heads,shared,counts", [
+    (32, 32, 5200, (1, 2)),             # segments of 12 stages of 64 keys, the last of 9 and a half steps of 32 and 16 keys more
+    (64, 64, 4000, (2, 0, 1)),          # 16 stages, the last segment 29 steps
+    (64, 64, 4144, (1, 1)),             # 18 stages, the last segment 21 steps and 16 keys
+    (128, 128, 2992, (1,)),             # 24 stages, the last segment 45 steps and 16 keys
+    (64, 8, 12288, (10, 10, 10, 10)),   # two tiles of 256 columns, the second with 64
+], ids=lambda v: str(v).replace(" ", ""))
+def test_wide_tiles_go_round_their_rings(kernel_set, dim, heads, kv_heads, shared, counts):
+    """Segments long enough that every slot of the rings is filled again, several times."""
+    rows = sum(counts) * heads // kv_heads
+    segments, keys = cut_prefix(256, rows, kv_heads, shared, kernel_set.compute_units, False)
+    assert keys >= 10 * 64 and segments > 1
+    case = batch(torch.bfloat16, heads, kv_heads, dim, 16, shared, tuple(5 * i for i in range(len(counts))), counts, seed=75 + dim)
+    kernel_set.wide_prefix_tiles = True
+    try:
+        within(kernel_set, case, attend(kernel_set, case))
+    finally:
+        kernel_set.wide_prefix_tiles = None
+
+
+@pytest.mark.parametrize("scale", [None, 1.0], ids=["mild", "far"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("heads,dim,shared,own,counts,bound", [
+    (2, 64, 26000, (3, 40), (2, 1), 0),                                   # a block a row: more than a hundred segments of the prompt
+    (2, 32, 64, (30000, 9000, 10), (1, 2, 1), 0),                         # the same of own keys
+    (32, 16, 320, (30000,) + (70, 3) * 15 + (500,), (2,) * 32, 0),        # a wave a row, 79 segments and the prompt's
+    (32, 16, 320, (7, 3) * 16, (2,) * 32, 40000),                         # the same where nobody holds what the bound allows
+], ids=["prompt", "own", "own-waves", "bound"])
+def test_joins_of_more_segments_than_lanes(kernels, dtype, scale, heads, dim, shared, own, counts, bound):
+    case = batch(dtype, heads, 1, dim, 16, shared, own, counts, seed=76, scale=scale)
+    changes = {}
+    if bound:
+        table = torch.full((len(counts), bound // 16), -1, dtype=torch.int32)
+        table[:, :case["table"].shape[1]] = case["table"]
+        changes = dict(block_table=table.to(DEV), max_seq_len=bound)
+    most = (bound or max(case["lengths"])) - shared
+    segments = (cut_prefix(32, sum(counts) * heads, 1, shared, kernels.compute_units, dtype == torch.float32)[0]
+                + cut_own(len(counts), max(counts) * heads, 1, most, kernels.compute_units)[0])
+    assert segments > 64 and (sum(counts) * heads >= 8 * kernels.compute_units) == (heads == 32)
+    within(kernels, case, attend(kernels, case, **changes))
 
 
 def test_the_prompt_is_found_without_the_first_request(tiled):
