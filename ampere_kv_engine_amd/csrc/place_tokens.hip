@@ -93,7 +93,7 @@ __global__ __launch_bounds__(kThreads) void place_kernel(Place p) {
         count = brings;
         taken = max(0, need - had);
         if (writes_prompt(held == 0, length, brings)) fault |= 4;
-        else if (held != 0 || brings != 0) fault |= 8;
+        else if (prompt_end > 0 && (held != 0 || brings != 0)) fault |= 8;
         if (row < 0 || row >= p.table_rows || had + taken > p.table_width) {
           fault |= 2;
         } else if (p.rows != nullptr) {
@@ -109,7 +109,12 @@ __global__ __launch_bounds__(kThreads) void place_kernel(Place p) {
       length_of[r] = length;
       row_of[r] = row;
     }
-    if (fault != 0) atomicOr(&wrong, fault);
+    // (one of a wave says so for all: every request of a batch with a prompt has one, and a thousand of them on one word take 2 us)
+    int faults = 0;
+#pragma unroll
+    for (int bit = 1; bit <= 8; bit *= 2)
+      if (__any((fault & bit) != 0)) faults |= bit;
+    if (lane == 0 && faults != 0) atomicOr(&wrong, faults);
     const long token_end = sums_up_to(count), page_end = sums_up_to(taken);      // (64 bits hold any sum of 4,096 requests')
     if (lane == kWave - 1) { of_waves[0][wave] = token_end; of_waves[1][wave] = page_end; }
     __syncthreads();
