@@ -863,13 +863,13 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Args a) {
         for (int e = 0; e < kEach; ++e) sum[e] *= by;
       }
       top = m;
-      const float weight = __builtin_amdgcn_exp2f(one.x - reference);
+      const float weight = __builtin_amdgcn_exp2f(one.x - reference), worth = fmaxf(weight, kLittle);
       total += wave_sum(weight * one.y);
       const int end = min(i0 + kWave, used);
       auto add = [&](int from, int end) {
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-          const float by = fmaxf(__shfl(weight, min(from + u * kStride, end - 1) - i0, kWave), kLittle);
+          const float by = __shfl(worth, min(from + u * kStride, end - 1) - i0, kWave);
           if (from + u * kStride < end) {
 #pragma unroll
             for (int e = 0; e < kEach; ++e) sum[e] = fmaf(by, fetched[u][e], sum[e]);
