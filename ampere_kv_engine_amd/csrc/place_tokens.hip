@@ -12,7 +12,7 @@
 // Nothing but `status` is written where the step cannot be laid out - or, `clear_rest`, a layout in which nobody brings anything: every
 // block finds that out before it writes.
 // What bounds it is latency: a launch (2.8 us), the lengths' reads, the scan's barriers, one dependent read (free list or table) a token:
-// 8 requests 4.2 us, 500 of up to 5 tokens 6.4, 64 prompts of 115,000 tokens together 6.0; a call takes the host 9.
+// 8 requests 4.7 us, 500 of up to 5 tokens 6.6, 64 prompts of 115,000 tokens together 6.4; a call takes the host 9.
 
 #include "common.h"
 #include "api_rounds.h"

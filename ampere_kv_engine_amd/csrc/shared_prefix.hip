@@ -178,7 +178,7 @@ __device__ __forceinline__ float sum_over_halves(float v) {
 // `row0`: the tile's first row of the kv head's, `columns` how many of the 32 are there.  A column sees the keys below `visible`
 // (its lane's), `all_see` the least of them over the tile.  `wanted`: a bit for each column whose results are written.
 // Reads and their latency are what bounds it where there are few columns, 16 KB a step asked for a step ahead: own keys of 64 requests of
-// 328 each, 86 MB, 19 us (4.5 TB/s), of 4 to 2,048 26 us; 8 requests behind 8,192 shared tokens, 42 MB in all, 13.6 us, of which 8 are the
+// 328 each, 86 MB, 19 us (4.5 TB/s), of 4 to 2,048 26 us; 8 requests behind 8,192 shared tokens, 42 MB in all, 13.0 us, of which 8 are the
 // way to the first keys - launch, page, read - and the results' way back.  A block alone on its unit takes 2.8 us a step of its four
 // waves.  With a wave a vector unit and many tiles a step takes 1.4 us: 0.35 of matrix instructions, as much of exponentials, the rest
 // waits for operands whose rows' 32-byte pieces are fetched line by line (`walk_wide` has them in LDS).
@@ -402,8 +402,11 @@ __device__ __forceinline__ void walk(const Args& a, const int* table, int head, 
 // do not wait for each other, and nothing in it depends on what the scores are.  A column's weights are taken below a fixed point,
 // the maximum of the segment's first step, and may grow: bfloat16 and float32 reach to 2^127, and a sum that is divided by another of the
 // same scale loses nothing.  Where a column's weights pass 2^40, its sums are not finite, or there is no such point (nothing but minus
-// infinity, a NaN), the column is done again by `walk`, which keeps a running maximum: what a column gets hangs on nothing beside it.  (A branch that moves the point in
-// the loop costs it half as much again: the compiler then keeps the sums in two sets of registers.)
+// infinity, a NaN), the column is done again by `walk`, which keeps a running maximum: what a column gets hangs on nothing beside it.
+// (A branch that moves the point in the loop costs it half as much again: the compiler then keeps the sums in two sets of registers.)
+// That is dear where it is met - a block does its groups of 32 columns one after the other: 256 columns of 8 heads over 32,768 keys,
+// calls, 77 us, and 173 where every head looks at one key 28 nats above its segment's first 32, 222 where each segment has such a
+// key; 2,560 over 8,192 131 and 353 (in narrow tiles, the same keys, 100 and 253 us).
 // The weights are rounded to bfloat16, once: a second part would cost half the matrix instructions again, and the sum that they are
 // divided by is the sum of the rounded ones, so that what is left is the error of an average over the keys.
 // What bounds it: the matrix cores while it runs, 1.68 us a stage of 64 keys on all units (1.28 PFLOP/s; a large library product has
@@ -802,7 +805,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 4 || D > 128 ? 1 : 2)) void
 // A row - (token, query head) - a wave, four of a token a block, or, SHARE, where there are too few rows to fill the device, a block: its
 // waves then take the segments in turn.  What a row waits for is a chain of reads - whose the token is, what it sees -, so many
 // short waves run beside each other, and the segments that a row is sure to have are on their way meanwhile (20,480 rows of four segments
-// 13.9 -> 12.2 us, 43 MB read and 5 written; 2,048 rows of 33 to 38: 8.8 us for 36 MB).
+// 13.9 -> 12.2 us, 43 MB read and 5 written; 2,048 rows of 33 to 38: 8.9 us for 36 MB).
 template <typename T, bool SHARE>
 __global__ __launch_bounds__(kThreads) void join_kernel(Args a) {
   constexpr int kEach = D <= kWave ? 1 : D <= 2 * kWave ? 2 : 4;    // dims of a lane, kEach in a row (the last lanes may have none)

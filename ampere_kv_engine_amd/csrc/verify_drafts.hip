@@ -13,8 +13,8 @@
 // Everything that is compared with a random number is summed in 64 bits: the draw looks for a place among up to 151,936 cumulative
 // weights, and sums in 32 bits, off by 1e-7, would choose another id for one draw in thirty; off by 1e-13, for none.  The vector units
 // have 64-bit products at the rate of 32-bit ones, so that the exponentials cost nine operations each and not much more time than
-// the reads: 64 requests of five rows and four draft rows of 151,936 logits (350 MB) take 73 us, 4.8 TB/s of the 6.2 that plain reads
-// reach, and the second launch, which reads two rows of each request again (78 MB), 29 us; a single request 5.6 and 6.2 us, which are a
+// the reads: 64 requests of five rows and four draft rows of 151,936 logits (350 MB) take 75 us, 4.7 TB/s of the 6.2 that plain reads
+// reach, and the second launch, which reads two rows of each request again (78 MB), 30 us; a single request 5.3 and 6.5 us, which are a
 // launch's way to the first data and back.  Two parts a block: with one the first launch takes 78 us (its ends are paid twice as often),
 // while parts of twice the size cost the second launch 17 us more, since one block ends with a whole part.
 

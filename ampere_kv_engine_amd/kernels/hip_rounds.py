@@ -29,10 +29,12 @@ def wide_tiles_fit(head_dim: int, page_size: int, dtype) -> bool:
 def wide_tiles(rows: int, kv_heads: int, shared: int, units: int) -> bool:
     """Whether the prompt's keys are multiplied in tiles of 256 columns that share them through LDS (`wide_prefix_kernel`, a launch of its
     own) rather than of 32 beside the requests' own keys.  The shared ones cost 8 to 10 us more at their start and end and less a column
-    and key.  Whole calls, narrow / wide us, 256 units, 64 own keys: 32 heads over 8 of 128, 32,768 shared, 64 rows 38 / 52, 96 49 / 51, 112
+    and key.  (Whole calls, narrow / wide us, 256 units, 64 own keys: 32 heads over 8 of 128, 32,768 shared, 64 rows 38 / 52, 96 49 / 51, 112
     57 / 53; 16,000 shared, 160 rows 42 / 43, 192 49 / 45, 256 57 / 49; 8,192 shared, 256 rows 35 / 42, 320 42 / 42; 2,048 shared, 960 rows
     36 / 43, 1,280 53 / 46; 16 over 4 of 64, 32,768 shared, 128 rows 24 / 29, 192 33 / 31, 256 40 / 33.  Two tiles of 32 wait
-    for reads however long the prompt: 131,072 shared, 64 rows 139 / 148, 80 186 / 155."""
+    for reads however long the prompt: 131,072 shared, 64 rows 139 / 148, 80 186 / 155.  A product of rows and keys does not know how many
+    segments they make: of these points two lie on its wrong side, 32,768 shared with 96 rows (wide, 2 us more than narrow) and 2,048
+    shared with 1,280 rows (narrow, 7 us more than wide).)"""
     return rows > 64 and rows * kv_heads * shared >= 85_000 * units
 
 
