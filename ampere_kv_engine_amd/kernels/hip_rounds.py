@@ -195,7 +195,7 @@ class RoundKernels:
         if num_pages == 0:
             raise self._error("there are no pages")
         group = q_heads // kv_heads
-        max_new_tokens = min(max_new_tokens, tokens)
+        max_new_tokens, max_seq_len = min(max_new_tokens, tokens), min(max_seq_len, 2 ** 30)       # (nobody brings or holds more)
         wide = not two_part_weights and wide_tiles_fit(head_dim, page_size, q.dtype) and (
             self.wide_prefix_tiles if self.wide_prefix_tiles is not None else wide_tiles(tokens * group, kv_heads, shared, self.compute_units))
         of_segment = 4 * tokens * q_heads * (head_dim + 2)
@@ -268,8 +268,9 @@ class RoundKernels:
         row of `table` (row r, or rows[r]), and held_after [requests] and cursor_after [1] say what is held and taken then.  A request
         that holds no page starts on `prefix_pages`, if they are given: they are entered too, and `lengths` counts their tokens.  What it
         brings at places within them is written into them: so a prompt is filled, by a batch none of whose requests has it yet, a place
-        by one request at most - other batches are refused (-4), those outside the batch nobody sees.  (A request that is to have no
-        part of the prompt goes into a call without prefix_pages.)
+        by one request at most - other batches are refused (-4), those outside the batch nobody sees.  (Where some requests of a batch start on
+        the prompt and others without one, the caller enters its pages into the rows of the former, counts them in `held`, and gives no
+        prefix_pages.)
         q_start [requests + 1], seq_lens [requests] (the tokens held after the step); positions, seq_of_token and slot_map [tokens]: of
         every token, request by request; tokens are all that the requests bring, or more: entries behind the last are left as they are.  A
         token whose page is negative, or so far that its slot does not fit 31 bits, has slot -1.

@@ -79,3 +79,15 @@ def test_attention_refuses_pages_of_a_prompt_that_are_too_few():
         with pytest.raises(KernelError):
             kernels.attention_shared_prefix(**attention(prefix_pages=pages))
     assert len(kernels.calls) == 3
+
+
+def test_bounds_beyond_31_bits_are_no_bounds():
+    """A table of pages so long that its width in tokens does not fit the lengths' type."""
+    q = torch.zeros(5, 16)
+    kernels = Recorder()
+    kernels.attention_shared_prefix(**attention(q=q, out=torch.zeros_like(q), q_heads=1, kv_heads=1, head_dim=16, k_pages=torch.zeros(1, 1, 1 << 20, 16),
+                                                v_pages=torch.zeros(1, 1, 16, 1 << 20), block_table=torch.zeros(3, 4097, dtype=torch.int32),
+                                                shared=1 << 20, max_seq_len=1 << 32, max_new_tokens=1 << 40))
+    max_own, max_new, _, _, own_segments, own_keys = kernels.calls[0][-8:-2]
+    assert max_own == (1 << 30) - (1 << 20) and max_new == 5
+    assert own_segments <= 256 and own_segments * own_keys >= max_own and (1 << 30) + own_keys < 2 ** 31
